@@ -503,6 +503,61 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
                           int64_t num_segments, int num_heads, int head_dim, float scale,
                           int dtype, void *stream);
 
+/*
+ * Caches held in 8 bits: K and V pools of e4m3 elements (OCP FP8: 448 the largest, no
+ * infinities) in the 16-bit pools' shape and layout, and one fp32 scale per (block, head) for
+ * each, kv_scales [num_blocks][num_heads][2] (K's, V's).  An element stands for itself times
+ * its block's and head's scale.  Pools 16-byte aligned; dtype is that of the 32- or 16-bit
+ * operands beside them.  No vllm_cpu_attn counterpart.
+ *
+ * vfl_reshape_and_cache_8bit: vfl_reshape_and_cache into such a cache, same slots and strides.
+ * Consecutive tokens whose slots lie in one block are a run; a block's tokens must form one
+ * run of the call, and a block belong to one sequence (a second run in the call, or a call
+ * that overlaps this one on another stream, would race for the block's scale).  Per run
+ * and head, for K and for V,
+ *   new = max(old, the smallest power of two with max |x| / new <= 448)   (2^-100 at least)
+ * where max is over the run's finite values and old = 0 when the run holds the block's first
+ * slot: the block then starts over, and its other slots become 0.  Else they become rnd(q *
+ * old / new).  A token's elements are rnd(x / new), to nearest even, NaN for an infinity or
+ * a NaN.  At most 2^31 - 1 tokens and 65535 heads.
+ *
+ * vfl_attention_with_kv_cache_8bit: vfl_attention_with_kv_cache over such a cache; groups
+ * (group_start) are rows sharing one table, at most 8 of them, block_table lists
+ * max_blocks_per_seq blocks a row (longer contexts are clamped to that).  query and out
+ * share dtype; out contiguous.  Sums and softmax in fp32, the weights kept to 2^-17 (fp32:
+ * 2^-25) through the product with V.
+ */
+int vfl_reshape_and_cache_8bit(const void *key, const void *value, int64_t key_stride_token,
+                               int64_t key_stride_head, int64_t value_stride_token,
+                               int64_t value_stride_head, void *k_cache, void *v_cache,
+                               float *kv_scales, const int64_t *slot_mapping, int64_t num_tokens,
+                               int num_heads, int head_dim, int block_size, int64_t num_blocks,
+                               int dtype, void *stream);
+int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_token,
+                                     int64_t query_stride_head, const void *k_cache,
+                                     const void *v_cache, const float *kv_scales, void *out,
+                                     const int32_t *seq_lens, const int32_t *block_table,
+                                     int64_t block_table_stride, int64_t max_blocks_per_seq,
+                                     const int32_t *group_start, const int32_t *group_order,
+                                     int64_t num_rows, int64_t num_groups, int num_heads,
+                                     int head_dim, int block_size, int64_t num_blocks,
+                                     float scale, int dtype, void *stream);
+
+/*
+ * Log probabilities of given tokens, entropy and best alternatives (no vllm_cpu_attn
+ * counterpart).  Per row r of `logits` ([rows][vocab], row stride in elements), with
+ * p = softmax of the row in fp32:
+ *   logprobs[r][i] = log p(tokens[r][i]) for i < num_tokens (NaN for a token outside
+ *                    [0, vocab)); tokens DEVICE int64 [rows][num_tokens]
+ *   entropy[r]     = -sum p log p
+ *   top_logprobs[r][j], top_ids[r][j], j < k: the k best by (logit, then lower id), best first
+ * A row that holds a NaN or +inf, or nothing above -inf, gets NaN throughout and ids -1.
+ * 0 <= k <= min(20, vocab).
+ */
+int vfl_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int vocab, int dtype,
+                       const int64_t *tokens, int num_tokens, int k, float *logprobs,
+                       float *entropy, float *top_logprobs, int64_t *top_ids, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

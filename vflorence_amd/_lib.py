@@ -45,6 +45,9 @@ EXPORTED_SYMBOLS = (
     "vfl_linear_residual",
     "vfl_linear_norm",
     "vfl_layer_norm_apply",
+    "vfl_reshape_and_cache_8bit",
+    "vfl_attention_with_kv_cache_8bit",
+    "vfl_token_logprobs",
 )
 
 
@@ -149,6 +152,20 @@ _SIGNATURES = {
     "vfl_layer_norm_apply": (
         ctypes.c_int,
         [_vp, _i64, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i32, _i32, _vp],
+    ),
+    "vfl_reshape_and_cache_8bit": (
+        ctypes.c_int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64,
+         _i32, _vp],
+    ),
+    "vfl_attention_with_kv_cache_8bit": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32,
+         _i32, _i32, _i64, _f32, _i32, _vp],
+    ),
+    "vfl_token_logprobs": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp],
     ),
 }
 

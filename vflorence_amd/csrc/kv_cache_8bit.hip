@@ -1,0 +1,292 @@
+// Appending keys and values to a paged cache held in e4m3, one scale per (block, head) for
+// K and one for V (gfx950).
+//
+// A run is the consecutive tokens of a call whose slots lie in one block.  Per run and head
+//   a = max |x| over the run's finite values,  need = the smallest power of two with
+//   a / need <= 448,  new = max(old, need)  (old = 0 where the run holds the block's offset
+//   0: the block starts over, what it held is dropped)
+//   held bytes <- rne(held * old / new),  the run's tokens <- rne(x / new)
+// Powers of two make x / new exact, so each value is rounded once, and a block whose scale
+// grows later loses nothing but what falls under e4m3's smallest step: no value's error
+// grows with the number of appends, which any other scale would cost.  Infinities and NaN
+// become NaN and leave the scale alone.
+#include <stdio.h>
+
+#include "e4m3.h"
+
+namespace vfl {
+
+int check_8bit_cache(const char *who, int dtype, int num_heads, int head_dim, int block_size,
+                     int64_t num_blocks) {
+  if (dtype != VFL_FLOAT32 && dtype != VFL_BFLOAT16 && dtype != VFL_FLOAT16) {
+    set_error("%s: unsupported dtype code %d", who, dtype);
+    return VFL_E_INVALID;
+  }
+  if (num_heads <= 0 || num_heads > 65535 || num_blocks < 0) {
+    set_error("%s: bad sizes (heads %d blocks %lld)", who, num_heads, (long long)num_blocks);
+    return VFL_E_INVALID;
+  }
+  if (!vfl_get_isa(dtype, block_size, head_dim)) {
+    set_error("%s: no kernel for block_size %d, head_dim %d", who, block_size, head_dim);
+    return VFL_E_UNSUPPORTED;
+  }
+  return VFL_OK;
+}
+
+// N consecutive elements as fp32 (16-byte loads, 8-byte ones for four 16-bit elements,
+// where the rows are aligned for them).
+template <int DT, bool ALIGNED, int N>
+__device__ __forceinline__ void load_elems(const typename Elem<DT>::T *p, float *f) {
+  if constexpr (!ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (DT == VFL_FLOAT32) f[i] = p[i];
+      else f[i] = Mfma<DT>::widen(p[i]);
+    }
+  } else if constexpr (DT == VFL_FLOAT32 || N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += Elem<DT>::VEC)
+      unpack16<DT>(*reinterpret_cast<const uint4 *>(p + i), f + i);
+  } else {
+    static_assert(N == 4, "a 16-bit quad");
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    f[0] = Mfma<DT>::widen_lo(u.x), f[1] = Mfma<DT>::widen_hi(u.x);
+    f[2] = Mfma<DT>::widen_lo(u.y), f[3] = Mfma<DT>::widen_hi(u.y);
+  }
+}
+
+// |x|, or 0 for an infinity or a NaN (which `x` then becomes).
+__device__ __forceinline__ float finite_abs(float &x) {
+  const float a = fabsf(x);
+  if (a < INFINITY) return a;
+  x = __uint_as_float(0x7fc00000u);
+  return 0.f;
+}
+
+__device__ __forceinline__ float wave_max64(float x) {
+  x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
+  x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
+  x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
+  x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
+  return rows_max4(x);
+}
+
+// A workgroup takes the runs that begin among `window` tokens, for one head; its NS waves
+// take 64 dims each and share the maxima through LDS.  PARTS: 16-token parts of a block.
+// K: lane = (token l / 4 of a part, dims 16 (l % 4) ..), a row's 16 values per 16-byte
+// store.  V: lane = (tokens 4 (l / 16) .. + 3, dims 4 (l % 16) .. + 3), whose 16 bytes lie
+// together in the token-interleaved pool.
+template <int DT, bool ALIGNED, int NS, int PARTS>
+__global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
+    const typename Elem<DT>::T *__restrict__ key, const typename Elem<DT>::T *__restrict__ value,
+    int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, uint8_t *__restrict__ kc,
+    uint8_t *__restrict__ vc, float *__restrict__ scales, const int64_t *__restrict__ slots,
+    int64_t T, int H, int D, int64_t num_blocks, int window) {
+  constexpr int BS = 16 * PARTS;
+  __shared__ float s_max[2][NS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.y;
+  const int64_t t0 = (int64_t)blockIdx.x * window;
+  const int kd = 64 * wave + 16 * (lane & 3), vd = 64 * wave + 4 * (lane & 15);
+  const bool k_in = kd < D, v_in = vd < D;
+
+  // block of a slot, -1 for a slot that is skipped
+  auto block_of = [&](int64_t slot) {
+    return slot >= 0 && slot < num_blocks * BS ? slot / BS : (int64_t)-1;
+  };
+  // first tokens of runs, one lane per token of the window
+  const int64_t tl = t0 + lane;
+  const bool mine = lane < window && tl < T;
+  const int64_t bl = mine ? block_of(slots[tl]) : -1;
+  const int64_t before = mine && tl > 0 ? block_of(slots[tl - 1]) : -1;
+  uint64_t leaders = __builtin_amdgcn_ballot_w64(bl >= 0 && bl != before);
+
+  for (; leaders; leaders &= leaders - 1) {
+    const int64_t t = t0 + __builtin_ctzll(leaders);
+    const int64_t blk = block_of(slots[t]);
+    // lane o: the run's token that takes the block's offset o (its last one), from t on
+    int src = -1;
+    for (int64_t base = t;; base += 64) {
+      const int64_t s = base + lane < T ? slots[base + lane] : -1;
+      const uint64_t same = __builtin_amdgcn_ballot_w64(block_of(s) == blk);
+      const int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
+      const int off = (int)(s & (BS - 1));
+      for (int i = 0; i < n; ++i)
+        if (__builtin_amdgcn_readlane(off, i) == lane) src = (int)(base - t) + i;
+      if (n < 64) break;
+    }
+    const bool fresh = __builtin_amdgcn_readlane(src, 0) >= 0;
+    float *sc = scales + 2 * (blk * H + h);
+    const float old_k = fresh ? 0.f : sc[0], old_v = fresh ? 0.f : sc[1];
+
+    float kx[PARTS][16], vx[PARTS][4][4];
+    int ks[PARTS], vs[PARTS][4];
+    float km = 0.f, vm = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      ks[p] = __shfl(src, 16 * p + (lane >> 2));
+      if (ks[p] >= 0 && k_in) {
+        load_elems<DT, ALIGNED, 16>(key + (t + ks[p]) * k_st + h * k_sh + kd, kx[p]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) km = fmaxf(km, finite_abs(kx[p][i]));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vs[p][j] = __shfl(src, 16 * p + 4 * (lane >> 4) + j);
+        if (vs[p][j] >= 0 && v_in) {
+          load_elems<DT, ALIGNED, 4>(value + (t + vs[p][j]) * v_st + h * v_sh + vd, vx[p][j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vm = fmaxf(vm, finite_abs(vx[p][j][i]));
+        }
+      }
+    }
+    km = wave_max64(km);
+    vm = wave_max64(vm);
+    if constexpr (NS > 1) {
+      __syncthreads();  // the previous run's maxima have been read
+      if (lane == 0) s_max[0][wave] = km, s_max[1][wave] = vm;
+      __syncthreads();  // and every wave has read the old scales
+#pragma unroll
+      for (int w = 0; w < NS; ++w) km = fmaxf(km, s_max[0][w]), vm = fmaxf(vm, s_max[1][w]);
+    }
+    const float new_k = fmaxf(old_k, e4m3_scale(km)), new_v = fmaxf(old_v, e4m3_scale(vm));
+    const bool all_k = fresh || new_k != old_k, all_v = fresh || new_v != old_v;
+    const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
+    const float ratio_k = old_k * inv_k, ratio_v = old_v * inv_v;
+
+    uint8_t *kt = kc + (blk * H + h) * (int64_t)(BS * D), *vt = vc + (blk * H + h) * (int64_t)(BS * D);
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      uint4 *row = reinterpret_cast<uint4 *>(kt + (16 * p + (lane >> 2)) * D + kd);
+      if (k_in && (ks[p] >= 0 || all_k)) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (ks[p] >= 0) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) kx[p][i] *= inv_k;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = e4m3_pack(kx[p] + 4 * i);
+        } else if (!fresh) {
+          const uint4 u = *row;
+          w[0] = e4m3_rescale(u.x, ratio_k), w[1] = e4m3_rescale(u.y, ratio_k);
+          w[2] = e4m3_rescale(u.z, ratio_k), w[3] = e4m3_rescale(u.w, ratio_k);
+        }
+        *row = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      const bool any = vs[p][0] >= 0 || vs[p][1] >= 0 || vs[p][2] >= 0 || vs[p][3] >= 0;
+      if (v_in && (any || all_v)) {
+        uint4 *group = reinterpret_cast<uint4 *>(vt + ((4 * p + (lane >> 4)) * D + vd) * 4);
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (!fresh) {
+          const uint4 u = *group;
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+          if (all_v) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = e4m3_rescale(w[i], ratio_v);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (vs[p][j] < 0) continue;
+          float f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = vx[p][j][i] * inv_v;
+          const uint32_t u = e4m3_pack(f);  // dim i's value of token j
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = (w[i] & ~(0xffu << (8 * j))) | (((u >> (8 * i)) & 0xffu) << (8 * j));
+        }
+        *group = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (threadIdx.x == 0) {
+      if (all_k) sc[0] = new_k;
+      if (all_v) sc[1] = new_v;
+    }
+  }
+}
+
+template <int DT, bool ALIGNED, int PARTS, typename... A>
+static void launch_append_steps(int steps, dim3 grid, hipStream_t stream, A... a) {
+#define VFL_APPEND(NS) \
+  append_8bit_kernel<DT, ALIGNED, NS, PARTS><<<grid, dim3(64 * NS), 0, stream>>>(a...)
+  switch (steps) {
+    case 1: VFL_APPEND(1); break;
+    case 2: VFL_APPEND(2); break;
+    case 3: VFL_APPEND(3); break;
+    case 4: VFL_APPEND(4); break;
+    default: VFL_APPEND(8); break;  // head size 512
+  }
+#undef VFL_APPEND
+}
+
+template <int DT>
+static int launch_append(bool aligned, const void *key, const void *value, int64_t k_st,
+                         int64_t k_sh, int64_t v_st, int64_t v_sh, void *kc, void *vc,
+                         float *scales, const int64_t *slots, int64_t T, int H, int D, int BS,
+                         int64_t num_blocks, hipStream_t stream) {
+  using E = typename Elem<DT>::T;
+  const int window = 1;
+  const dim3 grid((unsigned)((T + window - 1) / window), (unsigned)H);
+  const int steps = (D + 63) / 64;
+  auto go = [&](auto al, auto parts) {
+    launch_append_steps<DT, decltype(al)::value, decltype(parts)::value>(
+        steps, grid, stream, (const E *)key, (const E *)value, k_st, k_sh, v_st, v_sh,
+        (uint8_t *)kc, (uint8_t *)vc, scales, slots, T, H, D, num_blocks, window);
+  };
+  using std::integral_constant;
+  if (aligned) {
+    if (BS == 16) go(integral_constant<bool, true>{}, integral_constant<int, 1>{});
+    else go(integral_constant<bool, true>{}, integral_constant<int, 2>{});
+  } else {
+    if (BS == 16) go(integral_constant<bool, false>{}, integral_constant<int, 1>{});
+    else go(integral_constant<bool, false>{}, integral_constant<int, 2>{});
+  }
+  return launch_status("reshape_and_cache_8bit");
+}
+
+}  // namespace vfl
+
+using namespace vfl;
+
+extern "C" int vfl_reshape_and_cache_8bit(const void *key, const void *value,
+                                          int64_t key_stride_token, int64_t key_stride_head,
+                                          int64_t value_stride_token, int64_t value_stride_head,
+                                          void *k_cache, void *v_cache, float *kv_scales,
+                                          const int64_t *slot_mapping, int64_t num_tokens,
+                                          int num_heads, int head_dim, int block_size,
+                                          int64_t num_blocks, int dtype, void *stream) {
+  clear_error();
+  const int st = check_8bit_cache("reshape_and_cache_8bit", dtype, num_heads, head_dim,
+                                  block_size, num_blocks);
+  if (st != VFL_OK) return st;
+  if (num_tokens < 0 || num_tokens > 2147483647LL) {
+    set_error("reshape_and_cache_8bit: %lld tokens", (long long)num_tokens);
+    return VFL_E_INVALID;
+  }
+  if (num_tokens == 0 || num_blocks == 0) return VFL_OK;
+  if (!key || !value || !k_cache || !v_cache || !kv_scales || !slot_mapping) {
+    set_error("reshape_and_cache_8bit: null pointer argument");
+    return VFL_E_INVALID;
+  }
+  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)kv_scales % 4 ||
+      (uintptr_t)slot_mapping % 8 || (uintptr_t)key % elem_bytes(dtype) ||
+      (uintptr_t)value % elem_bytes(dtype)) {
+    set_error("reshape_and_cache_8bit: misaligned pointer (caches 16 bytes, others their "
+              "element)");
+    return VFL_E_INVALID;
+  }
+  const int64_t vec = 16 / elem_bytes(dtype);
+  const bool aligned = (uintptr_t)key % 16 == 0 && (uintptr_t)value % 16 == 0 &&
+                       key_stride_token % vec == 0 && key_stride_head % vec == 0 &&
+                       value_stride_token % vec == 0 && value_stride_head % vec == 0;
+  hipStream_t s = (hipStream_t)stream;
+  auto go = [&](auto dt) {
+    return launch_append<decltype(dt)::value>(
+        aligned, key, value, key_stride_token, key_stride_head, value_stride_token,
+        value_stride_head, k_cache, v_cache, kv_scales, slot_mapping, num_tokens, num_heads,
+        head_dim, block_size, num_blocks, s);
+  };
+  if (dtype == VFL_FLOAT32) return go(std::integral_constant<int, VFL_FLOAT32>{});
+  if (dtype == VFL_BFLOAT16) return go(std::integral_constant<int, VFL_BFLOAT16>{});
+  return go(std::integral_constant<int, VFL_FLOAT16>{});
+}

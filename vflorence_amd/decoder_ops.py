@@ -9,7 +9,9 @@ attention output and cross-attention query projections,
 vflorence/models/bart.py:111,114,142,146); ``linear_fits`` says when it applies.
 ``logprob_topk`` is the device half of sampling (vflorence/engine/model_runner.py:355-398):
 log-softmax, the history-free generation rules and the per-row top-k in one read of
-the logits.  All run on the current stream; CPU tensors are rejected.
+the logits.  ``token_logprobs`` scores given tokens: their log probabilities, each row's
+entropy and its best alternatives.  All run on the current stream; CPU tensors are
+rejected.
 """
 
 from __future__ import annotations
@@ -17,7 +19,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .hip_attn import _dtype_code, _require_gpu, _stream, on_current_device, plain_eager
+from .hip_attn import (_dtype_code, _require_gpu, _stream, on_current_device, on_device,
+                       plain_eager, refuse_gradients)
 
 # largest k of logprob_topk (each lane keeps its k best in registers)
 MAX_K = 16
@@ -518,3 +521,40 @@ def logprob_topk(logits: torch.Tensor, k: int, *, log_softmax: bool,
         ids.data_ptr(), _stream(dev)))
     return scores, ids
 
+
+# largest k of token_logprobs
+MAX_ALTERNATIVES = 20
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
+    """Scores of given tokens: (logprobs, entropy, top_logprobs, top_ids).
+
+    logits: [rows, vocab] in float32, bfloat16 or float16, rows contiguous.  tokens: int64
+    [rows] or [rows, n].  Of each row's ``log_softmax``: ``logprobs`` (float32, tokens' shape)
+    at its tokens, NaN for one outside the vocabulary; ``entropy`` (float32 [rows], in nats);
+    and with k > 0 the k best, best first, equal logits by the lower id: ``top_logprobs``
+    (float32 [rows, k]) and ``top_ids`` (int64 [rows, k]), else None.  A row that holds a NaN
+    or +inf, or nothing above -inf, has NaN throughout and ids -1."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+        raise ValueError(f"tokens must be int64 [{rows}] or [{rows}, n], got {tokens.dtype} "
+                         f"{tuple(tokens.shape)}")
+    if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
+        raise ValueError(f"k must be in [0, min({MAX_ALTERNATIVES}, vocab)], got {k}")
+    dtype = _dtype_code(logits.dtype)
+    dev = _require_gpu(logits, tokens)
+    refuse_gradients("token_logprobs", logits)
+    tokens = tokens.contiguous()
+    logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top = ids = None
+    if k:
+        top = torch.empty(rows, k, dtype=torch.float32, device=dev)
+        ids = torch.empty(rows, k, dtype=torch.int64, device=dev)
+    on_device(logits, lib.vfl_token_logprobs, logits.data_ptr(), logits.stride(0), rows, vocab,
+              dtype, tokens.data_ptr(), tokens.shape[1] if tokens.dim() == 2 else 1, k,
+              logprobs.data_ptr(), entropy.data_ptr(), top.data_ptr() if k else None,
+              ids.data_ptr() if k else None)
+    return logprobs, entropy, top, ids

@@ -785,6 +785,162 @@ def encoder_attention(qkv: torch.Tensor, segments, out: torch.Tensor, num_heads:
     torch.autograd.graph.increment_version(out)  # autograd's check of saved tensors
 
 
+# ---------------------------------------------------------------------------
+# caches held in 8 bits
+# ---------------------------------------------------------------------------
+def kv_cache_8bit(num_blocks: int, num_heads: int, block_size: int, head_dim: int,
+                  device) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A zero-filled paged cache in 8 bits: K and V pools ``[num_blocks, H, block_size, D]``
+    of ``torch.float8_e4m3fn`` and their scales, float32 ``[num_blocks, H, 2]`` (K's, V's).  A
+    value is its e4m3 element times its block's and head's scale.  Pools have the layout of
+    the 16-bit ones (``v_cache_logical`` gives V in token order).  ``copy_blocks`` copies
+    pool blocks, and with an even number of heads their scales (``[scales]``) as well."""
+    if head_dim not in SUPPORTED_HEAD_DIMS or block_size not in SUPPORTED_BLOCK_SIZES:
+        raise ValueError(f"no gfx950 kernel for block_size={block_size} head_dim={head_dim}; "
+                         f"supported head_dim {sorted(SUPPORTED_HEAD_DIMS)}, block_size "
+                         f"{sorted(SUPPORTED_BLOCK_SIZES)}")
+    shape = (num_blocks, num_heads, block_size, head_dim)
+    k_cache, v_cache = (torch.zeros(shape, dtype=torch.uint8, device=device)
+                        .view(torch.float8_e4m3fn) for _ in range(2))
+    return k_cache, v_cache, torch.zeros(num_blocks, num_heads, 2, device=device)
+
+
+def kv_cache_8bit_values(k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         kv_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The float32 keys and values that an 8-bit cache stands for, ``[num_blocks, H,
+    block_size, D]`` in token order."""
+    scales = kv_scales[..., None, None]
+    return (k_cache.float() * scales[:, :, 0],
+            v_cache_logical(v_cache).float() * scales[:, :, 1])
+
+
+def _check_8bit_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: torch.Tensor):
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("k_cache/v_cache must be [num_blocks, H, block_size, D] of one shape")
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise ValueError("an 8-bit cache holds torch.float8_e4m3fn, got "
+                         f"{k_cache.dtype}, {v_cache.dtype}")
+    num_blocks, num_heads, block_size, head_dim = shape = k_cache.shape
+    if kv_scales.dtype != torch.float32 or kv_scales.shape != (num_blocks, num_heads, 2):
+        raise ValueError(f"kv_scales must be float32 [{num_blocks}, {num_heads}, 2], got "
+                         f"{kv_scales.dtype} {tuple(kv_scales.shape)}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and kv_scales.is_contiguous()):
+        raise ValueError("caches and their scales must be contiguous")
+    if block_size not in SUPPORTED_BLOCK_SIZES or head_dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"block_size={block_size}, head_dim={head_dim} has no attention kernel; "
+                         f"supported: {sorted(SUPPORTED_BLOCK_SIZES)}, "
+                         f"{sorted(SUPPORTED_HEAD_DIMS)}")
+    return shape
+
+
+def refuse_gradients(name: str, *tensors: torch.Tensor) -> None:
+    """Raise where autograd would record the call: these kernels have no backward pass."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad()")
+
+
+def on_device(tensor: torch.Tensor, function, *args) -> None:
+    """A checked C-ABI call on ``tensor``'s device and its current stream, the last argument
+    (a null stream handle, every default stream's, means the current device's)."""
+    if on_current_device(tensor):
+        check(function(*args, _stream(tensor.device)))
+    else:
+        with torch.cuda.device(tensor.device):
+            check(function(*args, _stream(tensor.device)))
+
+
+def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, kv_scales: torch.Tensor,
+                           slot_mapping: torch.Tensor) -> None:
+    """``reshape_and_cache`` into an 8-bit cache (``kv_cache_8bit``), in place.
+
+    key/value: [T, H, D] in float32, bfloat16 or float16, any token and head strides, a
+    contiguous last dimension.  slot_mapping: int64 [T]; a token whose slot is negative or
+    past the pool is skipped.  A block's tokens of one call must follow one another in it
+    (as positions of a sequence do), a block appended to must belong to one sequence, and
+    a slot that comes twice takes the later token.
+
+    A block's scale is a power of two that brings its largest value to 448 or less.  It only
+    grows: what the block holds is then rescaled, exactly but for values under e4m3's smallest
+    step.  Writing a block's first slot starts the block over: what it held is dropped.
+    Infinities and NaN are stored as NaN and leave the scale alone."""
+    num_blocks, num_heads, block_size, head_dim = _check_8bit_cache(k_cache, v_cache, kv_scales)
+    if key.dim() != 3 or value.shape != key.shape or key.shape[1:] != (num_heads, head_dim):
+        raise ValueError(f"key/value must be [T, {num_heads}, {head_dim}], got "
+                         f"{tuple(key.shape)}, {tuple(value.shape)}")
+    if key.dtype != value.dtype:
+        raise ValueError("key and value must share one dtype")
+    dtype = _dtype_code(key.dtype)
+    if key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("key/value need a contiguous last dimension")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],):
+        raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
+                         f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
+    _require_gpu(key, value, k_cache, v_cache, kv_scales, slot_mapping)
+    refuse_gradients("reshape_and_cache_8bit", key, value)
+    slot_mapping = slot_mapping.contiguous()
+    on_device(key, lib.vfl_reshape_and_cache_8bit, key.data_ptr(), value.data_ptr(),
+              key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+              k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
+              slot_mapping.data_ptr(), key.shape[0], num_heads, head_dim, block_size, num_blocks,
+              dtype)
+
+
+def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
+                                 v_cache: torch.Tensor, kv_scales: torch.Tensor,
+                                 out: torch.Tensor, seq_lens: torch.Tensor, *, scale: float,
+                                 block_table: torch.Tensor,
+                                 scheduler_metadata: SchedulerMetadata | None = None) -> None:
+    """``attention_with_kv_cache`` over an 8-bit cache (``kv_cache_8bit``), into ``out``.
+
+    query: [N, H, D] in float32, bfloat16 or float16, any token and head strides; out: a
+    contiguous tensor of its shape and dtype.  Row r attends to the first ``seq_lens[r]``
+    tokens (int32, as many as the table lists at most) of the blocks ``block_table[r]`` (int32
+    [N, max_blocks]) lists; a block id outside the pool contributes nothing, and a row
+    without tokens is zero.  Of ``scheduler_metadata`` the row groups (``group_start``,
+    ``group_order``) are used: a group that shares its table is read once for all of its
+    rows, one whose rows keep their own tables runs row by row."""
+    num_blocks, num_heads, block_size, head_dim = _check_8bit_cache(k_cache, v_cache, kv_scales)
+    if query.dim() != 3 or query.stride(2) != 1 or query.shape[1:] != (num_heads, head_dim):
+        raise ValueError(f"query must be [N, {num_heads}, {head_dim}] with a contiguous last "
+                         f"dimension, got {tuple(query.shape)}")
+    num_rows = query.shape[0]
+    dtype = _dtype_code(query.dtype)
+    if out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of query's shape and dtype")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (num_rows,):
+        raise ValueError(f"seq_lens must be int32 [{num_rows}], got {seq_lens.dtype} "
+                         f"{tuple(seq_lens.shape)}")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2
+            or block_table.shape[0] != num_rows):
+        raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
+                         f"{block_table.dtype} {tuple(block_table.shape)}")
+    _require_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
+    refuse_gradients("attention_with_kv_cache_8bit", query, out)
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    start = order = None
+    num_groups = num_rows
+    sm = scheduler_metadata
+    if sm is not None:
+        if (sm.num_heads, sm.head_dim, sm.block_size) != (num_heads, head_dim, block_size):
+            raise ValueError("scheduler_metadata was made for another cache: "
+                             f"H={sm.num_heads}, D={sm.head_dim}, block_size={sm.block_size}")
+        if sm.group_plan is not None and sm.group_plan.folded:
+            raise ValueError("a group plan with copy-on-write folded in is for "
+                             "self_attention_with_kv_write alone")
+        if not sm.own_tables or sm.group_start is None:
+            start, order, num_groups = sm.group_start, sm.group_order, sm.num_groups
+        _require_gpu(query, *(t for t in (start, order) if t is not None))
+    on_device(query, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
+              query.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
+              out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+              block_table.shape[1], None if start is None else start.data_ptr(),
+              None if order is None else order.data_ptr(), num_rows, num_groups, num_heads,
+              head_dim, block_size, num_blocks, float(scale), dtype)
+
+
 def cache_pointer_table(caches: list[torch.Tensor]) -> torch.Tensor:
     """Device int64 tensor of cache base addresses, the ``caches`` argument of copy_blocks."""
     if not caches:
