@@ -552,11 +552,15 @@ int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_tok
  *   entropy[r]     = -sum p log p
  *   top_logprobs[r][j], top_ids[r][j], j < k: the k best by (logit, then lower id), best first
  * A row that holds a NaN or +inf, or nothing above -inf, gets NaN throughout and ids -1.
- * 0 <= k <= min(20, vocab).
+ * 0 <= k <= min(20, vocab); vocab up to 2^20.  workspace: DEVICE memory, 16-byte aligned, of
+ * vfl_token_logprobs_workspace(vocab, dtype, k) bytes a row (0: none needed; rows up to
+ * 57344 fp32 or 65536 16-bit values); calls that may overlap need one each.
  */
+int64_t vfl_token_logprobs_workspace(int vocab, int dtype, int k);
 int vfl_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int vocab, int dtype,
                        const int64_t *tokens, int num_tokens, int k, float *logprobs,
-                       float *entropy, float *top_logprobs, int64_t *top_ids, void *stream);
+                       float *entropy, float *top_logprobs, int64_t *top_ids, void *workspace,
+                       void *stream);
 
 #ifdef __cplusplus
 }

@@ -161,9 +161,9 @@ def test_c_entries_check_before_launch():
         assert append(**bad) == -1 and b"misaligned" in lib.vfl_last_error()
 
     def score(x=A, stride=100, rows=4, vocab=100, dt=1, tokens=A, n=1, k=0, lp=A, ent=A, top=A,
-              ids=A):
+              ids=A, ws=None):
         return lib.vfl_token_logprobs(x, stride, rows, vocab, dt, tokens, n, k, lp, ent, top, ids,
-                                      None)
+                                      ws, None)
 
     assert score(rows=0) == 0
     assert score(dt=5) == -1 and score(vocab=0) == -1 and score(stride=99) == -1
@@ -172,6 +172,12 @@ def test_c_entries_check_before_launch():
     assert score(x=None) == -1 and score(ent=None) == -1 and score(tokens=None) == -1
     assert score(lp=None) == -1 and score(k=2, top=None) == -1 and score(k=2, ids=None) == -1
     assert score(x=A + 1) == -1
+    assert score(vocab=(1 << 20) + 1, stride=1 << 21) == -1
+    assert score(vocab=200000, stride=200000) == -1 and b"null" in lib.vfl_last_error()
+    assert score(vocab=200000, stride=200000, ws=A + 8) == -1
+    assert lib.vfl_token_logprobs_workspace(50265, 0, 20) == 0
+    assert lib.vfl_token_logprobs_workspace(65536, 1, 20) == 0
+    assert lib.vfl_token_logprobs_workspace(200000, 1, 20) == 4 * (16 + 8 * 20)
 
 
 def test_oracle_append_rescales_a_growing_block():

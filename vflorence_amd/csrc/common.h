@@ -272,6 +272,15 @@ __device__ __forceinline__ float rows_sum4(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Maximum over the 64 lanes of a wave.
+__device__ __forceinline__ float wave_max64(float x) {
+  x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
+  x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
+  x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
+  x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
+  return rows_max4(x);
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr float NEG_INF_F = -__builtin_huge_valf();

@@ -63,14 +63,6 @@ __device__ __forceinline__ float finite_abs(float &x) {
   return 0.f;
 }
 
-__device__ __forceinline__ float wave_max64(float x) {
-  x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
-  x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
-  x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
-  x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
-  return rows_max4(x);
-}
-
 // A workgroup takes the runs that begin among `window` tokens, for one head; its NS waves
 // take 64 dims each and share the maxima through LDS.  PARTS: 16-token parts of a block.
 // K: lane = (token l / 4 of a part, dims 16 (l % 4) ..), a row's 16 values per 16-byte
@@ -154,7 +146,8 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
     const float ratio_k = old_k * inv_k, ratio_v = old_v * inv_v;
 
-    uint8_t *kt = kc + (blk * H + h) * (int64_t)(BS * D), *vt = vc + (blk * H + h) * (int64_t)(BS * D);
+    const int64_t tile = (blk * H + h) * (int64_t)(BS * D);
+    uint8_t *kt = kc + tile, *vt = vc + tile;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       uint4 *row = reinterpret_cast<uint4 *>(kt + (16 * p + (lane >> 2)) * D + kd);

@@ -16,6 +16,8 @@ rejected.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ._lib import check, lib
@@ -522,8 +524,14 @@ def logprob_topk(logits: torch.Tensor, k: int, *, log_softmax: bool,
     return scores, ids
 
 
-# largest k of token_logprobs
-MAX_ALTERNATIVES = 20
+MAX_ALTERNATIVES = 20  # largest k of token_logprobs
+MAX_SCORED_VOCAB = 1 << 20  # its longest row
+
+
+@functools.lru_cache(maxsize=None)
+def _logprobs_workspace(vocab: int, dtype: int, k: int) -> int:
+    """Bytes a row of ``vfl_token_logprobs``' workspace."""
+    return lib.vfl_token_logprobs_workspace(vocab, dtype, k)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
@@ -543,6 +551,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
                          f"{tuple(tokens.shape)}")
     if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
         raise ValueError(f"k must be in [0, min({MAX_ALTERNATIVES}, vocab)], got {k}")
+    if not 0 < vocab <= MAX_SCORED_VOCAB:
+        raise ValueError(f"vocab must be in [1, {MAX_SCORED_VOCAB}], got {vocab}")
     dtype = _dtype_code(logits.dtype)
     dev = _require_gpu(logits, tokens)
     refuse_gradients("token_logprobs", logits)
@@ -553,8 +563,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
     if k:
         top = torch.empty(rows, k, dtype=torch.float32, device=dev)
         ids = torch.empty(rows, k, dtype=torch.int64, device=dev)
+    workspace = None
+    need = _logprobs_workspace(vocab, dtype, k)
+    if need:
+        workspace = torch.empty(rows * need, dtype=torch.uint8, device=dev)
     on_device(logits, lib.vfl_token_logprobs, logits.data_ptr(), logits.stride(0), rows, vocab,
               dtype, tokens.data_ptr(), tokens.shape[1] if tokens.dim() == 2 else 1, k,
               logprobs.data_ptr(), entropy.data_ptr(), top.data_ptr() if k else None,
-              ids.data_ptr() if k else None)
+              ids.data_ptr() if k else None, workspace.data_ptr() if need else None)
     return logprobs, entropy, top, ids
