@@ -554,7 +554,7 @@ int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_tok
  * A row that holds a NaN or +inf, or nothing above -inf, gets NaN throughout and ids -1.
  * 0 <= k <= min(20, vocab); vocab up to 2^20.  workspace: DEVICE memory, 16-byte aligned, of
  * vfl_token_logprobs_workspace(vocab, dtype, k) bytes a row (0: none needed; rows up to
- * 57344 fp32 or 65536 16-bit values); calls that may overlap need one each.
+ * 57344 values); calls that may overlap need one each.
  */
 int64_t vfl_token_logprobs_workspace(int vocab, int dtype, int k);
 int vfl_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int vocab, int dtype,

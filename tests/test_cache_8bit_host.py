@@ -176,7 +176,7 @@ def test_c_entries_check_before_launch():
     assert score(vocab=200000, stride=200000) == -1 and b"null" in lib.vfl_last_error()
     assert score(vocab=200000, stride=200000, ws=A + 8) == -1
     assert lib.vfl_token_logprobs_workspace(50265, 0, 20) == 0
-    assert lib.vfl_token_logprobs_workspace(65536, 1, 20) == 0
+    assert lib.vfl_token_logprobs_workspace(57344, 1, 20) == 0
     assert lib.vfl_token_logprobs_workspace(200000, 1, 20) == 4 * (16 + 8 * 20)
 
 

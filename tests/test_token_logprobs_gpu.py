@@ -31,7 +31,8 @@ def check(logits, tokens, k, got):
 
     def near(have, want, tol):
         assert have.dtype == torch.float32
-        same = (have.double() == want) | ((have.double() - want).abs() <= tol)
+        # (a logprob past fp32's range is -inf in fp32)
+        same = (have == want.float()) | ((have.double() - want).abs() <= tol)
         assert same.all(), ((have.double() - want).abs() / tol).nan_to_num(0).max()
 
     tol = off_s + 2.0**-23 * (1 + S.log())
@@ -65,7 +66,7 @@ def case(rows, vocab, dtype, seed=0, std=2.5, pad=0):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [1, 2, 3, 7, 8, 9, 63, 64, 65, 255, 1000, 4097, 12289, 33000,
-                                   50265, 51289, 57329, 65536, 130001, 256000])
+                                   50265, 51289, 57344, 57345, 65536, 130001, 256000])
 def test_vocabularies(dtype, vocab):
     for rows, k in ((3, min(20, vocab)), (2, 0), (1, min(5, vocab))):
         logits, tokens = case(rows, vocab, dtype)
@@ -153,6 +154,40 @@ def test_rows_at_any_alignment(dtype, vocab, offset, pad):
     logits = flat.as_strided((3, vocab), (vocab + pad, 1), offset)
     tokens = torch.randint(0, vocab, (3,), generator=gen).to(DEV)
     check(logits, tokens, 20, score(logits, tokens, 20))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [31, 5001, 50265, 130001])
+@pytest.mark.parametrize("level", [2e38, -2e38, -3.3e38])
+def test_rows_at_the_types_limits(dtype, vocab, level):
+    """Maxima whose product with log2 e overflows: the weight lies on the equal values alone.
+    A row masked throughout with one low value is uniform."""
+    logits, tokens = case(4, vocab, dtype)
+    logits[0] = level
+    logits[1] = torch.where(logits[1] > 0, level, torch.finfo(dtype).min)
+    logits[2] = -math.inf
+    logits[2, vocab // 2:] = level
+    logits[3, tokens[3]] = level
+    got = score(logits, tokens, 5)
+    check(logits, tokens, 5, got)
+    assert abs(float(got[1][0]) - math.log(vocab)) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [3000, 50265, 130001])
+def test_rows_below_zero(dtype, vocab):
+    """Log probabilities themselves, -0.0 and 0.0 among the best, and the same bits again."""
+    logits, tokens = case(5, vocab, dtype)
+    logits.copy_(torch.log_softmax(logits.float(), 1))
+    logits[3:] = logits[3:].clamp(max=-2.0)
+    logits[2, [5, 900, 77]] = torch.tensor([-0.0, 0.0, 0.0], dtype=dtype, device=DEV)
+    logits[4, 100:130:2], logits[4, 101:130:2] = 0.0, -0.0
+    for k in (2, 3, 9):
+        check(logits, tokens, k, score(logits, tokens, k))
+    got = score(logits, tokens, 20)
+    check(logits, tokens, 20, got)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(got, score(logits, tokens, 20)))
 
 
 def test_best_values_side_by_side():

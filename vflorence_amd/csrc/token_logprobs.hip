@@ -18,7 +18,43 @@ constexpr int TLP_MAX_K = 20;
 constexpr int TLP_MAX_VOCAB = 1 << 20;
 constexpr int TLP_CAP = 512;        // candidates for the alternatives kept in LDS
 constexpr int TLP_MAX_SEGMENTS = 64;
-constexpr float TLP_FLOOR = -1e4f;  // exp() is 0 long before
+constexpr float TLP_FLOOR = -1e4f;  // exp2() is 0 long before
+constexpr float TLP_NONE = -3e38f;  // reference of a thread that has seen no value
+// A row whose maximum lies past this has weight on the values equal to it alone (their
+// neighbours are 2^100 away), and its products with log2 e overflow: taken apart.
+constexpr float TLP_EXTREME = 1e38f;
+constexpr float TLP_SLACK = 16.f;  // log2 units a reference may lag behind: sums stay < 2^33
+constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
+
+// Sums of exp2(x log2 e - c) and of its product with the exponent.
+struct Sums {
+  float c, s, w;
+
+  // Move the reference to `to` (or stay, where to == c).
+  __device__ __forceinline__ void move(float to) {
+    const float d = c - to, f = d == 0.f ? 1.f : fast_exp2(d);
+    w = f == 0.f ? 0.f : f * (w + d * s);
+    s *= f;
+    c = to;
+  }
+};
+
+// Sum over the wave, the first lane's for every lane: a product before the first addition is
+// fused into it, which then rounds differently on the two lanes of a pair.
+__device__ __forceinline__ float wave_total(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(group_sum<64>(x))));
+}
+
+// A row's normaliser and what it makes of a value.
+struct Normaliser {
+  float c, log2_s, mx;
+  bool extreme;
+
+  __device__ __forceinline__ float logprob(float x) const {
+    if (extreme || fabsf(x) > TLP_EXTREME) return (x - mx) - LN2_F * log2_s;
+    return LN2_F * (fmaf(x, LOG2E_F, -c) - log2_s);
+  }
+};
 
 template <int DT> __device__ __forceinline__ float logit(typename Elem<DT>::T v) {
   if constexpr (DT == VFL_FLOAT32) return v;
@@ -48,9 +84,51 @@ __device__ __forceinline__ bool ahead(float a, int ia, float b, int ib) {
   return a > b || (a == b && ia < ib);
 }
 
-// One segment's statistics, kept for the join.
+// Whether an element of the vector may reach tau (a NaN may seem to).  16-bit patterns order
+// like their values where they are positive, and against it where negative: packed maxima
+// of signed, or minima of unsigned patterns (which take 0 as -0), instead of eight widened
+// elements.
+template <int DT> __device__ __forceinline__ bool may_reach(const uint4 &u, float tau) {
+  if constexpr (DT == VFL_FLOAT32) {
+    return vector_max<DT>(u) >= tau;
+  } else {
+    typedef short s2_t __attribute__((ext_vector_type(2)));
+    typedef unsigned short u2_t __attribute__((ext_vector_type(2)));
+    const uint32_t bits = Mfma<DT>::narrow(tau == 0.f ? -0.f : tau);
+    if (tau > 0.f) {
+      const s2_t m = __builtin_elementwise_max(
+          __builtin_elementwise_max(__builtin_bit_cast(s2_t, u.x), __builtin_bit_cast(s2_t, u.y)),
+          __builtin_elementwise_max(__builtin_bit_cast(s2_t, u.z), __builtin_bit_cast(s2_t, u.w)));
+      return max(m.x, m.y) >= (short)bits;
+    }
+    const u2_t m = __builtin_elementwise_min(
+        __builtin_elementwise_min(__builtin_bit_cast(u2_t, u.x), __builtin_bit_cast(u2_t, u.y)),
+        __builtin_elementwise_min(__builtin_bit_cast(u2_t, u.z), __builtin_bit_cast(u2_t, u.w)));
+    return min(m.x, m.y) <= (unsigned short)bits;
+  }
+}
+
+// The k best of `count` candidates in LDS: a wave takes every waves-th one and counts those
+// ahead of it, 64 at a time.  put(rank, value, id) runs on one lane.
+template <typename F>
+__device__ __forceinline__ void rank_candidates(const float *cv, const int *ci, int count,
+                                                int wave, int waves, int k, F &&put) {
+  const int lane = __lane_id();
+  for (int c = wave; c < count; c += waves) {
+    const float v = cv[c];
+    const int id = ci[c];
+    int rank = 0;
+    for (int j = 0; j < count; j += 64) {
+      const bool over = j + lane < count && ahead(cv[j + lane], ci[j + lane], v, id);
+      rank += __builtin_popcountll(__builtin_amdgcn_ballot_w64(over));
+    }
+    if (lane == 0 && rank < k) put(rank, v, id);
+  }
+}
+
+// One segment's sums and maximum, kept for the join.
 struct Partial {
-  float m, s, w, unused;
+  float c, s, w, mx;
 };
 
 // Where a workgroup's results go: a row's final figures, or a segment's for the join.
@@ -67,6 +145,15 @@ struct LogprobOut {
 // A row, or with SPLIT one segment of it, lives in the registers of NT threads, NV vectors
 // of 16 bytes each, read once.
 //
+// What bounds it: many rows the vector work, about 10 operations a value and the exponential
+// at a quarter of their rate (4.3 us of a row's 5.8 on its CU), two workgroups of 64 VGPRs a
+// CU overlapping it with the other's loads; few rows their own chain of loads,
+// exponentials and picks.  Device time, us: 4096 x 50265 bf16 k = 5 93 (4.4 TB/s), k = 0 82
+// (5.0); 256 x 50265 k = 0 8.5; 4 x 51289 k = 8 8.5; 93 x 51289 fp32 k = 20 10.7.  What
+// the steps gave (the same cases): loads that no condition holds back 106 -> 93, 10.4 ->
+// 8.5; ranks by ballot and packed compares for the alternatives k = 8 10.0 -> 8.5, k = 20
+// 13.1 -> 10.7.
+//
 // The alternatives: the k-th largest of the maxima of 64 groups of threads, tau, bounds the
 // k-th value from below (k groups hold a value >= tau); every value >= tau (24 of a random
 // row at k = 20) goes to LDS, and its rank is the number of candidates ahead of it.  Rows
@@ -79,7 +166,7 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
   using T = typename Elem<DT>::T;
   constexpr int NWAVE = NT / 64, VE = Elem<DT>::VEC;
   constexpr int GL = NT / 64;  // lanes of a group
-  __shared__ float s_group[64], s_cv[TLP_CAP], s_red[2][NWAVE], s_tau, s_bv[NWAVE];
+  __shared__ float s_group[64], s_cv[TLP_CAP], s_red[3][NWAVE], s_tau, s_bv[NWAVE];
   __shared__ int s_ci[TLP_CAP], s_count, s_bi[NWAVE];
 
   const int64_t row = blockIdx.x;
@@ -93,36 +180,71 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
   // few values before (threads 0..) and after them (threads 8..); absent values are -inf
   const int head = min(n, (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
   const int nvec = (n - head) / VE;
-  const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+  const __amdgpu_buffer_rsrc_t xv =
+      __builtin_amdgcn_make_buffer_rsrc((void *)(x + head), 0, nvec * 16, 0x00020000);
   constexpr uint32_t NI = DT == VFL_FLOAT32    ? 0xff800000u
                           : DT == VFL_BFLOAT16 ? 0xff80ff80u
                                                : 0xfc00fc00u;
+  // No load under a condition, whose branch would wait for it before the next one goes out:
+  // buffer loads return 0 past the row's last vector.  The given token of this thread first:
+  // its logit follows while the row is on its way.
+  int64_t token = 0;
+  if constexpr (!SPLIT) {
+    if (o.num_tokens > 0) token = o.tokens[row * o.num_tokens + min(tid, o.num_tokens - 1)];
+  }
   uint4 u[NV];
 #pragma unroll
-  for (int r = 0; r < NV; ++r) {
-    u[r] = make_uint4(NI, NI, NI, NI);
-    if (tid + r * NT < nvec) u[r] = xv[tid + r * NT];
-  }
+  for (int r = 0; r < NV; ++r)
+    u[r] = __builtin_bit_cast(
+        uint4, __builtin_amdgcn_raw_buffer_load_b128(xv, (tid + r * NT) * 16, 0, 0));
   int xi = -1;  // the scalar's place
   if (tid < head) xi = tid;
   else if (tid >= 8 && head + nvec * VE + tid - 8 < n) xi = head + nvec * VE + tid - 8;
-  const float xs = xi >= 0 ? logit<DT>(x[xi]) : NEG_INF_F;
-  // the row's first given tokens, on their way during the rest
-  float given = 0.f;
-  bool inside = false;
-  if constexpr (!SPLIT) {
-    if (tid < o.num_tokens) {
-      const int64_t t = o.tokens[row * o.num_tokens + tid];
-      inside = t >= 0 && t < vocab;
-      if (inside) given = logit<DT>(x[t]);
-    }
-  }
-  if (tid == 0) s_count = 0;
+  const T xraw = x[max(xi, 0)];
+  bool inside = token >= 0 && token < vocab;
+  T graw = 0;
+  if constexpr (!SPLIT) graw = x[inside ? token : 0];
+  if (tid == 0) s_count = 0, s_tau = NEG_INF_F;
 
-  float tmax = fmaxf(NEG_INF_F, xs);  // (a NaN bounds nothing)
+  // Each thread's sums about a reference of its own, moved only when a vector's maximum
+  // exceeds it by TLP_SLACK, so that the first vectors are summed while the last ones
+  // are on their way.
+  Sums sums{TLP_NONE, 0.f, 0.f};
+  float tmax = NEG_INF_F;  // (a NaN bounds nothing)
+  auto refer = [&](float v) {  // v: the maximum of what comes next
+    tmax = fmaxf(tmax, v);
+    const float to = v * LOG2E_F;
+    const bool need = to > sums.c + TLP_SLACK;
+    if (__builtin_amdgcn_ballot_w64(need) != 0) sums.move(need ? to : sums.c);
+  };
+  auto add = [&](float v, float &s, float &w) {
+    // one fused step, the same for a row's given tokens: what c lost in rounding is lost by
+    // every term alike and cancels.  exp2(-inf) = 0 must not meet its -inf.
+    const float t = fmaf(v, LOG2E_F, -sums.c), e = fast_exp2(t);
+    s += e;
+    w = fmaf(fmaxf(t, TLP_FLOOR), e, w);
+  };
 #pragma unroll
-  for (int r = 0; r < NV; ++r)
-    if (r * NT < nvec) tmax = fmaxf(tmax, vector_max<DT>(u[r]));  // workgroup-uniform
+  for (int r = 0; r < NV; ++r) {
+    if (r * NT >= nvec) continue;  // workgroup-uniform
+    if (__builtin_expect(r * NT + NT > nvec, 0)) {
+      if (tid + r * NT >= nvec) u[r] = make_uint4(NI, NI, NI, NI);
+      opaque(u[r]);
+    }
+    refer(vector_max<DT>(u[r]));
+    float s2 = 0.f, w2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) {
+      add(logit_of<DT>(u[r], j), sums.s, sums.w);
+      add(logit_of<DT>(u[r], j + 1), s2, w2);
+    }
+    sums.s += s2, sums.w += w2;
+    opaque(u[r]);
+  }
+  const float xs = xi >= 0 ? logit<DT>(xraw) : NEG_INF_F;
+  refer(xs);
+  add(xs, sums.s, sums.w);
+
   float g = tmax;
   if constexpr (GL >= 4) {
     g = fmaxf(g, dpp<DPP_QUAD_XOR1>(g));
@@ -133,83 +255,90 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
     g = fmaxf(g, dpp<DPP_ROW_MIRROR>(g));
   }
   if (tid % GL == 0) s_group[tid / GL] = g;
+  sums.move(wave_max64(sums.c));
+  const float ws = group_sum<64>(sums.s), ww = group_sum<64>(sums.w);
+  if (lane == 0) s_red[0][wave] = sums.c, s_red[1][wave] = ws, s_red[2][wave] = ww;
   __syncthreads();
   g = s_group[lane];
   const float mx = wave_max64(g);
-  if (wave == 0 && k > 0) {
+  // tau: one wave takes the best k - 1 groups away, several waves rank their shares of them
+  // (4096 x 3000, k = 5: 13.0 against 17.6 us with ranks for both)
+  if (NWAVE == 1 && k > 0) {
     float tau = mx;
-    if (k > 1) {
-      int rank = 0;
-#pragma unroll
-      for (int j = 0; j < 64; ++j) {
-        const float og = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
-        rank += og > g || (og == g && j < lane);
-      }
-      const uint64_t at = __builtin_amdgcn_ballot_w64(rank == k - 1);
-      tau = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), __builtin_ctzll(at)));
+    for (int r = k; r > 1; --r) {
+      const uint64_t top = __builtin_amdgcn_ballot_w64(g == tau);
+      if (lane == __builtin_ctzll(top | (1ull << 63))) g = NEG_INF_F;
+      tau = wave_max64(g);
     }
     if (lane == 0) s_tau = tau;
-  }
-
-  // S and W.  t = x - max first, then its product with log2 e: one fused step would round
-  // max * log2 e, an error common to every term.  exp(-inf) = 0 must not meet its -inf.
-  constexpr float LOG2E_F = 1.4426950408889634f;
-  const float ref = mx == NEG_INF_F ? 0.f : mx;
-  float s4[4] = {0.f, 0.f, 0.f, 0.f}, w4[4] = {0.f, 0.f, 0.f, 0.f};
+  } else if (k > 0) {
 #pragma unroll
-  for (int r = 0; r < NV; ++r) {
-    if (r * NT >= nvec) continue;
-    opaque(u[r]);
-#pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float t = logit_of<DT>(u[r], j) - ref, e = fast_exp2(t * LOG2E_F);
-      s4[j % 4] += e;
-      w4[j % 4] = fmaf(fmaxf(t, TLP_FLOOR), e, w4[j % 4]);
+    for (int j = 0; j < 64 / NWAVE; ++j) {
+      const int at = wave * (64 / NWAVE) + j;
+      const float og = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), at));
+      const uint64_t over = __builtin_amdgcn_ballot_w64(g > og);
+      const uint64_t level = __builtin_amdgcn_ballot_w64(g == og) & ((1ull << at) - 1);
+      if (__builtin_popcountll(over) + __builtin_popcountll(level) == k - 1 && lane == 0)
+        s_tau = og;
     }
   }
-  {
-    const float t = xs - ref, e = fast_exp2(t * LOG2E_F);
-    s4[0] += e;
-    w4[0] = fmaf(fmaxf(t, TLP_FLOOR), e, w4[0]);
+  // the waves' sums, joined by every wave for itself
+  Sums all{TLP_NONE, 0.f, 0.f};
+  if (lane < NWAVE) all = Sums{s_red[0][lane], s_red[1][lane], s_red[2][lane]};
+  all.move(wave_max64(all.c));
+  float S = wave_total(all.s), W = wave_total(all.w);
+  const bool extreme = fabsf(mx) > TLP_EXTREME && fabsf(mx) < INFINITY;
+  if (extreme) {  // its sum is the number of values that equal the maximum
+    int level = 0;
+    bool nan = false;
+#pragma nounroll
+    for (int i = tid; i < n; i += NT) {
+      const float v = logit<DT>(x[i]);
+      level += v == mx;
+      nan |= v != v;
+    }
+    for (int d = 1; d < 64; d *= 2) level += __shfl_xor(level, d);
+    nan = __syncthreads_or(nan);
+    if (lane == 0) s_bi[wave] = level;
+    __syncthreads();
+    level = 0;
+    for (int w = 0; w < NWAVE; ++w) level += s_bi[w];
+    S = nan ? NAN : (float)level, W = 0.f;
+    __syncthreads();  // s_bi may be written again
   }
-  const float ws = group_sum<64>((s4[0] + s4[1]) + (s4[2] + s4[3]));
-  const float ww = group_sum<64>((w4[0] + w4[1]) + (w4[2] + w4[3]));
-  if (lane == 0) s_red[0][wave] = ws, s_red[1][wave] = ww;
-  __syncthreads();
-  float S = 0.f, W = 0.f;
-#pragma unroll
-  for (int w = 0; w < NWAVE; ++w) S += s_red[0][w], W += s_red[1][w];
   // a NaN, +inf or an empty row leaves S NaN or 0
   const bool bad = !SPLIT && !(S > 0.f);
-  const float log_s = SPLIT ? 0.f : logf(S);
+  const Normaliser norm{all.c, log2f(S), mx, extreme};
   const int64_t seg = SPLIT ? row * gridDim.y + blockIdx.y : row;
   if constexpr (SPLIT) {
-    if (tid == 0) o.part[seg] = Partial{mx, S, W, 0.f};
+    if (tid == 0) o.part[seg] = Partial{all.c, S, W, mx};
   } else {
-    if (tid == 0) o.entropy[row] = bad ? NAN : log_s - W / S;
+    if (tid == 0) o.entropy[row] = bad ? NAN : LN2_F * (norm.log2_s - W / S);
     for (int i = tid; i < o.num_tokens; i += NT) {
       if (i != tid) {
-        const int64_t t = o.tokens[row * o.num_tokens + i];
-        inside = t >= 0 && t < vocab;
-        if (inside) given = logit<DT>(x[t]);
+        token = o.tokens[row * o.num_tokens + i];
+        inside = token >= 0 && token < vocab;
+        graw = x[inside ? token : 0];
       }
-      o.logprobs[row * o.num_tokens + i] = bad || !inside ? NAN : (given - mx) - log_s;
+      o.logprobs[row * o.num_tokens + i] =
+          bad || !inside ? NAN : norm.logprob(logit<DT>(graw));
     }
   }
   if (k == 0) return;
+  __syncthreads();  // s_tau
 
   auto put = [&](int rank, float v, int id) {
     if constexpr (SPLIT) {
       o.cand[seg * k + rank] = v;
       o.cand_id[seg * k + rank] = id;
     } else {
-      o.top[row * k + rank] = bad ? NAN : (v - mx) - log_s;
+      o.top[row * k + rank] = bad ? NAN : norm.logprob(v);
       o.ids[row * k + rank] = bad ? -1 : id;
     }
   };
   const float tau = s_tau;
   const bool bounded = tau != NEG_INF_F;
-  if (bounded && tmax >= tau) {
+  if (bounded) {
     auto keep = [&](float v, int i) {
       if (v >= tau) {
         const int slot = atomicAdd(&s_count, 1);
@@ -217,24 +346,28 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
       }
     };
     if (xi >= 0) keep(xs, xi);
+    uint32_t hits = 0;  // vectors of this thread that may hold one
 #pragma unroll
-    for (int r = 0; r < NV; ++r) {
-      opaque(u[r]);
-      if (r * NT >= nvec || !(vector_max<DT>(u[r]) >= tau)) continue;
+    for (int r = 0; r < NV; ++r)
+      if (r * NT < nvec && may_reach<DT>(u[r], tau)) hits |= 1u << r;
+    if (!(tmax >= tau)) hits = 0;
+    // one copy of the search for all of them: the code runs once a row, from a cold
+    // instruction cache
+    while (hits) {
+      const int r = __builtin_ctz(hits);
+      hits &= hits - 1;
+      uint4 h = u[0];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) keep(logit_of<DT>(u[r], j), head + (tid + r * NT) * VE + j);
+      for (int q = 1; q < NV; ++q)
+        if (r == q) h = u[q];
+#pragma unroll
+      for (int j = 0; j < VE; ++j) keep(logit_of<DT>(h, j), head + (tid + r * NT) * VE + j);
     }
   }
   __syncthreads();
   const int count = s_count;
   if (bounded && count <= TLP_CAP) {
-    for (int c = tid; c < count; c += NT) {
-      const float v = s_cv[c];
-      const int id = s_ci[c];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += ahead(s_cv[j], s_ci[j], v, id);
-      if (rank < k) put(rank, v, id);
-    }
+    rank_candidates(s_cv, s_ci, count, wave, NWAVE, k, put);
     return;
   }
   float last = INFINITY;
@@ -275,43 +408,39 @@ __global__ __launch_bounds__(TLP_JOIN_NT) void token_logprobs_join_kernel(
   const int tid = threadIdx.x, lane = tid & 63, k = o.k, count = segments * k;
   for (int i = tid; i < count; i += TLP_JOIN_NT)
     s_cv[i] = o.cand[row * count + i], s_ci[i] = o.cand_id[row * count + i];
-  Partial p{NEG_INF_F, 0.f, 0.f, 0.f};
+  Partial p{TLP_NONE, 0.f, 0.f, NEG_INF_F};
   if (lane < segments) p = o.part[row * segments + lane];
-  const float mx = wave_max64(p.m);
-  // W about the common maximum: sum (x - M) e = f (W + (m - M) S).  A segment of weight 0 adds
-  // nothing (0 times an m - M past fp32's range), but hands on its NaN.
-  const float dm = p.m - mx, f = p.m == NEG_INF_F ? 0.f : expf(dm);
-  const float S = group_sum<64>(p.m == NEG_INF_F ? p.s : f * p.s);
-  const float W = group_sum<64>(f == 0.f ? 0.f : f * (p.w + dm * p.s));
+  const float mx = wave_max64(p.mx);
+  const bool extreme = fabsf(mx) > TLP_EXTREME && fabsf(mx) < INFINITY;
+  // a segment that counted its values at an extreme maximum has weight 0 elsewhere
+  const bool counted = fabsf(p.mx) > TLP_EXTREME && fabsf(p.mx) < INFINITY;
+  const bool apart = p.s == p.s && (extreme ? p.mx != mx : counted);
+  Sums all{apart || extreme ? TLP_NONE : p.c, apart ? 0.f : p.s, apart ? 0.f : p.w};
+  all.move(wave_max64(all.c));
+  const float S = wave_total(all.s), W = wave_total(all.w);
   const bool bad = !(S > 0.f);
-  const float log_s = logf(S);
-  if (tid == 0) o.entropy[row] = bad ? NAN : log_s - W / S;
+  const Normaliser norm{all.c, log2f(S), mx, extreme};
+  if (tid == 0) o.entropy[row] = bad ? NAN : LN2_F * (norm.log2_s - W / S);
   const typename Elem<DT>::T *x = logits + row * stride;
   for (int i = tid; i < o.num_tokens; i += TLP_JOIN_NT) {
     const int64_t t = o.tokens[row * o.num_tokens + i];
     o.logprobs[row * o.num_tokens + i] =
-        bad || t < 0 || t >= vocab ? NAN : (logit<DT>(x[t]) - mx) - log_s;
+        bad || t < 0 || t >= vocab ? NAN : norm.logprob(logit<DT>(x[t]));
   }
   __syncthreads();
-  for (int c = tid; c < count; c += TLP_JOIN_NT) {
-    const float v = s_cv[c];
-    const int id = s_ci[c];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += ahead(s_cv[j], s_ci[j], v, id);
-    if (rank < k) {
-      o.top[row * k + rank] = bad ? NAN : (v - mx) - log_s;
-      o.ids[row * k + rank] = bad ? -1 : id;
-    }
-  }
+  rank_candidates(s_cv, s_ci, count, tid >> 6, TLP_JOIN_NT / 64, k, [&](int rank, float v, int id) {
+    o.top[row * k + rank] = bad ? NAN : norm.logprob(v);
+    o.ids[row * k + rank] = bad ? -1 : id;
+  });
 }
 
 // Values that a workgroup of 1024 threads holds, and so the longest row of one launch.
-constexpr int tlp_capacity(int dtype) { return dtype == VFL_FLOAT32 ? 1024 * 14 * 4 : 1024 * 8 * 8; }
-constexpr int TLP_SEGMENT_BYTES = 1024 * 8 * 16;
+constexpr int TLP_CAPACITY = 1024 * 7 * 8;
+constexpr int TLP_SEGMENT_BYTES = 1024 * 7 * 16;
 
 // Segments of a row that does not fit (0: it does), of equal length, a multiple of 8.
 inline int tlp_segments(int vocab, int dtype, int *segment) {
-  if (vocab <= tlp_capacity(dtype)) return 0;
+  if (vocab <= TLP_CAPACITY) return 0;
   const int most = TLP_SEGMENT_BYTES / elem_bytes(dtype);
   const int parts = (vocab + most - 1) / most;
   *segment = ((vocab + parts - 1) / parts + 7) / 8 * 8;
@@ -330,7 +459,7 @@ static int launch_token_logprobs(const void *logits, int64_t stride, int64_t row
     o.part = (Partial *)workspace;
     o.cand = (float *)(o.part + rows * segments);
     o.cand_id = (int32_t *)(o.cand + rows * segments * o.k);
-    token_logprobs_kernel<DT, 1024, 8, 8, true>
+    token_logprobs_kernel<DT, 1024, 7, 8, true>
         <<<dim3((unsigned)rows, (unsigned)segments), dim3(1024), 0, s>>>(x, stride, vocab, segment,
                                                                          o);
     const int st = launch_status("token_logprobs");
@@ -342,9 +471,9 @@ static int launch_token_logprobs(const void *logits, int64_t stride, int64_t row
 #define VFL_TLP(NT, NV, OCC)                                                       \
   token_logprobs_kernel<DT, NT, NV, OCC, false><<<dim3((unsigned)rows), dim3(NT), 0, s>>>( \
       x, stride, vocab, 0, o)
-  if (vocab <= 64 * 8 * VE) VFL_TLP(64, 8, 8);
-  else if (vocab <= 256 * 8 * VE) VFL_TLP(256, 8, 8);
-  else if (vocab <= 1024 * 8 * VE) VFL_TLP(1024, 8, 8);
+  if (vocab <= 64 * 7 * VE) VFL_TLP(64, 7, 8);
+  else if (vocab <= 256 * 7 * VE) VFL_TLP(256, 7, 8);
+  else if (vocab <= 1024 * 7 * VE) VFL_TLP(1024, 7, 8);
   else if constexpr (DT == VFL_FLOAT32) VFL_TLP(1024, 14, 4);
 #undef VFL_TLP
   return launch_status("token_logprobs");
