@@ -525,7 +525,10 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * (group_start) are rows sharing one table, at most 8 of them, block_table lists
  * max_blocks_per_seq blocks a row (longer contexts are clamped to that).  query and out
  * share dtype; out contiguous.  Sums and softmax in fp32, the weights kept to 2^-17 (fp32:
- * 2^-25) through the product with V.
+ * 2^-25) through the product with V.  kv_scales 8-byte aligned.  A launch of few rows over
+ * long tables splits their contexts, and a second one joins the parts: workspace is DEVICE
+ * memory, 16-byte aligned, of vfl_attention_8bit_workspace bytes for the call's sizes (0: none
+ * needed); calls that may overlap need one each.
  */
 int vfl_reshape_and_cache_8bit(const void *key, const void *value, int64_t key_stride_token,
                                int64_t key_stride_head, int64_t value_stride_token,
@@ -533,6 +536,8 @@ int vfl_reshape_and_cache_8bit(const void *key, const void *value, int64_t key_s
                                float *kv_scales, const int64_t *slot_mapping, int64_t num_tokens,
                                int num_heads, int head_dim, int block_size, int64_t num_blocks,
                                int dtype, void *stream);
+int64_t vfl_attention_8bit_workspace(int64_t num_rows, int64_t num_groups, int num_heads,
+                                     int head_dim, int block_size, int64_t max_blocks_per_seq);
 int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_token,
                                      int64_t query_stride_head, const void *k_cache,
                                      const void *v_cache, const float *kv_scales, void *out,
@@ -541,7 +546,7 @@ int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_tok
                                      const int32_t *group_start, const int32_t *group_order,
                                      int64_t num_rows, int64_t num_groups, int num_heads,
                                      int head_dim, int block_size, int64_t num_blocks,
-                                     float scale, int dtype, void *stream);
+                                     float scale, int dtype, void *workspace, void *stream);
 
 /*
  * Log probabilities of given tokens, entropy and best alternatives (no vllm_cpu_attn

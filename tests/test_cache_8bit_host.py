@@ -160,6 +160,31 @@ def test_c_entries_check_before_launch():
                 dict(key=A + 1)):
         assert append(**bad) == -1 and b"misaligned" in lib.vfl_last_error()
 
+    def attend(q=A, kc=A, vc=A, sc=A, out=A, lens=A, bt=A, stride=8, width=8, starts=None, rows=4,
+               groups=4, heads=2, dim=64, bs=16, nb=10, dt=1, ws=None):
+        return lib.vfl_attention_with_kv_cache_8bit(q, 128, 64, kc, vc, sc, out, lens, bt, stride,
+                                                    width, starts, None, rows, groups, heads, dim,
+                                                    bs, nb, 0.125, dt, ws, None)
+
+    assert attend(rows=0, groups=0) == 0 and attend(groups=0, starts=A) == 0
+    assert attend(dt=3) == -1 and attend(dim=72) == -2 and attend(bs=48) == -2
+    assert attend(rows=-1) == -1 and attend(groups=5) == -1 and attend(groups=3) == -1
+    assert attend(width=-1) == -1 and attend(stride=7) == -1
+    assert attend(width=1 << 28, stride=1 << 28) == -1  # more tokens than an int counts
+    assert attend(rows=1 << 30, groups=1 << 30) == -1
+    for bad in (dict(q=None), dict(kc=None), dict(vc=None), dict(sc=None), dict(out=None),
+                dict(lens=None), dict(bt=None)):
+        assert attend(**bad) == -1 and b"null" in lib.vfl_last_error()
+    for bad in (dict(kc=A + 8), dict(vc=A + 8), dict(sc=A + 4), dict(q=A + 1), dict(out=A + 1),
+                dict(ws=A + 4)):
+        assert attend(**bad) == -1 and b"misaligned" in lib.vfl_last_error()
+    # few rows over a long table need a workspace, many or short ones none
+    assert attend(width=4096, stride=4096) == -1 and b"workspace" in lib.vfl_last_error()
+    assert lib.vfl_attention_8bit_workspace(4, 4, 2, 64, 16, 4096) > 0
+    assert lib.vfl_attention_8bit_workspace(4, 4, 2, 64, 16, 64) == 0
+    assert lib.vfl_attention_8bit_workspace(4096, 4096, 16, 64, 16, 4096) == 0
+    assert lib.vfl_attention_8bit_workspace(0, 0, 2, 64, 16, 64) == 0
+
     def score(x=A, stride=100, rows=4, vocab=100, dt=1, tokens=A, n=1, k=0, lp=A, ent=A, top=A,
               ids=A, ws=None):
         return lib.vfl_token_logprobs(x, stride, rows, vocab, dt, tokens, n, k, lp, ent, top, ids,

@@ -46,6 +46,7 @@ EXPORTED_SYMBOLS = (
     "vfl_linear_norm",
     "vfl_layer_norm_apply",
     "vfl_reshape_and_cache_8bit",
+    "vfl_attention_8bit_workspace",
     "vfl_attention_with_kv_cache_8bit",
     "vfl_token_logprobs_workspace",
     "vfl_token_logprobs",
@@ -159,10 +160,11 @@ _SIGNATURES = {
         [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64,
          _i32, _vp],
     ),
+    "vfl_attention_8bit_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i64]),
     "vfl_attention_with_kv_cache_8bit": (
         ctypes.c_int,
         [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32,
-         _i32, _i32, _i64, _f32, _i32, _vp],
+         _i32, _i32, _i64, _f32, _i32, _vp, _vp],
     ),
     "vfl_token_logprobs_workspace": (_i64, [_i32, _i32, _i32]),
     "vfl_token_logprobs": (

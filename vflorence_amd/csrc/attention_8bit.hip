@@ -39,53 +39,136 @@ __device__ __forceinline__ uint2 take_bf16(float (&f)[4]) {
   return w;
 }
 
-// One lane's share of a 16-token part: per 64 dims, 16 dims of token l % 16 (K) and 4 dims x
-// 4 tokens (V).
-template <int NS> struct Part {
-  uint4 k[NS], v[NS];
+template <int DT>
+__device__ __forceinline__ void store_result(typename Elem<DT>::T *p, float S, float o) {
+  const float y = S > 0.f ? o / S : S == S ? 0.f : S;  // NaN scores stay NaN
+  if constexpr (DT == VFL_FLOAT32) *p = y;
+  else *p = (uint16_t)Mfma<DT>::narrow(y);
+}
+
+// One lane's share of 32 tokens, two 16-token parts: per 64 dims, 16 dims of token l % 16 (K)
+// and 4 dims x 4 tokens (V); and their blocks' scales.
+template <int NS> struct Pair {
+  uint4 k[2][NS], v[2][NS];
+  float ks[2], vs[2];
+  bool ok[2];
 };
 
-// NS: ceil(D / 64).  PARTS: 16-token parts of a block.  NW waves split a context.
+// The ids and scales of a run of blocks, 64 at a time in a lane each.  The next 64 ids and
+// their scales are requested while the current ones are used: ids two refills ahead, scales
+// (which need the id) one.
+struct BlockWalk {
+  const int32_t *table;
+  const float2 *scales;  // of the head, H apart
+  int H, end;            // of the row's blocks
+  int64_t num_blocks;
+  int base;  // of the current 64
+  int id, id1, id2;
+  float2 sc, sc1;
+
+  __device__ __forceinline__ int fetch_id(int b) const {
+    const int i = b + (int)__lane_id();
+    const int x = table[max(min(i, end - 1), 0)];  // the row lists at least one block
+    return i < end && x >= 0 && x < num_blocks ? x : -1;
+  }
+  __device__ __forceinline__ float2 fetch_scale(int x) const {
+    return scales[(int64_t)max(x, 0) * H];
+  }
+  __device__ __forceinline__ void start(int b) {
+    base = b;
+    id = fetch_id(b);
+    id1 = fetch_id(b + 64);
+    id2 = fetch_id(b + 128);
+    sc = fetch_scale(id);
+    sc1 = fetch_scale(id1);
+  }
+  __device__ __forceinline__ void advance() {
+    base += 64;
+    id = id1, sc = sc1;
+    id1 = id2, sc1 = fetch_scale(id2);
+    id2 = fetch_id(base + 128);
+  }
+};
+
+// What is added to a softmax when its context is split: [row][head][split].
+struct SplitOut {
+  float *acc;  // [D]
+  float2 *ml;
+};
+
+struct Attn8Args {
+  const void *q;
+  int64_t q_st, q_sh;
+  const uint8_t *kc, *vc;
+  const float *scales;
+  void *out;
+  const int32_t *seq_lens, *bt;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t *group_start, *group_order;
+  int64_t num_rows, num_groups;
+  int H, D;
+  int64_t num_blocks;
+  float scale_log2;
+  int splits;
+  SplitOut part;
+};
+
+constexpr int ATTN8_COLS = 8;  // rows of a group
+
+// Rows of the group at dispatch position `pos`, from row0 on (0: no such group).
+__device__ __forceinline__ int group_rows(const Attn8Args &a, int64_t pos, int64_t &row0) {
+  if (pos >= a.num_groups) return 0;
+  int64_t g = pos;
+  if (a.group_order) g = a.group_order[pos];
+  if (g < 0 || g >= a.num_groups) return 0;
+  row0 = g;
+  int n = 1;
+  if (a.group_start) {
+    row0 = a.group_start[g];
+    n = a.group_start[g + 1] - (int)row0;
+  }
+  if (row0 < 0 || row0 >= a.num_rows) return 0;
+  return (int)min((int64_t)min(n, ATTN8_COLS), a.num_rows - row0);
+}
+
+// NS: ceil(D / 64).  PARTS: 16-token parts of a block.  NW waves split a context, and
+// a.splits workgroups do where there are few rows (their sums then go to a.part).
 template <int DT, int NS, int PARTS, int NW>
-__global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(
-    const typename Elem<DT>::T *__restrict__ q, int64_t q_st, int64_t q_sh,
-    const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc,
-    const float *__restrict__ scales, typename Elem<DT>::T *__restrict__ out,
-    const int32_t *__restrict__ seq_lens, const int32_t *__restrict__ bt, int64_t bt_stride,
-    int max_blocks, const int32_t *__restrict__ group_start,
-    const int32_t *__restrict__ group_order, int64_t num_rows, int64_t num_groups, int H, int D,
-    int64_t num_blocks, float scale_log2) {
+__global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   using T = typename Elem<DT>::T;
   constexpr int KT = Terms<DT>::KT, QT = Terms<DT>::Q, PT = Terms<DT>::P;
-  constexpr int COLS = 8;  // rows of a group
+  constexpr int COLS = ATTN8_COLS;
   constexpr int BPP = 2 / PARTS;  // blocks per 32 tokens
   __shared__ float s_acc[NW][64 * NS][COLS + 1];
   __shared__ float s_ml[NW][2][COLS];
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int col = lane & 15, rg = lane >> 4;
+  const int H = a.H, D = a.D;
   int64_t pos;
   int h;
   xcd_position(blockIdx.x, (unsigned)H, pos, h);
-  if (pos >= num_groups) return;
-  int64_t g = pos;
-  if (group_order) g = group_order[pos];
-  if (g < 0 || g >= num_groups) return;
-  int64_t row0 = g;
-  int nrows = 1;
-  if (group_start) {
-    row0 = group_start[g];
-    nrows = group_start[g + 1] - (int)row0;
-  }
-  if (row0 < 0 || row0 >= num_rows) return;
-  nrows = (int)min((int64_t)min(nrows, COLS), num_rows - row0);
+  const int split = (int)(pos % a.splits);
+  int64_t row0;
+  const int nrows = group_rows(a, pos / a.splits, row0);
   if (nrows <= 0) return;
 
-  const int64_t room = (int64_t)max_blocks * 16 * PARTS;  // tokens the table can list
-  const int L = (int)min((int64_t)max(seq_lens[row0], 0), room);
+  const int64_t room = (int64_t)a.max_blocks * 16 * PARTS;  // tokens the table can list
+  const int L = (int)min((int64_t)max(a.seq_lens[row0], 0), room);
   const int pairs = (L + 31) / 32;
-  const int chunk = (pairs + NW - 1) / NW;
-  const int p0 = min(pairs, wave * chunk), p1 = min(pairs, p0 + chunk);
+  const int per_split = (pairs + a.splits - 1) / a.splits;
+  const int s0 = min(pairs, split * per_split), s1 = min(pairs, s0 + per_split);
+  const int chunk = (s1 - s0 + NW - 1) / NW;
+  const int p0 = min(s1, s0 + wave * chunk), p1 = min(s1, p0 + chunk);
+
+  BlockWalk walk;
+  walk.table = a.bt + row0 * a.bt_stride;
+  walk.scales = reinterpret_cast<const float2 *>(a.scales) + h;
+  walk.H = H;
+  walk.end = (L + 16 * PARTS - 1) / (16 * PARTS);
+  walk.num_blocks = a.num_blocks;
+  if (p0 < p1) walk.start(p0 * BPP);
 
   // Q operand: per 64 dims, dims 16 rg .. + 7 and + 8 .. + 15 of row `col`
   uint4 qop[NS][2][QT];
@@ -95,18 +178,18 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(
     for (int e = 0; e < 2; ++e) {
       const int d = 64 * s + 16 * rg + 8 * e;
       const bool in = col < nrows && d < D;
-      const T *p = q + (row0 + col) * q_st + h * q_sh + d;
+      const T *p = (const T *)a.q + (row0 + (in ? col : 0)) * a.q_st + h * a.q_sh + (in ? d : 0);
       if constexpr (DT != VFL_FLOAT32) {
-        qop[s][e][0] = make_uint4(0, 0, 0, 0);
-        if (in) qop[s][e][0] = load16_unaligned<DT>(p);
+        const uint4 u = load16_unaligned<DT>(p);
+        qop[s][e][0] = in ? u : make_uint4(0, 0, 0, 0);
       } else {
         float f[2][4];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i / 4][i % 4] = in ? p[i] : 0.f;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          const uint2 a = take_bf16(f[0]), b = take_bf16(f[1]);
-          qop[s][e][t] = make_uint4(a.x, a.y, b.x, b.y);
+          const uint2 x = take_bf16(f[0]), y = take_bf16(f[1]);
+          qop[s][e][t] = make_uint4(x.x, x.y, y.x, y.y);
         }
       }
     }
@@ -118,61 +201,77 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(
     for (int c = 0; c < 4; ++c) acc[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   float m = NEG_INF_F, l = 0.f;
 
-  const int32_t *table = bt + row0 * bt_stride;
-  const int64_t block_bytes = (int64_t)H * 16 * PARTS * D;
-  const int head_off = h * 16 * PARTS * D;
-  for (int p = p0; p < p1; ++p) {
-    Part<NS> part[2];
-    bool ok[2];
-    float ks[2], vs[2];
+  // A part's tile is read through a buffer descriptor that ends with its last token: what lies
+  // behind, or an id outside the pool, or dims past the head, reads as 0 without a branch.
+  uint32_t k_off[NS], v_off[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    k_off[s] = 64 * s + 16 * rg < D ? col * D + 64 * s + 16 * rg : 0x7fffffffu;
+    v_off[s] = 64 * s + 4 * col < D ? (rg * D + 64 * s + 4 * col) * 4 : 0x7fffffffu;
+  }
+  const int tile = 16 * PARTS * D;
+  auto load = [&](int p, Pair<NS> &x) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int b = p * BPP + u / PARTS;  // the part's block
-      const int tok = 32 * p + 16 * u;    // its first token
-      int id = -1;
-      if (tok < L) id = table[b];
-      ok[u] = id >= 0 && id < num_blocks;
-      ks[u] = vs[u] = 0.f;
-      if (ok[u]) {
-        const float *sc = scales + 2 * ((int64_t)id * H + h);
-        ks[u] = sc[0] * scale_log2, vs[u] = sc[1];
-      }
-      const int64_t base =
-          (ok[u] ? (int64_t)id : 0) * block_bytes + head_off + (u % PARTS) * 16 * D;
+      const int b = p * BPP + u / PARTS;
+      const int n = min(max(L - (32 * p + 16 * u), 0), 16);  // the part's tokens
+      const int id = n > 0 ? __builtin_amdgcn_readlane(walk.id, b - walk.base) : -1;
+      x.ok[u] = id >= 0;
+      x.ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(walk.sc.x), b - walk.base));
+      x.vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(walk.sc.y), b - walk.base));
+      const int64_t at =
+          ((int64_t)(x.ok[u] ? id : 0) * H + h) * tile + (u % PARTS) * 16 * D;
+      const auto kr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.kc + at), 0,
+                                                        x.ok[u] ? n * D : 0, 0x00020000);
+      const auto vr = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)(a.vc + at), 0, x.ok[u] ? (n + 3) / 4 * 4 * D : 0, 0x00020000);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        part[u].k[s] = part[u].v[s] = make_uint4(0, 0, 0, 0);
-        if (ok[u] && 64 * s + 16 * rg < D && tok + col < L)
-          part[u].k[s] = *reinterpret_cast<const uint4 *>(kc + base + col * D + 64 * s + 16 * rg);
-        if (ok[u] && 64 * s + 4 * col < D && tok + 4 * rg < L)
-          part[u].v[s] =
-              *reinterpret_cast<const uint4 *>(vc + base + (rg * D + 64 * s + 4 * col) * 4);
+        x.k[u][s] =
+            __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[s], 0, 0));
+        x.v[u][s] =
+            __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[s], 0, 0));
       }
     }
+  };
+
+  auto consume = [&](int p, Pair<NS> &x) {
+    const bool whole = 32 * p + 32 <= L && x.ok[0] && x.ok[1];  // wave-uniform
     float sv[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      floatx4_t x = {0.f, 0.f, 0.f, 0.f};
+      floatx4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const uint4 w = part[u].k[s];
-        const uint2 a = e4m3_widen<KT>(w.x), b = e4m3_widen<KT>(w.y), c = e4m3_widen<KT>(w.z),
-                    d = e4m3_widen<KT>(w.w);
+        const uint4 w = x.k[u][s];
+        const uint2 k0 = e4m3_widen<KT>(w.x), k1 = e4m3_widen<KT>(w.y), k2 = e4m3_widen<KT>(w.z),
+                    k3 = e4m3_widen<KT>(w.w);
 #pragma unroll
         for (int t = QT - 1; t >= 0; --t) {
-          x = Mfma<KT>::qk(make_uint4(a.x, a.y, b.x, b.y), qop[s][0][t], x);
-          x = Mfma<KT>::qk(make_uint4(c.x, c.y, d.x, d.y), qop[s][1][t], x);
+          y = Mfma<KT>::qk(make_uint4(k0.x, k0.y, k1.x, k1.y), qop[s][0][t], y);
+          y = Mfma<KT>::qk(make_uint4(k2.x, k2.y, k3.x, k3.y), qop[s][1][t], y);
         }
       }
+      const float ks = x.ks[u] * a.scale_log2;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sv[u][j] = ok[u] && 32 * p + 16 * u + 4 * rg + j < L ? x[j] * ks[u] : NEG_INF_F;
+      for (int j = 0; j < 4; ++j) sv[u][j] = y[j] * ks;
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(x.ok[u] && 32 * p + 16 * u + 4 * rg + j < L)) sv[u][j] = NEG_INF_F;
+        // what lies behind the last token must not meet a zero weight (0 * NaN)
+        const int n = L - (32 * p + 16 * u + 4 * rg);  // tokens of the lane's four
+        const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const uint4 v = x.v[u][s];
+          x.v[u][s] = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
+        }
+        if (!x.ok[u]) x.vs[u] = 0.f;
+      }
     }
-    float mb = NEG_INF_F;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mb = fmaxf(mb, sv[u][j]);
+    float mb = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
+                     fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
     mb = rows_max4(mb);
     const bool need = mb > m + RESCALE_SLACK_LOG2;
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
@@ -192,37 +291,42 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(
       for (int j = 0; j < 4; ++j) {
         const float e = fast_exp2(sv[u][j] - ms);
         l += e;
-        w[u][j] = e * vs[u];
+        w[u][j] = e * x.vs[u];
       }
     uint4 pop[PT];
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
-      const uint2 a = take_bf16(w[0]), b = take_bf16(w[1]);
-      pop[t] = make_uint4(a.x, a.y, b.x, b.y);
-    }
-    // what lies behind the last token must not meet a zero weight (0 * NaN)
-    if (32 * p + 32 > L) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int n = L - (32 * p + 16 * u + 4 * rg);  // tokens of the lane's four
-        const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          uint4 &v = part[u].v[s];
-          v = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
-        }
-      }
+      const uint2 p0 = take_bf16(w[0]), p1 = take_bf16(w[1]);
+      pop[t] = make_uint4(p0.x, p0.y, p1.x, p1.y);
     }
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const uint2 a = e4m3_widen<VFL_BFLOAT16>((&part[0].v[s].x)[c]);
-        const uint2 b = e4m3_widen<VFL_BFLOAT16>((&part[1].v[s].x)[c]);
+        const uint2 v0 = e4m3_widen<VFL_BFLOAT16>((&x.v[0][s].x)[c]);
+        const uint2 v1 = e4m3_widen<VFL_BFLOAT16>((&x.v[1][s].x)[c]);
 #pragma unroll
         for (int t = PT - 1; t >= 0; --t)
-          acc[s][c] = Bf16::qk(make_uint4(a.x, a.y, b.x, b.y), pop[t], acc[s][c]);
+          acc[s][c] = Bf16::qk(make_uint4(v0.x, v0.y, v1.x, v1.y), pop[t], acc[s][c]);
       }
+  };
+
+  // the next pair's loads go out before the current one is used
+  if (p0 < p1) {
+    Pair<NS> x, y;
+    load(p0, x);
+    for (int p = p0; p < p1; p += 2) {
+      auto next = [&](int q, Pair<NS> &z) {
+        if (q >= p1) return;
+        if (q * BPP - walk.base >= 64) walk.advance();
+        load(q, z);
+      };
+      next(p + 1, y);
+      consume(p, x);
+      if (p + 1 >= p1) break;
+      next(p + 2, x);
+      consume(p + 1, y);
+    }
   }
   l = rows_sum4(l);
 
@@ -251,48 +355,82 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(
       S = fmaf(s_ml[w][1][r], f, S);
       o = fmaf(s_acc[w][d][r], f, o);
     }
-    const float y = S > 0.f ? o / S : S == S ? 0.f : S;  // NaN scores stay NaN
-    if constexpr (DT == VFL_FLOAT32) out[((row0 + r) * H + h) * D + d] = y;
-    else out[((row0 + r) * H + h) * D + d] = (T)Mfma<DT>::narrow(y);
+    const int64_t at = (row0 + r) * H + h;
+    if (a.splits > 1) {
+      a.part.acc[(at * a.splits + split) * D + d] = o;
+      if (d == 0) a.part.ml[at * a.splits + split] = make_float2(M, S);
+    } else {
+      store_result<DT>((T *)a.out + at * D + d, S, o);
+    }
   }
 }
 
-struct Attn8Args {
-  const void *q;
-  int64_t q_st, q_sh;
-  const uint8_t *kc, *vc;
-  const float *scales;
-  void *out;
-  const int32_t *seq_lens, *bt;
-  int64_t bt_stride;
-  int max_blocks;
-  const int32_t *group_start, *group_order;
-  int64_t num_rows, num_groups;
-  int H, D;
-  int64_t num_blocks;
-  float scale_log2;
+// The splits of a (row, head) joined: 64 threads take a dim each, D / 64 times.
+template <int DT>
+__global__ __launch_bounds__(64) void attention_8bit_join_kernel(Attn8Args a) {
+  using T = typename Elem<DT>::T;
+  int64_t row0;
+  if ((int)blockIdx.y >= group_rows(a, blockIdx.x / a.H, row0)) return;
+  const int64_t at = (row0 + blockIdx.y) * a.H + blockIdx.x % a.H;
+  const float2 *ml = a.part.ml + at * a.splits;
+  float M = NEG_INF_F;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[s].x);
+  const float Ms = M == NEG_INF_F ? 0.f : M;
+  for (int d = threadIdx.x; d < a.D; d += 64) {
+    float S = 0.f, o = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const float f = fast_exp2(ml[s].x - Ms);
+      S = fmaf(ml[s].y, f, S);
+      o = fmaf(a.part.acc[(at * a.splits + s) * a.D + d], f, o);
+    }
+    store_result<DT>((T *)a.out + at * a.D + d, S, o);
+  }
+}
+
+// Waves of a workgroup and workgroups of a context.
+struct Attn8Plan {
+  int waves, splits;
 };
 
+inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens) {
+  Attn8Plan p{D > 256 ? 2 : 4, 1};
+  const int64_t wgs = num_groups * H;
+  if (D <= 128 && wgs <= 512) p.waves = 8;
+  const int64_t bytes = max_tokens * 2 * D;
+  if (bytes > (256 << 10) && wgs * p.waves < 4096) {
+    const int64_t fill = 4096 / (wgs * p.waves);
+    const int64_t most = max_tokens / 32 / (p.waves * 2);
+    p.splits = (int)(fill < most ? fill : most);
+    if (p.splits < 1) p.splits = 1;
+  }
+  return p;
+}
+
 template <int DT, int NS, int PARTS>
-static void launch_attention_8bit(const Attn8Args &a, hipStream_t stream) {
-  using T = typename Elem<DT>::T;
-  constexpr int NW = NS >= 8 ? 2 : NS >= 4 ? 4 : 4;
-  attention_8bit_kernel<DT, NS, PARTS, NW>
-      <<<dim3((unsigned)xcd_grid(a.num_groups, a.H)), dim3(64 * NW), 0, stream>>>(
-          (const T *)a.q, a.q_st, a.q_sh, a.kc, a.vc, a.scales, (T *)a.out, a.seq_lens, a.bt,
-          a.bt_stride, a.max_blocks, a.group_start, a.group_order, a.num_rows, a.num_groups, a.H,
-          a.D, a.num_blocks, a.scale_log2);
+static void launch_attention_8bit(const Attn8Args &a, int waves, hipStream_t stream) {
+  const dim3 grid((unsigned)xcd_grid(a.num_groups * a.splits, a.H));
+#define VFL_ATTN8(NW) \
+  attention_8bit_kernel<DT, NS, PARTS, NW><<<grid, dim3(64 * NW), 0, stream>>>(a)
+  if constexpr (NS == 8) VFL_ATTN8(2);
+  else if (NS <= 2 && waves == 8) { if constexpr (NS <= 2) VFL_ATTN8(8); }
+  else VFL_ATTN8(4);
+#undef VFL_ATTN8
 }
 
 template <int DT, int PARTS>
-static int launch_attention_8bit_steps(const Attn8Args &a, hipStream_t stream) {
+static int launch_attention_8bit_steps(const Attn8Args &a, int waves, hipStream_t stream) {
   switch ((a.D + 63) / 64) {
-    case 1: launch_attention_8bit<DT, 1, PARTS>(a, stream); break;
-    case 2: launch_attention_8bit<DT, 2, PARTS>(a, stream); break;
-    case 3: launch_attention_8bit<DT, 3, PARTS>(a, stream); break;
-    case 4: launch_attention_8bit<DT, 4, PARTS>(a, stream); break;
-    default: launch_attention_8bit<DT, 8, PARTS>(a, stream); break;  // head size 512
+    case 1: launch_attention_8bit<DT, 1, PARTS>(a, waves, stream); break;
+    case 2: launch_attention_8bit<DT, 2, PARTS>(a, waves, stream); break;
+    case 3: launch_attention_8bit<DT, 3, PARTS>(a, waves, stream); break;
+    case 4: launch_attention_8bit<DT, 4, PARTS>(a, waves, stream); break;
+    default: launch_attention_8bit<DT, 8, PARTS>(a, waves, stream); break;  // head size 512
   }
+  int st = launch_status("attention_with_kv_cache_8bit");
+  if (st != VFL_OK || a.splits == 1) return st;
+  const unsigned rows = a.group_start ? ATTN8_COLS : 1;
+  attention_8bit_join_kernel<DT>
+      <<<dim3((unsigned)(a.num_groups * a.H), rows), dim3(64), 0, stream>>>(a);
   return launch_status("attention_with_kv_cache_8bit");
 }
 
@@ -300,22 +438,36 @@ static int launch_attention_8bit_steps(const Attn8Args &a, hipStream_t stream) {
 
 using namespace vfl;
 
+// Bytes a (row, head) of one split takes in the workspace.
+static int64_t attn8_part_bytes(int head_dim) { return head_dim * 4 + 8; }
+
+extern "C" int64_t vfl_attention_8bit_workspace(int64_t num_rows, int64_t num_groups,
+                                                int num_heads, int head_dim, int block_size,
+                                                int64_t max_blocks_per_seq) {
+  if (num_rows <= 0 || num_groups <= 0 || num_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
+      max_blocks_per_seq <= 0)
+    return 0;
+  const Attn8Plan p =
+      attn8_plan(num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
+  return p.splits > 1 ? num_rows * num_heads * p.splits * attn8_part_bytes(head_dim) : 0;
+}
+
 extern "C" int vfl_attention_with_kv_cache_8bit(
     const void *query, int64_t query_stride_token, int64_t query_stride_head, const void *k_cache,
     const void *v_cache, const float *kv_scales, void *out, const int32_t *seq_lens,
     const int32_t *block_table, int64_t block_table_stride, int64_t max_blocks_per_seq,
     const int32_t *group_start, const int32_t *group_order, int64_t num_rows, int64_t num_groups,
     int num_heads, int head_dim, int block_size, int64_t num_blocks, float scale, int dtype,
-    void *stream) {
+    void *workspace, void *stream) {
   clear_error();
   const char *who = "attention_with_kv_cache_8bit";
   const int st = check_8bit_cache(who, dtype, num_heads, head_dim, block_size, num_blocks);
   if (st != VFL_OK) return st;
   if (num_rows < 0 || num_groups < 0 || num_groups > num_rows ||
       (!group_start && num_groups != num_rows) || max_blocks_per_seq < 0 ||
-      max_blocks_per_seq * block_size > 2147483647LL - 64 ||
+      max_blocks_per_seq > (2147483647LL - 64) / block_size ||
       block_table_stride < max_blocks_per_seq ||
-      (num_groups + XCDS) * (int64_t)num_heads > 2147483647LL) {
+      num_rows > 2147483647LL / num_heads - 8192) {
     set_error("%s: bad sizes (rows %lld groups %lld table %lld wide, stride %lld)", who,
               (long long)num_rows, (long long)num_groups, (long long)max_blocks_per_seq,
               (long long)block_table_stride);
@@ -328,21 +480,36 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
     return VFL_E_INVALID;
   }
   const int eb = elem_bytes(dtype);
-  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)kv_scales % 4 ||
-      (uintptr_t)query % eb || (uintptr_t)out % eb) {
-    set_error("%s: misaligned pointer (caches 16 bytes, others their element)", who);
+  if ((uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || (uintptr_t)kv_scales % 8 ||
+      (uintptr_t)query % eb || (uintptr_t)out % eb || (uintptr_t)workspace % 16) {
+    set_error("%s: misaligned pointer (caches and workspace 16 bytes, scales 8, others their "
+              "element)",
+              who);
     return VFL_E_INVALID;
   }
-  const Attn8Args a{query, query_stride_token, query_stride_head, (const uint8_t *)k_cache,
-                    (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
-                    block_table_stride, (int)max_blocks_per_seq, group_start, group_order,
-                    num_rows, num_groups, num_heads, head_dim, num_blocks,
-                    scale * 1.4426950408889634f};
+  // an empty pool holds nothing: every row is zero
+  const int64_t table = num_blocks ? max_blocks_per_seq : 0;
+  Attn8Args a{query, query_stride_token, query_stride_head, (const uint8_t *)k_cache,
+              (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
+              block_table_stride, (int)table, group_start, group_order,
+              num_rows, num_groups, num_heads, head_dim, num_blocks,
+              scale * 1.4426950408889634f, 1, {nullptr, nullptr}};
+  const Attn8Plan plan = attn8_plan(num_groups, num_heads, head_dim, table * block_size);
+  if (plan.splits > 1) {
+    if (!workspace) {
+      set_error("%s: null workspace", who);
+      return VFL_E_INVALID;
+    }
+    a.splits = plan.splits;
+    const int64_t parts = num_rows * num_heads * plan.splits;
+    a.part.ml = (float2 *)workspace;
+    a.part.acc = (float *)(a.part.ml + parts);
+  }
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    return block_size == 16 ? launch_attention_8bit_steps<DT, 1>(a, s)
-                            : launch_attention_8bit_steps<DT, 2>(a, s);
+    return block_size == 16 ? launch_attention_8bit_steps<DT, 1>(a, plan.waves, s)
+                            : launch_attention_8bit_steps<DT, 2>(a, plan.waves, s);
   };
   if (dtype == VFL_FLOAT32) return go(std::integral_constant<int, VFL_FLOAT32>{});
   if (dtype == VFL_BFLOAT16) return go(std::integral_constant<int, VFL_BFLOAT16>{});

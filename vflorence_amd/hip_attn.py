@@ -12,6 +12,7 @@ tensors are rejected: there is no host implementation behind these names.
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 from dataclasses import dataclass, field
 
@@ -886,6 +887,11 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
               dtype)
 
 
+@functools.lru_cache(maxsize=4096)
+def _attention_8bit_workspace(*sizes: int) -> int:
+    return lib.vfl_attention_8bit_workspace(*sizes)
+
+
 def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                                  v_cache: torch.Tensor, kv_scales: torch.Tensor,
                                  out: torch.Tensor, seq_lens: torch.Tensor, *, scale: float,
@@ -933,12 +939,16 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
         if not sm.own_tables or sm.group_start is None:
             start, order, num_groups = sm.group_start, sm.group_order, sm.num_groups
         _require_gpu(query, *(t for t in (start, order) if t is not None))
+    width = block_table.shape[1]
+    need = _attention_8bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     on_device(query, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
               query.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
               out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-              block_table.shape[1], None if start is None else start.data_ptr(),
+              width, None if start is None else start.data_ptr(),
               None if order is None else order.data_ptr(), num_rows, num_groups, num_heads,
-              head_dim, block_size, num_blocks, float(scale), dtype)
+              head_dim, block_size, num_blocks, float(scale), dtype,
+              workspace.data_ptr() if need else None)
 
 
 def cache_pointer_table(caches: list[torch.Tensor]) -> torch.Tensor:
