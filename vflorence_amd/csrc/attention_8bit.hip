@@ -46,6 +46,10 @@ __device__ __forceinline__ void store_result(typename Elem<DT>::T *p, float S, f
   else *p = (uint16_t)Mfma<DT>::narrow(y);
 }
 
+__device__ __forceinline__ float lane_float(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
+}
+
 // One lane's share of 32 tokens, two 16-token parts: per 64 dims, 16 dims of token l % 16 (K)
 // and 4 dims x 4 tokens (V); and their blocks' scales.
 template <int NS> struct Pair {
@@ -54,31 +58,35 @@ template <int NS> struct Pair {
   bool ok[2];
 };
 
-// The ids and scales of a run of blocks, 64 at a time in a lane each.  The next 64 ids and
-// their scales are requested while the current ones are used: ids two refills ahead, scales
+// The ids and scales of a wave's blocks, 64 at a time in a lane each.  Its i-th 32 tokens are
+// the context's (first + i * step)-th: which blocks those are does not hang on the row's
+// length, so the first ids are on their way together with it.  The next 64 ids and their
+// scales are requested while the current ones are used: ids two refills ahead, scales
 // (which need the id) one.
-struct BlockWalk {
+template <int BPP> struct BlockWalk {  // BPP: blocks per 32 tokens
   const int32_t *table;
   const float2 *scales;  // of the head, H apart
-  int H, end;            // of the row's blocks
+  int H, width, first, step;
   int64_t num_blocks;
-  int base;  // of the current 64
+  int base;  // of the current 64, counted in the wave's own blocks
   int id, id1, id2;
   float2 sc, sc1;
 
-  __device__ __forceinline__ int fetch_id(int b) const {
-    const int i = b + (int)__lane_id();
-    const int x = table[max(min(i, end - 1), 0)];  // the row lists at least one block
-    return i < end && x >= 0 && x < num_blocks ? x : -1;
+  __device__ __forceinline__ int fetch_id(int i) const {
+    i += (int)__lane_id();
+    const int64_t b = (first + (int64_t)(i / BPP) * step) * BPP + i % BPP;
+    return table[min(b, (int64_t)width - 1)];
   }
   __device__ __forceinline__ float2 fetch_scale(int x) const {
-    return scales[(int64_t)max(x, 0) * H];
+    return scales[max(min((int64_t)x, num_blocks - 1), (int64_t)0) * H];
   }
-  __device__ __forceinline__ void start(int b) {
-    base = b;
-    id = fetch_id(b);
-    id1 = fetch_id(b + 64);
-    id2 = fetch_id(b + 128);
+  __device__ __forceinline__ void start() {
+    base = 0;
+    id = fetch_id(0);
+    id1 = fetch_id(64);
+    id2 = fetch_id(128);
+  }
+  __device__ __forceinline__ void start_scales() {
     sc = fetch_scale(id);
     sc1 = fetch_scale(id1);
   }
@@ -89,6 +97,12 @@ struct BlockWalk {
     id2 = fetch_id(base + 128);
   }
 };
+
+// A descriptor of `bytes` bytes (wave-uniform) from p on; loads past them return 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, __builtin_amdgcn_readfirstlane(bytes),
+                                           0x00020000);
+}
 
 // What is added to a softmax when its context is split: [row][head][split].
 struct SplitOut {
@@ -104,12 +118,13 @@ struct Attn8Args {
   void *out;
   const int32_t *seq_lens, *bt;
   int64_t bt_stride;
-  int max_blocks;
+  int width, room;  // entries of a table row (one at least), tokens it can list
   const int32_t *group_start, *group_order;
   int64_t num_rows, num_groups;
   int H, D;
   int64_t num_blocks;
   float scale_log2;
+  bool q_vec;  // every 8 elements of a query are 16-byte aligned
   int splits;
   SplitOut part;
 };
@@ -143,7 +158,8 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   __shared__ float s_acc[NW][64 * NS][COLS + 1];
   __shared__ float s_ml[NW][2][COLS];
 
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  // (known to be wave-uniform, so that descriptors live in scalar registers)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, rg = lane >> 4;
   const int H = a.H, D = a.D;
   int64_t pos;
@@ -154,24 +170,23 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   const int nrows = group_rows(a, pos / a.splits, row0);
   if (nrows <= 0) return;
 
-  const int64_t room = (int64_t)a.max_blocks * 16 * PARTS;  // tokens the table can list
-  const int L = (int)min((int64_t)max(a.seq_lens[row0], 0), room);
-  const int pairs = (L + 31) / 32;
-  const int per_split = (pairs + a.splits - 1) / a.splits;
-  const int s0 = min(pairs, split * per_split), s1 = min(pairs, s0 + per_split);
-  const int chunk = (s1 - s0 + NW - 1) / NW;
-  const int p0 = min(s1, s0 + wave * chunk), p1 = min(s1, p0 + chunk);
-
-  BlockWalk walk;
+  BlockWalk<BPP> walk;
   walk.table = a.bt + row0 * a.bt_stride;
   walk.scales = reinterpret_cast<const float2 *>(a.scales) + h;
   walk.H = H;
-  walk.end = (L + 16 * PARTS - 1) / (16 * PARTS);
+  walk.width = a.width;
+  walk.first = split * NW + wave;
+  walk.step = a.splits * NW;
   walk.num_blocks = a.num_blocks;
-  if (p0 < p1) walk.start(p0 * BPP);
+  walk.start();
+  const int L = min(max(a.seq_lens[row0], 0), a.room);
+  const int pairs = (L + 31) / 32;
+  const int first = split * NW + wave, step = a.splits * NW;
+  const int count = first < pairs ? (pairs - first - 1) / step + 1 : 0;  // of this wave
 
-  // Q operand: per 64 dims, dims 16 rg .. + 7 and + 8 .. + 15 of row `col`
-  uint4 qop[NS][2][QT];
+  // Query: per 64 dims, dims 16 rg .. + 7 and + 8 .. + 15 of row `col`
+  constexpr int QV = DT == VFL_FLOAT32 ? 2 : 1;  // 16-byte vectors of 8 elements
+  uint4 qraw[NS][2][QV];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -179,18 +194,11 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       const int d = 64 * s + 16 * rg + 8 * e;
       const bool in = col < nrows && d < D;
       const T *p = (const T *)a.q + (row0 + (in ? col : 0)) * a.q_st + h * a.q_sh + (in ? d : 0);
-      if constexpr (DT != VFL_FLOAT32) {
-        const uint4 u = load16_unaligned<DT>(p);
-        qop[s][e][0] = in ? u : make_uint4(0, 0, 0, 0);
-      } else {
-        float f[2][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i / 4][i % 4] = in ? p[i] : 0.f;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          const uint2 x = take_bf16(f[0]), y = take_bf16(f[1]);
-          qop[s][e][t] = make_uint4(x.x, x.y, y.x, y.y);
-        }
+      for (int i = 0; i < QV; ++i) {
+        if (a.q_vec) qraw[s][e][i] = reinterpret_cast<const uint4 *>(p)[i];
+        else qraw[s][e][i] = load16_unaligned<DT>(p + 4 * i);
+        if (!in) qraw[s][e][i] = make_uint4(0, 0, 0, 0);
       }
     }
 
@@ -210,21 +218,21 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
     v_off[s] = 64 * s + 4 * col < D ? (rg * D + 64 * s + 4 * col) * 4 : 0x7fffffffu;
   }
   const int tile = 16 * PARTS * D;
-  auto load = [&](int p, Pair<NS> &x) {
+  // the wave's i-th 32 tokens (nothing at and past `count`)
+  auto load = [&](int i, Pair<NS> &x) {
+    const int p = first + i * step;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int b = p * BPP + u / PARTS;
+      const int from = (i * BPP + u / PARTS - walk.base) & 63;  // lane of the part's block
       const int n = min(max(L - (32 * p + 16 * u), 0), 16);  // the part's tokens
-      const int id = n > 0 ? __builtin_amdgcn_readlane(walk.id, b - walk.base) : -1;
-      x.ok[u] = id >= 0;
-      x.ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(walk.sc.x), b - walk.base));
-      x.vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(walk.sc.y), b - walk.base));
+      const int id = __builtin_amdgcn_readlane(walk.id, from);
+      x.ok[u] = n > 0 && id >= 0 && id < a.num_blocks;
+      x.ks[u] = lane_float(walk.sc.x, from);
+      x.vs[u] = lane_float(walk.sc.y, from);
       const int64_t at =
           ((int64_t)(x.ok[u] ? id : 0) * H + h) * tile + (u % PARTS) * 16 * D;
-      const auto kr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.kc + at), 0,
-                                                        x.ok[u] ? n * D : 0, 0x00020000);
-      const auto vr = __builtin_amdgcn_make_buffer_rsrc(
-          (void *)(a.vc + at), 0, x.ok[u] ? (n + 3) / 4 * 4 * D : 0, 0x00020000);
+      const auto kr = tile_buffer(a.kc + at, x.ok[u] ? n * D : 0);
+      const auto vr = tile_buffer(a.vc + at, x.ok[u] ? (n + 3) / 4 * 4 * D : 0);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         x.k[u][s] =
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
     }
   };
 
-  auto consume = [&](int p, Pair<NS> &x) {
+  auto consume = [&](int p, Pair<NS> &x, const uint4 (&qop)[NS][2][QT]) {
     const bool whole = 32 * p + 32 <= L && x.ok[0] && x.ok[1];  // wave-uniform
     float sv[2][4];
 #pragma unroll
@@ -311,21 +319,40 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       }
   };
 
-  // the next pair's loads go out before the current one is used
-  if (p0 < p1) {
+  // the next 32 tokens' loads go out before the current ones are used
+  uint4 qop[NS][2][QT];
+  if (count > 0) {
     Pair<NS> x, y;
-    load(p0, x);
-    for (int p = p0; p < p1; p += 2) {
-      auto next = [&](int q, Pair<NS> &z) {
-        if (q >= p1) return;
-        if (q * BPP - walk.base >= 64) walk.advance();
-        load(q, z);
-      };
-      next(p + 1, y);
-      consume(p, x);
-      if (p + 1 >= p1) break;
-      next(p + 2, x);
-      consume(p + 1, y);
+    walk.start_scales();
+    load(0, x);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if constexpr (DT != VFL_FLOAT32) {
+          qop[s][e][0] = qraw[s][e][0];
+        } else {
+          float f[2][4];
+          unpack16<DT>(qraw[s][e][0], f[0]);
+          unpack16<DT>(qraw[s][e][1], f[1]);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const uint2 lo = take_bf16(f[0]), hi = take_bf16(f[1]);
+            qop[s][e][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
+      }
+    // (a load under a condition would make the waits before a use count on its absence)
+    auto next = [&](int i, Pair<NS> &z) {
+      if (i < count && i * BPP - walk.base >= 64) walk.advance();
+      load(i, z);
+    };
+    for (int i = 0; i < count; i += 2) {
+      next(i + 1, y);
+      consume(first + i * step, x, qop);
+      if (i + 1 >= count) break;
+      next(i + 2, x);
+      consume(first + (i + 1) * step, y, qop);
     }
   }
   l = rows_sum4(l);
@@ -365,25 +392,47 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   }
 }
 
-// The splits of a (row, head) joined: 64 threads take a dim each, D / 64 times.
+// The splits of a (row, head) joined: a quarter of D threads take 4 dims each of a split, the
+// rest of the workgroup the next splits; their sums meet in LDS.
+constexpr int ATTN8_JOIN_NT = 256;
 template <int DT>
-__global__ __launch_bounds__(64) void attention_8bit_join_kernel(Attn8Args a) {
+__global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn8Args a) {
   using T = typename Elem<DT>::T;
+  __shared__ float4 s_o[ATTN8_JOIN_NT];
+  __shared__ float s_s[ATTN8_JOIN_NT];
   int64_t row0;
   if ((int)blockIdx.y >= group_rows(a, blockIdx.x / a.H, row0)) return;
   const int64_t at = (row0 + blockIdx.y) * a.H + blockIdx.x % a.H;
   const float2 *ml = a.part.ml + at * a.splits;
+  const int tid = threadIdx.x, quads = a.D / 4, teams = ATTN8_JOIN_NT / quads;
+  const int team = tid / quads, quad = tid % quads;
   float M = NEG_INF_F;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[s].x);
+  for (int s = tid & 63; s < a.splits; s += 64) M = fmaxf(M, ml[s].x);
+  M = wave_max64(M);
   const float Ms = M == NEG_INF_F ? 0.f : M;
-  for (int d = threadIdx.x; d < a.D; d += 64) {
-    float S = 0.f, o = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float f = fast_exp2(ml[s].x - Ms);
-      S = fmaf(ml[s].y, f, S);
-      o = fmaf(a.part.acc[(at * a.splits + s) * a.D + d], f, o);
+  float S = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (team < teams) {
+    for (int s = team; s < a.splits; s += teams) {
+      const float2 x = ml[s];
+      const float f = fast_exp2(x.x - Ms);
+      const float4 v =
+          *reinterpret_cast<const float4 *>(a.part.acc + (at * a.splits + s) * a.D + 4 * quad);
+      S = fmaf(x.y, f, S);
+      o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
     }
-    store_result<DT>((T *)a.out + at * a.D + d, S, o);
+  }
+  s_o[tid] = o;
+  s_s[tid] = S;
+  __syncthreads();
+  for (int d = tid; d < a.D; d += ATTN8_JOIN_NT) {
+    float sum = 0.f, y = 0.f;
+    for (int t = 0; t < teams; ++t) {
+      sum += s_s[t * quads + d / 4];
+      y += (&s_o[t * quads + d / 4].x)[d % 4];
+    }
+    store_result<DT>((T *)a.out + at * a.D + d, sum, y);
   }
 }
 
@@ -398,7 +447,7 @@ inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens
   if (D <= 128 && wgs <= 512) p.waves = 8;
   const int64_t bytes = max_tokens * 2 * D;
   if (bytes > (256 << 10) && wgs * p.waves < 4096) {
-    const int64_t fill = 4096 / (wgs * p.waves);
+    const int64_t fill = (D <= 64 ? 4096 : 2048) / (wgs * p.waves);
     const int64_t most = max_tokens / 32 / (p.waves * 2);
     p.splits = (int)(fill < most ? fill : most);
     if (p.splits < 1) p.splits = 1;
@@ -430,7 +479,7 @@ static int launch_attention_8bit_steps(const Attn8Args &a, int waves, hipStream_
   if (st != VFL_OK || a.splits == 1) return st;
   const unsigned rows = a.group_start ? ATTN8_COLS : 1;
   attention_8bit_join_kernel<DT>
-      <<<dim3((unsigned)(a.num_groups * a.H), rows), dim3(64), 0, stream>>>(a);
+      <<<dim3((unsigned)(a.num_groups * a.H), rows), dim3(ATTN8_JOIN_NT), 0, stream>>>(a);
   return launch_status("attention_with_kv_cache_8bit");
 }
 
@@ -491,9 +540,13 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
   const int64_t table = num_blocks ? max_blocks_per_seq : 0;
   Attn8Args a{query, query_stride_token, query_stride_head, (const uint8_t *)k_cache,
               (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
-              block_table_stride, (int)table, group_start, group_order,
+              block_table_stride, (int)table, (int)table * block_size, group_start, group_order,
               num_rows, num_groups, num_heads, head_dim, num_blocks,
-              scale * 1.4426950408889634f, 1, {nullptr, nullptr}};
+              scale * 1.4426950408889634f,
+              (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
+                  query_stride_head % (16 / eb) == 0,
+              1, {nullptr, nullptr}};
+  if (table == 0) a.bt = seq_lens, a.bt_stride = 0, a.width = 1;  // read, and not used
   const Attn8Plan plan = attn8_plan(num_groups, num_heads, head_dim, table * block_size);
   if (plan.splits > 1) {
     if (!workspace) {
