@@ -1,9 +1,9 @@
 // Paged decode attention over a cache held in e4m3 with a scale per (block, head) for K and
 // one for V, gfx950:
 //   out[r][h] = softmax_j(scale * ks_j <q[r][h], K8_j[h]>) (vs_j V8_j[h]),  j < seq_lens[r]
-// with ks_j, vs_j the scales of token j's block.  The K scale multiplies a block's scores and
-// the V scale its weights, so no element is dequantised in memory: e4m3 widens to 16 bits
-// exactly (one conversion per pair) on its way into the matrix cores.
+// with ks_j, vs_j the scales of token j's block, powers of two.  e4m3 times such a scale is
+// exact in bf16 (one conversion per pair, which adds the exponent) on its way into the matrix
+// cores.
 //
 // The rows of a group (a request's beams over one page list) sit in the 16 columns of the
 // tiles.  A wave takes 32 tokens at a time, two 16-token parts:
@@ -13,19 +13,18 @@
 //   O^T[d][row] += V^T[d][tok] . P[tok][row] v_mfma_f32_16x16x32 over the 32 tokens: a lane's
 //                  scores are already that product's operand, and V's token-interleaved
 //                  layout gives a lane 4 dims x 4 tokens per 16 bytes
-// Queries: 16-bit ones as they are; fp32 ones as three bf16 terms, which hold all 24 bits.
-// Weights go through the second product in bf16 (whose range holds any scale) as a sum of
-// two terms, 2^-17 relative, or three for fp32 outputs, 2^-25: below the output's rounding.
+// Queries go in as bf16 terms, which hold all of their bits: one of bf16, two of fp16, three of
+// fp32.  Weights as two terms, 2^-17 relative, or three for fp32 outputs, 2^-25: below the
+// output's rounding.  Their sum is the same product with a row of ones.
 #include <stdio.h>
 
 #include "e4m3.h"
 
 namespace vfl {
 
-// 16-bit type K is widened to, and terms of a query and of a weight
+// bf16 terms of a query and of a weight
 template <int DT> struct Terms {
-  static constexpr int KT = DT == VFL_FLOAT16 ? VFL_FLOAT16 : VFL_BFLOAT16;
-  static constexpr int Q = DT == VFL_FLOAT32 ? 3 : 1;
+  static constexpr int Q = DT == VFL_FLOAT32 ? 3 : DT == VFL_FLOAT16 ? 2 : 1;
   static constexpr int P = DT == VFL_FLOAT32 ? 3 : 2;
 };
 
@@ -55,7 +54,7 @@ __device__ __forceinline__ float lane_float(float x, int lane) {
 template <int NS> struct Pair {
   uint4 k[2][NS], v[2][NS];
   float ks[2], vs[2];
-  bool ok[2];
+  bool ok[2];  // holds tokens of the context
 };
 
 // The ids and scales of a wave's blocks, 64 at a time in a lane each.  Its i-th 32 tokens are
@@ -68,9 +67,13 @@ template <int BPP> struct BlockWalk {  // BPP: blocks per 32 tokens
   const float2 *scales;  // of the head, H apart
   int H, width, first, step;
   int64_t num_blocks;
-  int base;  // of the current 64, counted in the wave's own blocks
-  int id, id1, id2;
-  float2 sc, sc1;
+  int64_t block_bytes;
+  int base;        // of the current 64, counted in the wave's own blocks
+  uint64_t inside; // lanes whose block lies in the pool
+  uint64_t at;     // the block's first byte, of a lane's block
+  float2 sc;
+  int id1, id2;
+  float2 sc1;
 
   __device__ __forceinline__ int fetch_id(int i) const {
     i += (int)__lane_id();
@@ -80,20 +83,30 @@ template <int BPP> struct BlockWalk {  // BPP: blocks per 32 tokens
   __device__ __forceinline__ float2 fetch_scale(int x) const {
     return scales[max(min((int64_t)x, num_blocks - 1), (int64_t)0) * H];
   }
+  __device__ __forceinline__ void use(int x) {
+    const bool in = x >= 0 && x < num_blocks;
+    inside = __builtin_amdgcn_ballot_w64(in);
+    at = (uint64_t)(in ? x : 0) * (uint64_t)block_bytes;
+  }
+  // start() requests, begin() takes what came
   __device__ __forceinline__ void start() {
     base = 0;
-    id = fetch_id(0);
-    id1 = fetch_id(64);
-    id2 = fetch_id(128);
+    id1 = fetch_id(0);
+    id2 = fetch_id(64);
   }
-  __device__ __forceinline__ void start_scales() {
-    sc = fetch_scale(id);
-    sc1 = fetch_scale(id1);
+  __device__ __forceinline__ void begin() {
+    sc = fetch_scale(id1);
+    sc1 = fetch_scale(id2);
+    use(id1);
+    id1 = id2;
+    id2 = fetch_id(128);
   }
   __device__ __forceinline__ void advance() {
     base += 64;
-    id = id1, sc = sc1;
-    id1 = id2, sc1 = fetch_scale(id2);
+    use(id1);
+    sc = sc1;
+    sc1 = fetch_scale(id2);
+    id1 = id2;
     id2 = fetch_id(base + 128);
   }
 };
@@ -102,6 +115,14 @@ template <int BPP> struct BlockWalk {  // BPP: blocks per 32 tokens
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, __builtin_amdgcn_readfirstlane(bytes),
                                            0x00020000);
+}
+
+// x limited to 0 .. 16, on the scalar unit (a median of three would go to the vector unit, and
+// wait there for the registers of loads in flight).
+__device__ __forceinline__ int clamp_scalar(int x) {
+  int r;
+  asm("s_max_i32 %0, %1, 0\n\ts_min_i32 %0, %0, 16" : "=s"(r) : "s"(x) : "scc");
+  return r;
 }
 
 // What is added to a softmax when its context is split: [row][head][split].
@@ -123,13 +144,25 @@ struct Attn8Args {
   int64_t num_rows, num_groups;
   int H, D;
   int64_t num_blocks;
-  float scale_log2;
+  float scale_log2;  // its magnitude: the query takes the sign
+  uint32_t q_sign;   // flips the sign of a word's elements
   bool q_vec;  // every 8 elements of a query are 16-byte aligned
   int splits;
   SplitOut part;
 };
 
 constexpr int ATTN8_COLS = 8;  // rows of a group
+constexpr float NO_SCORE = -3e38f;
+
+// Maximum across the four 16-lane rows, a NaN passed on.
+__device__ __forceinline__ float rows_maximum4(float x) {
+  const auto a =
+      __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // Rows of the group at dispatch position `pos`, from row0 on (0: no such group).
 __device__ __forceinline__ int group_rows(const Attn8Args &a, int64_t pos, int64_t &row0) {
@@ -152,7 +185,7 @@ __device__ __forceinline__ int group_rows(const Attn8Args &a, int64_t pos, int64
 template <int DT, int NS, int PARTS, int NW>
 __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   using T = typename Elem<DT>::T;
-  constexpr int KT = Terms<DT>::KT, QT = Terms<DT>::Q, PT = Terms<DT>::P;
+  constexpr int QT = Terms<DT>::Q, PT = Terms<DT>::P;
   constexpr int COLS = ATTN8_COLS;
   constexpr int BPP = 2 / PARTS;  // blocks per 32 tokens
   __shared__ float s_acc[NW][64 * NS][COLS + 1];
@@ -178,6 +211,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   walk.first = split * NW + wave;
   walk.step = a.splits * NW;
   walk.num_blocks = a.num_blocks;
+  walk.block_bytes = (int64_t)H * 16 * PARTS * D;
   walk.start();
   const int L = min(max(a.seq_lens[row0], 0), a.room);
   const int pairs = (L + 31) / 32;
@@ -198,7 +232,9 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       for (int i = 0; i < QV; ++i) {
         if (a.q_vec) qraw[s][e][i] = reinterpret_cast<const uint4 *>(p)[i];
         else qraw[s][e][i] = load16_unaligned<DT>(p + 4 * i);
-        if (!in) qraw[s][e][i] = make_uint4(0, 0, 0, 0);
+        uint4 &r = qraw[s][e][i];
+        r = in ? make_uint4(r.x ^ a.q_sign, r.y ^ a.q_sign, r.z ^ a.q_sign, r.w ^ a.q_sign)
+               : make_uint4(0, 0, 0, 0);
       }
     }
 
@@ -207,7 +243,10 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int c = 0; c < 4; ++c) acc[s][c] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  float m = NEG_INF_F, l = 0.f;
+  // the sum of the weights, of the row `col`: the same products with a row of ones for V
+  floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
+  const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  float m = NO_SCORE;  // below every score: the first one moves it
 
   // A part's tile is read through a buffer descriptor that ends with its last token: what lies
   // behind, or an id outside the pool, or dims past the head, reads as 0 without a branch.
@@ -217,22 +256,25 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
     k_off[s] = 64 * s + 16 * rg < D ? col * D + 64 * s + 16 * rg : 0x7fffffffu;
     v_off[s] = 64 * s + 4 * col < D ? (rg * D + 64 * s + 4 * col) * 4 : 0x7fffffffu;
   }
-  const int tile = 16 * PARTS * D;
+  const uint8_t *kh = a.kc + (int64_t)h * 16 * PARTS * D, *vh = a.vc + (int64_t)h * 16 * PARTS * D;
   // the wave's i-th 32 tokens (nothing at and past `count`)
   auto load = [&](int i, Pair<NS> &x) {
-    const int p = first + i * step;
+    const int left = L - 32 * (first + i * step);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int from = (i * BPP + u / PARTS - walk.base) & 63;  // lane of the part's block
-      const int n = min(max(L - (32 * p + 16 * u), 0), 16);  // the part's tokens
-      const int id = __builtin_amdgcn_readlane(walk.id, from);
-      x.ok[u] = n > 0 && id >= 0 && id < a.num_blocks;
-      x.ks[u] = lane_float(walk.sc.x, from);
-      x.vs[u] = lane_float(walk.sc.y, from);
-      const int64_t at =
-          ((int64_t)(x.ok[u] ? id : 0) * H + h) * tile + (u % PARTS) * 16 * D;
-      const auto kr = tile_buffer(a.kc + at, x.ok[u] ? n * D : 0);
-      const auto vr = tile_buffer(a.vc + at, x.ok[u] ? (n + 3) / 4 * 4 * D : 0);
+      const bool in = (walk.inside >> from) & 1;
+      const int n = in ? clamp_scalar(left - 16 * u) : 0;  // the part's tokens
+      const float ks = lane_float(walk.sc.x, from), vs = lane_float(walk.sc.y, from);
+      x.ok[u] = n > 0;
+      x.ks[u] = n > 0 ? ks : 1.f;
+      x.vs[u] = n > 0 ? vs : 1.f;
+      const uint64_t at =
+          ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(walk.at >> 32), from) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)walk.at, from)) +
+          (uint32_t)((u % PARTS) * 16 * D);
+      const auto kr = tile_buffer(kh + at, n * D);
+      const auto vr = tile_buffer(vh + at, (n + 3) / 4 * 4 * D);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         x.k[u][s] =
@@ -244,63 +286,60 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   };
 
   auto consume = [&](int p, Pair<NS> &x, const uint4 (&qop)[NS][2][QT]) {
-    const bool whole = 32 * p + 32 <= L && x.ok[0] && x.ok[1];  // wave-uniform
-    float sv[2][4];
+    floatx4_t y[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      floatx4_t y = {0.f, 0.f, 0.f, 0.f};
+      y[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const uint4 w = x.k[u][s];
-        const uint2 k0 = e4m3_widen<KT>(w.x), k1 = e4m3_widen<KT>(w.y), k2 = e4m3_widen<KT>(w.z),
-                    k3 = e4m3_widen<KT>(w.w);
+        const uint2 k0 = e4m3_widen(w.x, x.ks[u]), k1 = e4m3_widen(w.y, x.ks[u]),
+                    k2 = e4m3_widen(w.z, x.ks[u]), k3 = e4m3_widen(w.w, x.ks[u]);
 #pragma unroll
         for (int t = QT - 1; t >= 0; --t) {
-          y = Mfma<KT>::qk(make_uint4(k0.x, k0.y, k1.x, k1.y), qop[s][0][t], y);
-          y = Mfma<KT>::qk(make_uint4(k2.x, k2.y, k3.x, k3.y), qop[s][1][t], y);
+          y[u] = Bf16::qk(make_uint4(k0.x, k0.y, k1.x, k1.y), qop[s][0][t], y[u]);
+          y[u] = Bf16::qk(make_uint4(k2.x, k2.y, k3.x, k3.y), qop[s][1][t], y[u]);
         }
       }
-      const float ks = x.ks[u] * a.scale_log2;
+    }
+    if (32 * p + 32 > L || !x.ok[0] || !x.ok[1]) {  // wave-uniform
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sv[u][j] = y[j] * ks;
-      if (!whole) {
+      for (int u = 0; u < 2; ++u) {
+        // what lies behind the last token must not meet a zero weight (0 * NaN)
+        const int n = x.ok[u] ? L - (32 * p + 16 * u + 4 * rg) : 0;  // tokens of the lane's four
+        const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (!(x.ok[u] && 32 * p + 16 * u + 4 * rg + j < L)) sv[u][j] = NEG_INF_F;
-        // what lies behind the last token must not meet a zero weight (0 * NaN)
-        const int n = L - (32 * p + 16 * u + 4 * rg);  // tokens of the lane's four
-        const uint32_t keep = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+          if (j >= n) y[u][j] = NEG_INF_F;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           const uint4 v = x.v[u][s];
           x.v[u][s] = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
         }
-        if (!x.ok[u]) x.vs[u] = 0.f;
       }
     }
-    float mb = fmaxf(fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[0][2], sv[0][3])),
-                     fmaxf(fmaxf(sv[1][0], sv[1][1]), fmaxf(sv[1][2], sv[1][3])));
-    mb = rows_max4(mb);
+    // (maxima that pass a NaN on: the others quiet their operands first, one by one)
+    float mb = __builtin_elementwise_maximum(
+        __builtin_elementwise_maximum(__builtin_elementwise_maximum(y[0][0], y[0][1]), y[0][2]),
+        __builtin_elementwise_maximum(
+            __builtin_elementwise_maximum(__builtin_elementwise_maximum(y[0][3], y[1][0]), y[1][1]),
+            __builtin_elementwise_maximum(y[1][2], y[1][3])));
+    mb = rows_maximum4(mb) * a.scale_log2;
     const bool need = mb > m + RESCALE_SLACK_LOG2;
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
       const float corr = need ? fast_exp2(m - mb) : 1.f;
-      l *= corr;
+      sum *= corr;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[s][c] *= corr;
       m = need ? mb : m;
     }
-    const float ms = m == NEG_INF_F ? 0.f : m;
     float w[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = fast_exp2(sv[u][j] - ms);
-        l += e;
-        w[u][j] = e * x.vs[u];
-      }
+      for (int j = 0; j < 4; ++j) w[u][j] = fast_exp2(fmaf(y[u][j], a.scale_log2, -m));
     uint4 pop[PT];
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
@@ -308,11 +347,13 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       pop[t] = make_uint4(p0.x, p0.y, p1.x, p1.y);
     }
 #pragma unroll
+    for (int t = PT - 1; t >= 0; --t) sum = Bf16::qk(ones, pop[t], sum);
+#pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const uint2 v0 = e4m3_widen<VFL_BFLOAT16>((&x.v[0][s].x)[c]);
-        const uint2 v1 = e4m3_widen<VFL_BFLOAT16>((&x.v[1][s].x)[c]);
+        const uint2 v0 = e4m3_widen((&x.v[0][s].x)[c], x.vs[0]);
+        const uint2 v1 = e4m3_widen((&x.v[1][s].x)[c], x.vs[1]);
 #pragma unroll
         for (int t = PT - 1; t >= 0; --t)
           acc[s][c] = Bf16::qk(make_uint4(v0.x, v0.y, v1.x, v1.y), pop[t], acc[s][c]);
@@ -322,22 +363,24 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   // the next 32 tokens' loads go out before the current ones are used
   uint4 qop[NS][2][QT];
   if (count > 0) {
+    constexpr bool AHEAD = NS <= 3;  // (wider heads: no registers for a second buffer)
     Pair<NS> x, y;
-    walk.start_scales();
+    walk.begin();
     load(0, x);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        if constexpr (DT != VFL_FLOAT32) {
+        if constexpr (DT == VFL_BFLOAT16) {
           qop[s][e][0] = qraw[s][e][0];
         } else {
-          float f[2][4];
-          unpack16<DT>(qraw[s][e][0], f[0]);
-          unpack16<DT>(qraw[s][e][1], f[1]);
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < QV; ++i) unpack16<DT>(qraw[s][e][i], f + 4 * i);
+          float f0[4] = {f[0], f[1], f[2], f[3]}, f1[4] = {f[4], f[5], f[6], f[7]};
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            const uint2 lo = take_bf16(f[0]), hi = take_bf16(f[1]);
+            const uint2 lo = take_bf16(f0), hi = take_bf16(f1);
             qop[s][e][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
           }
         }
@@ -347,16 +390,14 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       if (i < count && i * BPP - walk.base >= 64) walk.advance();
       load(i, z);
     };
-    for (int i = 0; i < count; i += 2) {
-      next(i + 1, y);
+    for (int i = 0; i < count; i += AHEAD ? 2 : 1) {
+      if constexpr (AHEAD) next(i + 1, y);
       consume(first + i * step, x, qop);
       if (i + 1 >= count) break;
-      next(i + 2, x);
-      consume(first + (i + 1) * step, y, qop);
+      next(AHEAD ? i + 2 : i + 1, x);
+      if constexpr (AHEAD) consume(first + (i + 1) * step, y, qop);
     }
   }
-  l = rows_sum4(l);
-
   // acc[s][c][j]: dim 64 s + 16 rg + 4 j + c of row `col`
   if (col < COLS) {
 #pragma unroll
@@ -366,19 +407,18 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           s_acc[wave][64 * s + 16 * rg + 4 * j + c][col] = acc[s][c][j];
-    if (rg == 0) s_ml[wave][0][col] = m, s_ml[wave][1][col] = l;
+    if (rg == 0) s_ml[wave][0][col] = m, s_ml[wave][1][col] = sum[0];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < nrows * D; i += 64 * NW) {
     const int r = i / D, d = i % D;
-    float M = NEG_INF_F;
+    float M = NO_SCORE;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, s_ml[w][0][r]);
-    const float Ms = M == NEG_INF_F ? 0.f : M;
     float S = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = fast_exp2(s_ml[w][0][r] - Ms);
+      const float f = fast_exp2(s_ml[w][0][r] - M);
       S = fmaf(s_ml[w][1][r], f, S);
       o = fmaf(s_acc[w][d][r], f, o);
     }
@@ -406,16 +446,15 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
   const float2 *ml = a.part.ml + at * a.splits;
   const int tid = threadIdx.x, quads = a.D / 4, teams = ATTN8_JOIN_NT / quads;
   const int team = tid / quads, quad = tid % quads;
-  float M = NEG_INF_F;
+  float M = NO_SCORE;
   for (int s = tid & 63; s < a.splits; s += 64) M = fmaxf(M, ml[s].x);
   M = wave_max64(M);
-  const float Ms = M == NEG_INF_F ? 0.f : M;
   float S = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (team < teams) {
     for (int s = team; s < a.splits; s += teams) {
       const float2 x = ml[s];
-      const float f = fast_exp2(x.x - Ms);
+      const float f = fast_exp2(x.x - M);
       const float4 v =
           *reinterpret_cast<const float4 *>(a.part.acc + (at * a.splits + s) * a.D + 4 * quad);
       S = fmaf(x.y, f, S);
@@ -542,7 +581,8 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
               (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
               block_table_stride, (int)table, (int)table * block_size, group_start, group_order,
               num_rows, num_groups, num_heads, head_dim, num_blocks,
-              scale * 1.4426950408889634f,
+              fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f),  // (0 * -inf is no score)
+              !(scale < 0.f) ? 0u : dtype == VFL_FLOAT32 ? 0x80000000u : 0x80008000u,
               (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
                   query_stride_head % (16 / eb) == 0,
               1, {nullptr, nullptr}};

@@ -37,17 +37,12 @@ __device__ __forceinline__ uint32_t e4m3_rescale(uint32_t w, float ratio) {
   return e4m3_pack(f);
 }
 
-// Four values as 16-bit elements of DT (bf16 and fp16 hold every e4m3 value exactly).
-template <int DT> __device__ __forceinline__ uint2 e4m3_widen(uint32_t w);
-template <> __device__ __forceinline__ uint2 e4m3_widen<VFL_BFLOAT16>(uint32_t w) {
+// Four values times `scale`, a power of two whose exponent the conversion adds, as bf16
+// (exact: bf16 holds every e4m3 value and fp32's exponents).
+__device__ __forceinline__ uint2 e4m3_widen(uint32_t w, float scale) {
   return make_uint2(
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)));
-}
-template <> __device__ __forceinline__ uint2 e4m3_widen<VFL_FLOAT16>(uint32_t w) {
-  return make_uint2(
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
-      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)));
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)));
 }
 
 // Shared argument checks of the 8-bit cache's entry points (kv_cache_8bit.hip).
