@@ -519,7 +519,7 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * where max is over the run's finite values and old = 0 when the run holds the block's first
  * slot: the block then starts over, and its other slots become 0.  Else they become rnd(q *
  * old / new).  A token's elements are rnd(x / new), to nearest even, NaN for an infinity or
- * a NaN.  At most 2^31 - 1 tokens and 65535 heads.
+ * a NaN.  Tokens x heads below 2^31, at most 2^31 - 1 blocks and 65535 heads.
  *
  * vfl_attention_with_kv_cache_8bit: vfl_attention_with_kv_cache over such a cache; groups
  * (group_start) are rows sharing one table, at most 8 of them, block_table lists

@@ -83,13 +83,14 @@ def test_append_prompts_then_steps(dtype):
         same_cache(want, cache)
 
 
-@pytest.mark.parametrize("count,bs", [(1, 16), (700, 16), (5000, 16), (5000, 32)])
-def test_append_many_runs(count, bs):
+@pytest.mark.parametrize("count,bs,dim", [(1, 16, 64), (511, 16, 64), (512, 16, 64), (513, 16, 64),
+                                          (1100, 16, 192), (5000, 16, 64), (5000, 32, 64)])
+def test_append_many_runs(count, bs, dim):
     """Calls from one token to many, runs at every place of the call, an odd head count."""
     from vflorence_amd import hip_attn
 
     gen = torch.Generator().manual_seed(count)
-    heads, dim = 5, 64
+    heads = 5
     slots, block = [], 0
     while len(slots) < count:
         n = int(torch.randint(1, 3 * bs, (1,), generator=gen))
@@ -127,6 +128,26 @@ def test_append_special_values(dtype):
     key[4, 0, 63] = 448.0
     slots = torch.tensor([0, 16, 32, 48, 64, 83, 83])
     key, value = key.to(dtype).to(DEV), value.to(dtype).to(DEV)
+    hip_attn.reshape_and_cache_8bit(key, value, *cache, slots.to(DEV))
+    want.append(key, value, slots)
+    same_cache(want, cache)
+
+
+@pytest.mark.parametrize("dim,bs", [(64, 16), (128, 32), (48, 16)])
+def test_append_out_of_order_and_repeated_slots(dim, bs):
+    """A run in any order, longer than a wave, with slots that come again: the later token is
+    stored, every one counts for the scale."""
+    from vflorence_amd import hip_attn
+
+    gen = torch.Generator().manual_seed(dim)
+    cache = random_cache(gen, 5, 2, bs, dim)
+    want = Cache.of(*cache)
+    blocks = [(2, torch.randint(1, bs, (9,), generator=gen)),
+              (0, torch.randint(0, bs, (150,), generator=gen)), (4, torch.arange(bs).flip(0)),
+              (1, torch.tensor([3, 3, 5, 3]))]
+    slots = torch.cat([b * bs + o for b, o in blocks])
+    key, value = tokens_of(gen, len(slots), 2, dim, torch.bfloat16)
+    key[-3] *= 64.0  # overwritten by the last token
     hip_attn.reshape_and_cache_8bit(key, value, *cache, slots.to(DEV))
     want.append(key, value, slots)
     same_cache(want, cache)

@@ -10,6 +10,11 @@
 // grows later loses nothing but what falls under e4m3's smallest step: no value's error
 // grows with the number of appends, which any other scale would cost.  Infinities and NaN
 // become NaN and leave the scale alone.
+//
+// What bounds it: prompts HBM (64 prompts of 256 to 1024 tokens x 16 heads, bf16: 54.6 us,
+// 4.6 TB/s read and written); steps their chain of slots, rows and stores (256 rows x 16 heads
+// 5.2 us, 4 x 12 3.3 us).  The heads of a block run on one XCD, whose L2 then writes the block's
+// line of scales whole.
 #include <stdio.h>
 
 #include "e4m3.h"
@@ -22,7 +27,7 @@ int check_8bit_cache(const char *who, int dtype, int num_heads, int head_dim, in
     set_error("%s: unsupported dtype code %d", who, dtype);
     return VFL_E_INVALID;
   }
-  if (num_heads <= 0 || num_heads > 65535 || num_blocks < 0) {
+  if (num_heads <= 0 || num_heads > 65535 || num_blocks < 0 || num_blocks > 2147483647LL) {
     set_error("%s: bad sizes (heads %d blocks %lld)", who, num_heads, (long long)num_blocks);
     return VFL_E_INVALID;
   }
@@ -63,8 +68,8 @@ __device__ __forceinline__ float finite_abs(float &x) {
   return 0.f;
 }
 
-// A workgroup takes the runs that begin among `window` tokens, for one head; its NS waves
-// take 64 dims each and share the maxima through LDS.  PARTS: 16-token parts of a block.
+// A workgroup takes the runs that begin among `window` tokens (up to 32), for one head; its NS
+// waves take 64 dims each and share the maxima through LDS.  PARTS: 16-token parts of a block.
 // K: lane = (token l / 4 of a part, dims 16 (l % 4) ..), a row's 16 values per 16-byte
 // store.  V: lane = (tokens 4 (l / 16) .. + 3, dims 4 (l % 16) .. + 3), whose 16 bytes lie
 // together in the token-interleaved pool.
@@ -73,63 +78,117 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     const typename Elem<DT>::T *__restrict__ key, const typename Elem<DT>::T *__restrict__ value,
     int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, uint8_t *__restrict__ kc,
     uint8_t *__restrict__ vc, float *__restrict__ scales, const int64_t *__restrict__ slots,
-    int64_t T, int H, int D, int64_t num_blocks, int window) {
+    int T, int H, int D, int num_blocks, int window) {
   constexpr int BS = 16 * PARTS;
   __shared__ float s_max[2][NS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.y;
-  const int64_t t0 = (int64_t)blockIdx.x * window;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t pos;
+  int h;
+  xcd_position(blockIdx.x, (unsigned)H, pos, h);  // a block's scales: written through one L2
+  if (pos * window >= T) return;
+  const int t0 = (int)pos * window;
   const int kd = 64 * wave + 16 * (lane & 3), vd = 64 * wave + 4 * (lane & 15);
   const bool k_in = kd < D, v_in = vd < D;
 
-  // block of a slot, -1 for a slot that is skipped
+  // Lane l: block and offset of token t0 - 1 + l (block -1: skipped, or no token).  One load
+  // covers the window, the token before it and the rest of its last run.
   auto block_of = [&](int64_t slot) {
-    return slot >= 0 && slot < num_blocks * BS ? slot / BS : (int64_t)-1;
+    return slot >= 0 && slot < (int64_t)num_blocks * BS ? (int)(slot / BS) : -1;
   };
-  // first tokens of runs, one lane per token of the window
-  const int64_t tl = t0 + lane;
-  const bool mine = lane < window && tl < T;
-  const int64_t bl = mine ? block_of(slots[tl]) : -1;
-  const int64_t before = mine && tl > 0 ? block_of(slots[tl - 1]) : -1;
-  uint64_t leaders = __builtin_amdgcn_ballot_w64(bl >= 0 && bl != before);
+  const int tl = t0 - 1 + lane;
+  const int64_t slot = slots[min(max(tl, 0), T - 1)];
+  const int bl = tl >= 0 && tl < T ? block_of(slot) : -1;
+  const int off = (int)(slot & (BS - 1));
+  const int before = __shfl_up(bl, 1);
+  uint64_t leaders = __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= window && bl >= 0 &&
+                                                 bl != before);
 
   for (; leaders; leaders &= leaders - 1) {
-    const int64_t t = t0 + __builtin_ctzll(leaders);
-    const int64_t blk = block_of(slots[t]);
+    const int at = __builtin_ctzll(leaders), t = t0 - 1 + at;
+    const int blk = __builtin_amdgcn_readlane(bl, at);
     // lane o: the run's token that takes the block's offset o (its last one), from t on
+    const uint64_t differ = ~(__builtin_amdgcn_ballot_w64(bl == blk) >> at);
+    const int n = differ ? __builtin_ctzll(differ) : 64;
+    const int off0 = __builtin_amdgcn_readlane(off, at);
     int src = -1;
-    for (int64_t base = t;; base += 64) {
-      const int64_t s = base + lane < T ? slots[base + lane] : -1;
-      const uint64_t same = __builtin_amdgcn_ballot_w64(block_of(s) == blk);
-      const int n = same == ~0ull ? 64 : __builtin_ctzll(~same);
-      const int off = (int)(s & (BS - 1));
-      for (int i = 0; i < n; ++i)
-        if (__builtin_amdgcn_readlane(off, i) == lane) src = (int)(base - t) + i;
-      if (n < 64) break;
+    float km = 0.f, vm = 0.f;
+    if (at + n < 64 && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
+                                                   off != off0 + lane - at) == 0) {
+      src = lane >= off0 && lane < off0 + n ? lane - off0 : -1;  // in order
+    } else {
+      // any order, slots that come twice: the later token is stored, both count for the scale
+      for (int i = 0; t + i < T; ++i) {
+        const int64_t s = slots[t + i];
+        if (block_of(s) != blk) break;
+        if ((int)(s & (BS - 1)) == lane) src = i;
+        if (64 * wave + lane < D) {
+          float x, y;
+          load_elems<DT, false, 1>(key + (t + i) * k_st + h * k_sh + 64 * wave + lane, &x);
+          load_elems<DT, false, 1>(value + (t + i) * v_st + h * v_sh + 64 * wave + lane, &y);
+          km = fmaxf(km, finite_abs(x)), vm = fmaxf(vm, finite_abs(y));
+        }
+      }
     }
     const bool fresh = __builtin_amdgcn_readlane(src, 0) >= 0;
-    float *sc = scales + 2 * (blk * H + h);
+    float *sc = scales + 2 * ((int64_t)blk * H + h);
     const float old_k = fresh ? 0.f : sc[0], old_v = fresh ? 0.f : sc[1];
 
     float kx[PARTS][16], vx[PARTS][4][4];
     int ks[PARTS], vs[PARTS][4];
-    float km = 0.f, vm = 0.f;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
       ks[p] = __shfl(src, 16 * p + (lane >> 2));
-      if (ks[p] >= 0 && k_in) {
-        load_elems<DT, ALIGNED, 16>(key + (t + ks[p]) * k_st + h * k_sh + kd, kx[p]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) km = fmaxf(km, finite_abs(kx[p][i]));
-      }
+      if (!k_in) ks[p] = -1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         vs[p][j] = __shfl(src, 16 * p + 4 * (lane >> 4) + j);
-        if (vs[p][j] >= 0 && v_in) {
-          load_elems<DT, ALIGNED, 4>(value + (t + vs[p][j]) * v_st + h * v_sh + vd, vx[p][j]);
+        if (!v_in) vs[p][j] = -1;
+      }
+    }
+    auto k_row = [&](int p, int i) {
+      load_elems<DT, ALIGNED, 16>(key + (t + i) * k_st + h * k_sh + (k_in ? kd : 0), kx[p]);
+    };
+    auto v_row = [&](int p, int j, int i) {
+      load_elems<DT, ALIGNED, 4>(value + (t + i) * v_st + h * v_sh + (v_in ? vd : 0), vx[p][j]);
+    };
+    auto k_max = [&](int p) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vm = fmaxf(vm, finite_abs(vx[p][j][i]));
+      for (int i = 0; i < 16; ++i) km = fmaxf(km, finite_abs(kx[p][i]));
+    };
+    auto v_max = [&](int p, int j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vm = fmaxf(vm, finite_abs(vx[p][j][i]));
+    };
+    if (n > 1) {
+      // every lane reads some row of the run (what repeats changes no maximum): a load under a
+      // condition would wait for the one before
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        k_row(p, max(ks[p], 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v_row(p, j, max(vs[p][j], 0));
+      }
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        k_max(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v_max(p, j);
+      }
+    } else {
+      // one token: the few lanes that hold it (256 rows x 16 heads 5.4 against 7.2 us)
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        if (ks[p] >= 0) {
+          k_row(p, 0);
+          k_max(p);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (vs[p][j] >= 0) {
+            v_row(p, j, 0);
+            v_max(p, j);
+          }
       }
     }
     km = wave_max64(km);
@@ -146,7 +205,7 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
     const float ratio_k = old_k * inv_k, ratio_v = old_v * inv_v;
 
-    const int64_t tile = (blk * H + h) * (int64_t)(BS * D);
+    const int64_t tile = ((int64_t)blk * H + h) * (BS * D);
     uint8_t *kt = kc + tile, *vt = vc + tile;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
@@ -212,19 +271,28 @@ static void launch_append_steps(int steps, dim3 grid, hipStream_t stream, A... a
 #undef VFL_APPEND
 }
 
+// Tokens whose runs a workgroup takes.  A decode step's tokens are runs of their own and want
+// a workgroup each; a prompt's come 16 a block.  The host does not see which they are: calls of
+// up to 512 tokens (the most rows of a step that the projections take) get one, longer ones 16.
+// Windows of 1 and of 16, us, bf16: steps of 256 and 512 rows x 16 heads 5.2 / 23.7 and 7.6 /
+// 25.2, of 2048 rows 23 / 36; a prompt of 590 tokens x 12 heads 7.4 / 3.5, 64 prompts of 256 to
+// 1024 tokens x 16 heads 177 / 54.6.
+inline int append_window(int64_t T) { return T <= 512 ? 1 : 16; }
+
 template <int DT>
 static int launch_append(bool aligned, const void *key, const void *value, int64_t k_st,
                          int64_t k_sh, int64_t v_st, int64_t v_sh, void *kc, void *vc,
                          float *scales, const int64_t *slots, int64_t T, int H, int D, int BS,
                          int64_t num_blocks, hipStream_t stream) {
   using E = typename Elem<DT>::T;
-  const int window = 1;
-  const dim3 grid((unsigned)((T + window - 1) / window), (unsigned)H);
+  const int window = append_window(T);
+  const dim3 grid((unsigned)xcd_grid((T + window - 1) / window, H));
   const int steps = (D + 63) / 64;
   auto go = [&](auto al, auto parts) {
     launch_append_steps<DT, decltype(al)::value, decltype(parts)::value>(
         steps, grid, stream, (const E *)key, (const E *)value, k_st, k_sh, v_st, v_sh,
-        (uint8_t *)kc, (uint8_t *)vc, scales, slots, T, H, D, num_blocks, window);
+        (uint8_t *)kc, (uint8_t *)vc, scales, slots, (int)T, H, D, (int)num_blocks,
+        window);
   };
   using std::integral_constant;
   if (aligned) {
@@ -252,8 +320,8 @@ extern "C" int vfl_reshape_and_cache_8bit(const void *key, const void *value,
   const int st = check_8bit_cache("reshape_and_cache_8bit", dtype, num_heads, head_dim,
                                   block_size, num_blocks);
   if (st != VFL_OK) return st;
-  if (num_tokens < 0 || num_tokens > 2147483647LL) {
-    set_error("reshape_and_cache_8bit: %lld tokens", (long long)num_tokens);
+  if (num_tokens < 0 || (num_tokens + XCDS) * num_heads > 2147483647LL) {
+    set_error("reshape_and_cache_8bit: %lld tokens x %d heads", (long long)num_tokens, num_heads);
     return VFL_E_INVALID;
   }
   if (num_tokens == 0 || num_blocks == 0) return VFL_OK;

@@ -21,7 +21,7 @@ import functools
 import torch
 
 from ._lib import check, lib
-from .hip_attn import (_dtype_code, _require_gpu, _stream, on_current_device, on_device,
+from .hip_attn import (_dtype_code, _require_gpu, _stream, on_current_device, on_device, one_gpu,
                        plain_eager, refuse_gradients)
 
 # largest k of logprob_topk (each lane keeps its k best in registers)
@@ -554,9 +554,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
     if not 0 < vocab <= MAX_SCORED_VOCAB:
         raise ValueError(f"vocab must be in [1, {MAX_SCORED_VOCAB}], got {vocab}")
     dtype = _dtype_code(logits.dtype)
-    dev = _require_gpu(logits, tokens)
+    index = one_gpu(logits, tokens)
     refuse_gradients("token_logprobs", logits)
     tokens = tokens.contiguous()
+    dev = logits.device
     logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
     entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     top = ids = None
@@ -567,7 +568,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
     need = _logprobs_workspace(vocab, dtype, k)
     if need:
         workspace = torch.empty(rows * need, dtype=torch.uint8, device=dev)
-    on_device(logits, lib.vfl_token_logprobs, logits.data_ptr(), logits.stride(0), rows, vocab,
+    on_device(index, lib.vfl_token_logprobs, logits.data_ptr(), logits.stride(0), rows, vocab,
               dtype, tokens.data_ptr(), tokens.shape[1] if tokens.dim() == 2 else 1, k,
               logprobs.data_ptr(), entropy.data_ptr(), top.data_ptr() if k else None,
               ids.data_ptr() if k else None, workspace.data_ptr() if need else None)

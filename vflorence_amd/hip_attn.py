@@ -840,14 +840,23 @@ def refuse_gradients(name: str, *tensors: torch.Tensor) -> None:
         raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad()")
 
 
-def on_device(tensor: torch.Tensor, function, *args) -> None:
-    """A checked C-ABI call on ``tensor``'s device and its current stream, the last argument
-    (a null stream handle, every default stream's, means the current device's)."""
-    if on_current_device(tensor):
-        check(function(*args, _stream(tensor.device)))
+def one_gpu(*tensors: torch.Tensor) -> int:
+    """The index of the GPU that holds all of the tensors (``_require_gpu``'s errors; integers,
+    as device objects cost a small call 2 us)."""
+    index = tensors[0].get_device()
+    if index < 0 or any(t.get_device() != index for t in tensors):
+        _require_gpu(*tensors)
+    return index
+
+
+def on_device(index: int, function, *args) -> None:
+    """A checked C-ABI call on a GPU and its current stream, the last argument (a null stream
+    handle, every default stream's, means the current device's)."""
+    if index == torch.cuda.current_device():
+        check(function(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
-        with torch.cuda.device(tensor.device):
-            check(function(*args, _stream(tensor.device)))
+        with torch.cuda.device(index):
+            check(function(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -877,10 +886,10 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],):
         raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
                          f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
-    _require_gpu(key, value, k_cache, v_cache, kv_scales, slot_mapping)
+    index = one_gpu(key, value, k_cache, v_cache, kv_scales, slot_mapping)
     refuse_gradients("reshape_and_cache_8bit", key, value)
     slot_mapping = slot_mapping.contiguous()
-    on_device(key, lib.vfl_reshape_and_cache_8bit, key.data_ptr(), value.data_ptr(),
+    on_device(index, lib.vfl_reshape_and_cache_8bit, key.data_ptr(), value.data_ptr(),
               key.stride(0), key.stride(1), value.stride(0), value.stride(1),
               k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
               slot_mapping.data_ptr(), key.shape[0], num_heads, head_dim, block_size, num_blocks,
@@ -921,7 +930,7 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
             or block_table.shape[0] != num_rows):
         raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
                          f"{block_table.dtype} {tuple(block_table.shape)}")
-    _require_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
+    index = one_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
     refuse_gradients("attention_with_kv_cache_8bit", query, out)
     if block_table.stride(1) != 1:
         block_table = block_table.contiguous()
@@ -938,11 +947,13 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                              "self_attention_with_kv_write alone")
         if not sm.own_tables or sm.group_start is None:
             start, order, num_groups = sm.group_start, sm.group_order, sm.num_groups
-        _require_gpu(query, *(t for t in (start, order) if t is not None))
+        for t in (start, order):
+            if t is not None:
+                one_gpu(query, t)
     width = block_table.shape[1]
     need = _attention_8bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    on_device(query, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
+    on_device(index, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
               query.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
               out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
               width, None if start is None else start.data_ptr(),
