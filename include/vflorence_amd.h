@@ -511,8 +511,8 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * operands beside them.  No vllm_cpu_attn counterpart.
  *
  * vfl_reshape_and_cache_8bit: vfl_reshape_and_cache into such a cache, same slots and strides.
- * Consecutive tokens whose slots lie in one block are a run; a block's tokens must form one
- * run of the call, and a block belong to one sequence (a second run in the call, or a call
+ * Consecutive tokens whose slots lie in one block are a run (of a slot that comes twice in it,
+ * the later token); a block's tokens must form one run of the call, and a block belong to one sequence (a second run in the call, or a call
  * that overlaps this one on another stream, would race for the block's scale).  Per run
  * and head, for K and for V,
  *   new = max(old, the smallest power of two with max |x| / new <= 448)   (2^-100 at least)

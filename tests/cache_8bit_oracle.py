@@ -50,9 +50,10 @@ class Cache:
             block, j = slots[i] // bs, i
             while j < len(slots) and 0 <= slots[j] < nb * bs and slots[j] // bs == block:
                 j += 1
-            offsets = [s % bs for s in slots[i:j]]
+            taken = {s % bs: t for t, s in enumerate(slots[i:j], i)}  # offset: its last token
+            offsets = list(taken)
             for n, x in enumerate((key, value)):
-                x = x[i:j].double().cpu()
+                x = x[list(taken.values())].double().cpu()
                 for h in range(heads):
                     old = 0.0 if 0 in offsets else float(self.scales[block, h, n])
                     new = max(old, needed_scale(x[:, h]))

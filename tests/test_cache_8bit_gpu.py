@@ -136,7 +136,7 @@ def test_append_special_values(dtype):
 @pytest.mark.parametrize("dim,bs", [(64, 16), (128, 32), (48, 16)])
 def test_append_out_of_order_and_repeated_slots(dim, bs):
     """A run in any order, longer than a wave, with slots that come again: the later token is
-    stored, every one counts for the scale."""
+    taken, the earlier one does not count for the scale either."""
     from vflorence_amd import hip_attn
 
     gen = torch.Generator().manual_seed(dim)

@@ -1,7 +1,8 @@
 // Appending keys and values to a paged cache held in e4m3, one scale per (block, head) for
 // K and one for V (gfx950).
 //
-// A run is the consecutive tokens of a call whose slots lie in one block.  Per run and head
+// A run is the consecutive tokens of a call whose slots lie in one block (of a slot that comes
+// twice, the later token).  Per run and head
 //   a = max |x| over the run's finite values,  need = the smallest power of two with
 //   a / need <= 448,  new = max(old, need)  (old = 0 where the run holds the block's offset
 //   0: the block starts over, what it held is dropped)
@@ -111,23 +112,17 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     const uint64_t differ = ~(__builtin_amdgcn_ballot_w64(bl == blk) >> at);
     const int n = differ ? __builtin_ctzll(differ) : 64;
     const int off0 = __builtin_amdgcn_readlane(off, at);
-    int src = -1;
-    float km = 0.f, vm = 0.f;
+    int src = -1, last = n - 1;  // (the last token is always taken)
     if (at + n < 64 && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
                                                    off != off0 + lane - at) == 0) {
       src = lane >= off0 && lane < off0 + n ? lane - off0 : -1;  // in order
     } else {
-      // any order, slots that come twice: the later token is stored, both count for the scale
+      // any order; of a slot that comes twice the later token is taken
       for (int i = 0; t + i < T; ++i) {
         const int64_t s = slots[t + i];
         if (block_of(s) != blk) break;
         if ((int)(s & (BS - 1)) == lane) src = i;
-        if (64 * wave + lane < D) {
-          float x, y;
-          load_elems<DT, false, 1>(key + (t + i) * k_st + h * k_sh + 64 * wave + lane, &x);
-          load_elems<DT, false, 1>(value + (t + i) * v_st + h * v_sh + 64 * wave + lane, &y);
-          km = fmaxf(km, finite_abs(x)), vm = fmaxf(vm, finite_abs(y));
-        }
+        last = i;
       }
     }
     const bool fresh = __builtin_amdgcn_readlane(src, 0) >= 0;
@@ -146,6 +141,7 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
         if (!v_in) vs[p][j] = -1;
       }
     }
+    float km = 0.f, vm = 0.f;
     auto k_row = [&](int p, int i) {
       load_elems<DT, ALIGNED, 16>(key + (t + i) * k_st + h * k_sh + (k_in ? kd : 0), kx[p]);
     };
@@ -161,13 +157,13 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
       for (int i = 0; i < 4; ++i) vm = fmaxf(vm, finite_abs(vx[p][j][i]));
     };
     if (n > 1) {
-      // every lane reads some row of the run (what repeats changes no maximum): a load under a
-      // condition would wait for the one before
+      // every lane reads some row that is taken (what repeats changes no maximum): a load under
+      // a condition would wait for the one before
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        k_row(p, max(ks[p], 0));
+        k_row(p, ks[p] < 0 ? last : ks[p]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v_row(p, j, max(vs[p][j], 0));
+        for (int j = 0; j < 4; ++j) v_row(p, j, vs[p][j] < 0 ? last : vs[p][j]);
       }
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
@@ -272,12 +268,13 @@ static void launch_append_steps(int steps, dim3 grid, hipStream_t stream, A... a
 }
 
 // Tokens whose runs a workgroup takes.  A decode step's tokens are runs of their own and want
-// a workgroup each; a prompt's come 16 a block.  The host does not see which they are: calls of
-// up to 512 tokens (the most rows of a step that the projections take) get one, longer ones 16.
-// Windows of 1 and of 16, us, bf16: steps of 256 and 512 rows x 16 heads 5.2 / 23.7 and 7.6 /
-// 25.2, of 2048 rows 23 / 36; a prompt of 590 tokens x 12 heads 7.4 / 3.5, 64 prompts of 256 to
-// 1024 tokens x 16 heads 177 / 54.6.
-inline int append_window(int64_t T) { return T <= 512 ? 1 : 16; }
+// a workgroup each; a prompt's fill blocks.  The host does not see which they are: calls of up
+// to 512 tokens (the most rows of a step that the projections take) get one, longer ones a
+// block's.  Windows of 1 and of 16, us, bf16: steps of 256 and 512 rows x 16 heads 5.2 / 23.7 and
+// 7.6 / 25.2, of 2048 rows 23 / 36; a prompt of 590 tokens x 12 heads 7.4 / 3.5, 64 prompts of
+// 256 to 1024 tokens x 16 heads 177 / 54.6; the same in blocks of 32, windows of 16 and 32, 63.5
+// / 54.8.
+inline int append_window(int64_t T, int BS) { return T <= 512 ? 1 : BS; }
 
 template <int DT>
 static int launch_append(bool aligned, const void *key, const void *value, int64_t k_st,
@@ -285,7 +282,7 @@ static int launch_append(bool aligned, const void *key, const void *value, int64
                          float *scales, const int64_t *slots, int64_t T, int H, int D, int BS,
                          int64_t num_blocks, hipStream_t stream) {
   using E = typename Elem<DT>::T;
-  const int window = append_window(T);
+  const int window = append_window(T, BS);
   const dim3 grid((unsigned)xcd_grid((T + window - 1) / window, H));
   const int steps = (D + 63) / 64;
   auto go = [&](auto al, auto parts) {

@@ -867,8 +867,8 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
     key/value: [T, H, D] in float32, bfloat16 or float16, any token and head strides, a
     contiguous last dimension.  slot_mapping: int64 [T]; a token whose slot is negative or
     past the pool is skipped.  A block's tokens of one call must follow one another in it
-    (as positions of a sequence do), a block appended to must belong to one sequence, and
-    a slot that comes twice takes the later token.
+    (as positions of a sequence do), and a block appended to must belong to one sequence.
+    Of a slot that comes twice in a block's run, the later token is taken.
 
     A block's scale is a power of two that brings its largest value to 448 or less.  It only
     grows: what the block holds is then rescaled, exactly but for values under e4m3's smallest
