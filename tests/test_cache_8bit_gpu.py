@@ -382,6 +382,61 @@ def test_attention_strided_query_and_rows_left_alone():
     close(query[:3], out[:3], Cache.of(*cache), lens[:3], tables[:3], 0.125)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-6])
+def test_attention_any_finite_scale(dtype, scale):
+    from vflorence_amd import hip_attn
+
+    query, cache, lens, tables, dev, _ = paged_case(13, dtype, 80, 16, [0, 1, 37, 260])
+    out = torch.empty_like(query)
+    hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=scale,
+                                          block_table=dev[1])
+    close(query, out, Cache.of(*cache), lens, tables, scale)
+    for bad in (float("nan"), float("inf")):
+        with pytest.raises(RuntimeError, match="scale"):
+            hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=bad,
+                                                  block_table=dev[1])
+
+
+@pytest.mark.parametrize("length", [45, 6000])
+def test_attention_in_place_and_broadcast_tables(length):
+    """The output written over the query; rows that share one expanded table and length; a
+    single row whose strides say nothing."""
+    from vflorence_amd import hip_attn
+
+    query, cache, lens, tables, dev, _ = paged_case(14, torch.bfloat16, 64, 16, [length], 3)
+    want = Cache.of(*cache)
+    table = dev[1][:1].expand(3, -1)
+    out = query.clone()
+    hip_attn.attention_with_kv_cache_8bit(out, *cache, out, dev[0][:1].expand(3), scale=0.125,
+                                          block_table=table)
+    close(query, out, want, lens, tables, 0.125)
+    one = query[:1].as_strided((1, 2, 64), (7, 64, 1))
+    out = torch.empty_like(query[:1])
+    hip_attn.attention_with_kv_cache_8bit(
+        one, *cache, out, dev[0][:1], scale=0.125,
+        block_table=dev[1][:1].as_strided((1, dev[1].shape[1]), (0, 1)))
+    close(query[:1], out, want, lens[:1], tables[:1], 0.125)
+
+
+def test_attention_over_nothing():
+    """A table without columns, a pool without blocks: rows of zeros."""
+    from vflorence_amd import hip_attn
+
+    query, cache, lens, _, dev, _ = paged_case(15, torch.bfloat16, 64, 16, [20, 3])
+    out = torch.full_like(query, 7.0)
+    hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=0.125,
+                                          block_table=dev[1][:, :0])
+    assert (out == 0).all()
+    empty = hip_attn.kv_cache_8bit(0, 2, 16, 64, DEV)
+    out = torch.full_like(query, 7.0)
+    hip_attn.attention_with_kv_cache_8bit(query, *empty, out, dev[0], scale=0.125,
+                                          block_table=dev[1])
+    assert (out == 0).all()
+    key = torch.ones(2, 2, 64, device=DEV)
+    hip_attn.reshape_and_cache_8bit(key, key, *empty, torch.tensor([0, 5], device=DEV))
+
+
 @pytest.mark.parametrize("lens,beams", [([700, 20, 333], 4), ([9001], 2)])
 def test_graph_of_append_and_attention(lens, beams):
     """Captured once, replayed over new tokens with eager work of the same kind between:

@@ -153,6 +153,8 @@ def test_c_entries_check_before_launch():
     assert append(dt=3) == -1 and b"dtype" in lib.vfl_last_error()
     assert append(dim=72) == -2 and append(bs=24) == -2 and append(bs=8) == -2
     assert append(tokens=-1) == -1 and append(tokens=1 << 31) == -1
+    assert append(tokens=1 << 30, heads=64) == -1 and append(nb=1 << 31) == -1
+    assert append(tokens=1 << 29, heads=3, dim=512) == -1  # more threads than a launch takes
     assert append(heads=0) == -1 and append(heads=65536) == -1 and append(nb=-1) == -1
     for bad in (dict(key=None), dict(kc=None), dict(vc=None), dict(sc=None), dict(slots=None)):
         assert append(**bad) == -1 and b"null" in lib.vfl_last_error()
@@ -161,17 +163,18 @@ def test_c_entries_check_before_launch():
         assert append(**bad) == -1 and b"misaligned" in lib.vfl_last_error()
 
     def attend(q=A, kc=A, vc=A, sc=A, out=A, lens=A, bt=A, stride=8, width=8, starts=None, rows=4,
-               groups=4, heads=2, dim=64, bs=16, nb=10, dt=1, ws=None):
+               groups=4, heads=2, dim=64, bs=16, nb=10, dt=1, ws=None, scale=0.125):
         return lib.vfl_attention_with_kv_cache_8bit(q, 128, 64, kc, vc, sc, out, lens, bt, stride,
                                                     width, starts, None, rows, groups, heads, dim,
-                                                    bs, nb, 0.125, dt, ws, None)
+                                                    bs, nb, scale, dt, ws, None)
 
     assert attend(rows=0, groups=0) == 0 and attend(groups=0, starts=A) == 0
     assert attend(dt=3) == -1 and attend(dim=72) == -2 and attend(bs=48) == -2
     assert attend(rows=-1) == -1 and attend(groups=5) == -1 and attend(groups=3) == -1
     assert attend(width=-1) == -1 and attend(stride=7) == -1
     assert attend(width=1 << 28, stride=1 << 28) == -1  # more tokens than an int counts
-    assert attend(rows=1 << 30, groups=1 << 30) == -1
+    assert attend(rows=1 << 30, groups=1 << 30) == -1  # more threads than a launch takes
+    assert attend(scale=float("nan")) == -1 and attend(scale=float("inf")) == -1
     for bad in (dict(q=None), dict(kc=None), dict(vc=None), dict(sc=None), dict(out=None),
                 dict(lens=None), dict(bt=None)):
         assert attend(**bad) == -1 and b"null" in lib.vfl_last_error()
@@ -193,7 +196,8 @@ def test_c_entries_check_before_launch():
     assert score(rows=0) == 0
     assert score(dt=5) == -1 and score(vocab=0) == -1 and score(stride=99) == -1
     assert score(k=-1) == -1 and score(k=21) == -1 and score(vocab=5, k=6) == -1
-    assert score(rows=-1) == -1 and score(n=-1) == -1
+    assert score(rows=-1) == -1 and score(n=-1) == -1 and score(rows=1 << 22) == -1
+    assert score(x=None, stride=0) == -1  # (a stride of 0 is one row repeated)
     assert score(x=None) == -1 and score(ent=None) == -1 and score(tokens=None) == -1
     assert score(lp=None) == -1 and score(k=2, top=None) == -1 and score(k=2, ids=None) == -1
     assert score(x=A + 1) == -1

@@ -190,6 +190,17 @@ def test_rows_below_zero(dtype, vocab):
         assert all(torch.equal(a, b) for a, b in zip(got, score(logits, tokens, 20)))
 
 
+@pytest.mark.parametrize("vocab", [1003, 50265, 130001])
+def test_broadcast_rows(vocab):
+    """One row repeated by a stride of 0, and a single row whose stride says nothing."""
+    logits, _ = case(1, vocab, torch.bfloat16)
+    tokens = torch.arange(5, device=DEV)
+    wide = logits.expand(5, -1)
+    check(wide, tokens, 4, score(wide, tokens, 4))
+    one = logits.as_strided((1, vocab), (3, 1))
+    check(one, tokens[:1], 4, score(one, tokens[:1], 4))
+
+
 def test_best_values_side_by_side():
     """All alternatives inside one thread's share of the row, ascending, and at its ends."""
     for vocab in (3000, 50265, 130001):

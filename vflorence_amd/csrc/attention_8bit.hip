@@ -16,6 +16,7 @@
 // Queries go in as bf16 terms, which hold all of their bits: one of bf16, two of fp16, three of
 // fp32.  Weights as two terms, 2^-17 relative, or three for fp32 outputs, 2^-25: below the
 // output's rounding.  Their sum is the same product with a row of ones.
+#include <math.h>
 #include <stdio.h>
 
 #include "e4m3.h"
@@ -117,6 +118,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *p, 
                                            0x00020000);
 }
 
+// Pages are read once a launch: non-temporal loads (64 x 4 rows x 16 heads, 2048 tokens: 46.2
+// against 53.7 us, 5.8 TB/s; up to 1024 tokens, 85 MB, no change).
+__device__ __forceinline__ uint4 tile_load(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+  constexpr int NON_TEMPORAL = 2;
+  return __builtin_bit_cast(uint4,
+                            __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, NON_TEMPORAL));
+}
+
 // x limited to 0 .. 16, on the scalar unit (a median of three would go to the vector unit, and
 // wait there for the registers of loads in flight).
 __device__ __forceinline__ int clamp_scalar(int x) {
@@ -153,9 +162,6 @@ struct Attn8Args {
 
 constexpr int ATTN8_COLS = 8;  // rows of a group
 constexpr float NO_SCORE = -3e38f;
-// Pages are read once a launch: non-temporal loads (64 x 4 rows x 16 heads, 2048 tokens: 46.2
-// against 53.7 us, 5.8 TB/s; to 1024 tokens, 85 MB, no change).
-constexpr int NT_LOAD = 2;
 
 // Maximum across the four 16-lane rows, a NaN passed on.
 __device__ __forceinline__ float rows_maximum4(float x) {
@@ -280,10 +286,8 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
       const auto vr = tile_buffer(vh + at, (n + 3) / 4 * 4 * D);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        x.k[u][s] =
-            __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[s], 0, NT_LOAD));
-        x.v[u][s] =
-            __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[s], 0, NT_LOAD));
+        x.k[u][s] = tile_load(kr, k_off[s]);
+        x.v[u][s] = tile_load(vr, v_off[s]);
       }
     }
   };
@@ -558,12 +562,15 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
   if (st != VFL_OK) return st;
   if (num_rows < 0 || num_groups < 0 || num_groups > num_rows ||
       (!group_start && num_groups != num_rows) || max_blocks_per_seq < 0 ||
-      max_blocks_per_seq > (2147483647LL - 64) / block_size ||
-      block_table_stride < max_blocks_per_seq ||
-      num_rows > 2147483647LL / num_heads - 8192) {
+      max_blocks_per_seq > (1LL << 30) / block_size || block_table_stride < max_blocks_per_seq ||
+      num_groups > (1LL << 31) || !grid_fits(xcd_grid(num_groups, num_heads), 256)) {
     set_error("%s: bad sizes (rows %lld groups %lld table %lld wide, stride %lld)", who,
               (long long)num_rows, (long long)num_groups, (long long)max_blocks_per_seq,
               (long long)block_table_stride);
+    return VFL_E_INVALID;
+  }
+  if (!(fabsf(scale) < INFINITY)) {
+    set_error("%s: scale %f", who, (double)scale);
     return VFL_E_INVALID;
   }
   if (num_rows == 0 || num_groups == 0) return VFL_OK;

@@ -45,6 +45,9 @@ __device__ __forceinline__ uint2 e4m3_widen(uint32_t w, float scale) {
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)));
 }
 
+// Whether a launch stays below the runtime's 2^32 threads a dimension.
+inline bool grid_fits(int64_t groups, int threads) { return groups * threads < (1LL << 32); }
+
 // Shared argument checks of the 8-bit cache's entry points (kv_cache_8bit.hip).
 int check_8bit_cache(const char *who, int dtype, int num_heads, int head_dim, int block_size,
                      int64_t num_blocks);

@@ -282,9 +282,13 @@ static int launch_append(bool aligned, const void *key, const void *value, int64
                          float *scales, const int64_t *slots, int64_t T, int H, int D, int BS,
                          int64_t num_blocks, hipStream_t stream) {
   using E = typename Elem<DT>::T;
-  const int window = append_window(T, BS);
-  const dim3 grid((unsigned)xcd_grid((T + window - 1) / window, H));
-  const int steps = (D + 63) / 64;
+  const int window = append_window(T, BS), steps = (D + 63) / 64;
+  const int64_t groups = xcd_grid((T + window - 1) / window, H);
+  if (!grid_fits(groups, 64 * (steps > 4 ? 8 : steps))) {
+    set_error("reshape_and_cache_8bit: %lld tokens x %d heads exceed a launch", (long long)T, H);
+    return VFL_E_INVALID;
+  }
+  const dim3 grid((unsigned)groups);
   auto go = [&](auto al, auto parts) {
     launch_append_steps<DT, decltype(al)::value, decltype(parts)::value>(
         steps, grid, stream, (const E *)key, (const E *)value, k_st, k_sh, v_st, v_sh,

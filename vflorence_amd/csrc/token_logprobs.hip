@@ -9,8 +9,7 @@
 #include <math.h>
 #include <stdio.h>
 
-#include "common.h"
-#include "mfma_ops.h"
+#include "e4m3.h"
 
 namespace vfl {
 
@@ -498,10 +497,11 @@ extern "C" int vfl_token_logprobs(const void *logits, int64_t row_stride, int64_
     set_error("token_logprobs: unsupported dtype code %d", dtype);
     return VFL_E_INVALID;
   }
-  if (rows < 0 || rows > 2147483647LL || vocab <= 0 || vocab > TLP_MAX_VOCAB ||
-      row_stride < vocab || k < 0 || k > TLP_MAX_K || k > vocab || num_tokens < 0) {
-    set_error("token_logprobs: need 0 <= k <= min(%d, vocab), vocab up to %d and row_stride >= "
-              "vocab (k %d, vocab %d, stride %lld, rows %lld)",
+  if (rows < 0 || !grid_fits(rows, 1024) || vocab <= 0 || vocab > TLP_MAX_VOCAB ||
+      (row_stride != 0 && row_stride < vocab) || k < 0 || k > TLP_MAX_K || k > vocab ||
+      num_tokens < 0) {
+    set_error("token_logprobs: need 0 <= k <= min(%d, vocab), vocab up to %d, fewer than 2^22 rows "
+              "and row_stride 0 or at least vocab (k %d, vocab %d, stride %lld, rows %lld)",
               TLP_MAX_K, TLP_MAX_VOCAB, k, vocab, (long long)row_stride, (long long)rows);
     return VFL_E_INVALID;
   }

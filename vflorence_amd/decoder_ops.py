@@ -17,6 +17,7 @@ rejected.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 
@@ -549,6 +550,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
     if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
         raise ValueError(f"tokens must be int64 [{rows}] or [{rows}, n], got {tokens.dtype} "
                          f"{tuple(tokens.shape)}")
+    k = operator.index(k)
     if not 0 <= k <= min(MAX_ALTERNATIVES, vocab):
         raise ValueError(f"k must be in [0, min({MAX_ALTERNATIVES}, vocab)], got {k}")
     if not 0 < vocab <= MAX_SCORED_VOCAB:
@@ -568,8 +570,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
     need = _logprobs_workspace(vocab, dtype, k)
     if need:
         workspace = torch.empty(rows * need, dtype=torch.uint8, device=dev)
-    on_device(index, lib.vfl_token_logprobs, logits.data_ptr(), logits.stride(0), rows, vocab,
-              dtype, tokens.data_ptr(), tokens.shape[1] if tokens.dim() == 2 else 1, k,
+    on_device(index, lib.vfl_token_logprobs, logits.data_ptr(),
+              logits.stride(0) if rows > 1 else vocab, rows, vocab, dtype, tokens.data_ptr(),
+              tokens.shape[1] if tokens.dim() == 2 else 1, k,
               logprobs.data_ptr(), entropy.data_ptr(), top.data_ptr() if k else None,
               ids.data_ptr() if k else None, workspace.data_ptr() if need else None)
     return logprobs, entropy, top, ids

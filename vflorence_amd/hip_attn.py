@@ -793,9 +793,10 @@ def kv_cache_8bit(num_blocks: int, num_heads: int, block_size: int, head_dim: in
                   device) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """A zero-filled paged cache in 8 bits: K and V pools ``[num_blocks, H, block_size, D]``
     of ``torch.float8_e4m3fn`` and their scales, float32 ``[num_blocks, H, 2]`` (K's, V's).  A
-    value is its e4m3 element times its block's and head's scale.  Pools have the layout of
-    the 16-bit ones (``v_cache_logical`` gives V in token order).  ``copy_blocks`` copies
-    pool blocks, and with an even number of heads their scales (``[scales]``) as well."""
+    value is its e4m3 element times its block's and head's scale, a power of two (0 where
+    nothing was written).  Pools have the layout of the 16-bit ones (``v_cache_logical``
+    gives V in token order).  ``copy_blocks`` copies pool blocks, and with an even number of
+    heads their scales (``[scales]``) as well."""
     if head_dim not in SUPPORTED_HEAD_DIMS or block_size not in SUPPORTED_BLOCK_SIZES:
         raise ValueError(f"no gfx950 kernel for block_size={block_size} head_dim={head_dim}; "
                          f"supported head_dim {sorted(SUPPORTED_HEAD_DIMS)}, block_size "
@@ -909,7 +910,7 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
     """``attention_with_kv_cache`` over an 8-bit cache (``kv_cache_8bit``), into ``out``.
 
     query: [N, H, D] in float32, bfloat16 or float16, any token and head strides; out: a
-    contiguous tensor of its shape and dtype.  Row r attends to the first ``seq_lens[r]``
+    contiguous tensor of its shape and dtype, ``query`` itself or apart from it.  Row r attends to the first ``seq_lens[r]``
     tokens (int32, as many as the table lists at most) of the blocks ``block_table[r]`` (int32
     [N, max_blocks]) lists; a block id outside the pool contributes nothing, and a row
     without tokens is zero.  Of ``scheduler_metadata`` the row groups (``group_start``,
@@ -932,7 +933,9 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                          f"{block_table.dtype} {tuple(block_table.shape)}")
     index = one_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
     refuse_gradients("attention_with_kv_cache_8bit", query, out)
-    if block_table.stride(1) != 1:
+    width = block_table.shape[1]
+    if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
+                                                      and num_rows > 1):
         block_table = block_table.contiguous()
     seq_lens = seq_lens.contiguous()
     start = order = None
@@ -947,16 +950,19 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                              "self_attention_with_kv_write alone")
         if not sm.own_tables or sm.group_start is None:
             start, order, num_groups = sm.group_start, sm.group_order, sm.num_groups
-        for t in (start, order):
-            if t is not None:
-                one_gpu(query, t)
-    width = block_table.shape[1]
+        if start is not None:
+            one_gpu(query, start)
+            start = start.contiguous()
+        if order is not None:
+            one_gpu(query, order)
+            order = order.contiguous()
     need = _attention_8bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     on_device(index, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
               query.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
-              out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-              width, None if start is None else start.data_ptr(),
+              out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(),
+              block_table.stride(0) if num_rows > 1 else width, width,
+              None if start is None else start.data_ptr(),
               None if order is None else order.data_ptr(), num_rows, num_groups, num_heads,
               head_dim, block_size, num_blocks, float(scale), dtype,
               workspace.data_ptr() if need else None)
