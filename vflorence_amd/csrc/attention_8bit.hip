@@ -441,44 +441,47 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   }
 }
 
-// The splits of a (row, head) joined: a quarter of D threads take 4 dims each of a split, the
-// rest of the workgroup the next splits; their sums meet in LDS.
+// The splits of a (row, head) joined: a quarter of D threads, a team, take 4 dims each of
+// every teams-th split, about a maximum of their own, so that maxima and sums come in one round
+// trip; the teams meet in LDS.
 constexpr int ATTN8_JOIN_NT = 256;
 template <int DT>
 __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn8Args a) {
   using T = typename Elem<DT>::T;
   __shared__ float4 s_o[ATTN8_JOIN_NT];
-  __shared__ float s_s[ATTN8_JOIN_NT];
+  __shared__ float2 s_ml[ATTN8_JOIN_NT];
   int64_t row0;
   if ((int)blockIdx.y >= group_rows(a, blockIdx.x / a.H, row0)) return;
   const int64_t at = (row0 + blockIdx.y) * a.H + blockIdx.x % a.H;
-  const float2 *ml = a.part.ml + at * a.splits;
   const int tid = threadIdx.x, quads = a.D / 4, teams = ATTN8_JOIN_NT / quads;
   const int team = tid / quads, quad = tid % quads;
-  float M = NO_SCORE;
-  for (int s = tid & 63; s < a.splits; s += 64) M = fmaxf(M, ml[s].x);
-  M = wave_max64(M);
-  float S = 0.f;
+  const float2 *ml = a.part.ml + at * a.splits;
+  const float4 *acc = reinterpret_cast<const float4 *>(a.part.acc + at * a.splits * a.D) + quad;
+  float M = NO_SCORE, S = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (team < teams) {
+#pragma unroll 4
     for (int s = team; s < a.splits; s += teams) {
       const float2 x = ml[s];
-      const float f = fast_exp2(x.x - M);
-      const float4 v =
-          *reinterpret_cast<const float4 *>(a.part.acc + (at * a.splits + s) * a.D + 4 * quad);
-      S = fmaf(x.y, f, S);
-      o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+      const float4 v = acc[(int64_t)s * quads];
+      const float to = fmaxf(M, x.x), f = fast_exp2(M - to), e = fast_exp2(x.x - to);
+      S = S * f + x.y * e;
+      o.x = o.x * f + v.x * e, o.y = o.y * f + v.y * e;
+      o.z = o.z * f + v.z * e, o.w = o.w * f + v.w * e;
+      M = to;
     }
   }
   s_o[tid] = o;
-  s_s[tid] = S;
+  s_ml[tid] = make_float2(M, S);
   __syncthreads();
   for (int d = tid; d < a.D; d += ATTN8_JOIN_NT) {
-    float sum = 0.f, y = 0.f;
+    float top = NO_SCORE, sum = 0.f, y = 0.f;
+    for (int t = 0; t < teams; ++t) top = fmaxf(top, s_ml[t * quads + d / 4].x);
     for (int t = 0; t < teams; ++t) {
-      sum += s_s[t * quads + d / 4];
-      y += (&s_o[t * quads + d / 4].x)[d % 4];
+      const float2 x = s_ml[t * quads + d / 4];
+      const float e = fast_exp2(x.x - top);
+      sum = fmaf(x.y, e, sum);
+      y = fmaf((&s_o[t * quads + d / 4].x)[d % 4], e, y);
     }
     store_result<DT>((T *)a.out + at * a.D + d, sum, y);
   }

@@ -557,7 +557,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, k: int = 0):
         raise ValueError(f"vocab must be in [1, {MAX_SCORED_VOCAB}], got {vocab}")
     dtype = _dtype_code(logits.dtype)
     index = one_gpu(logits, tokens)
-    refuse_gradients("token_logprobs", logits)
+    if logits.requires_grad:
+        refuse_gradients("token_logprobs")
     tokens = tokens.contiguous()
     dev = logits.device
     logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)

@@ -835,9 +835,10 @@ def _check_8bit_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_scales: t
     return shape
 
 
-def refuse_gradients(name: str, *tensors: torch.Tensor) -> None:
-    """Raise where autograd would record the call: these kernels have no backward pass."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def refuse_gradients(name: str) -> None:
+    """For a call with operands that require gradients: raise where autograd would record it,
+    as these kernels have no backward pass."""
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient; call it under torch.no_grad()")
 
 
@@ -888,7 +889,8 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
         raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
                          f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
     index = one_gpu(key, value, k_cache, v_cache, kv_scales, slot_mapping)
-    refuse_gradients("reshape_and_cache_8bit", key, value)
+    if key.requires_grad or value.requires_grad:
+        refuse_gradients("reshape_and_cache_8bit")
     slot_mapping = slot_mapping.contiguous()
     on_device(index, lib.vfl_reshape_and_cache_8bit, key.data_ptr(), value.data_ptr(),
               key.stride(0), key.stride(1), value.stride(0), value.stride(1),
@@ -932,7 +934,8 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
                          f"{block_table.dtype} {tuple(block_table.shape)}")
     index = one_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
-    refuse_gradients("attention_with_kv_cache_8bit", query, out)
+    if query.requires_grad or out.requires_grad:
+        refuse_gradients("attention_with_kv_cache_8bit")
     width = block_table.shape[1]
     if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
                                                       and num_rows > 1):
