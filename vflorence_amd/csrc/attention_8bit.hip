@@ -487,18 +487,25 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
   }
 }
 
-// Waves of a workgroup and workgroups of a context.
+// Waves of a workgroup and workgroups of a context.  Few workgroups take eight waves (head size
+// 64, 16 heads, to 1024 tokens: 128 rows in groups of 4 10.1, one group 7.1; 1024 workgroups want
+// four, 18.5 against 19.9 us with eight).  A context of more than 256 KB is split where that
+// fills waves which the card would hold and leaves each 64 tokens: the join costs 4.6 us, about
+// what one workgroup streams 256 KB in.  Measured: 2 rows of 17001 and 39999 tokens x 8 heads of
+// 128, 16 splits 27.0 us, 8 27.6, 32 28.6, none 675; heads of 256, 64 groups to 1024 tokens, no
+// split 23.0 us, four 30.6.
 struct Attn8Plan {
   int waves, splits;
 };
 
 inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens) {
-  Attn8Plan p{D > 256 ? 2 : 4, 1};
+  // waves of a launch that the card holds at once, by the registers that a head of D takes
+  const int64_t resident = 256 * (D <= 128 ? 16 : D <= 192 ? 12 : D <= 256 ? 8 : 4);
   const int64_t wgs = num_groups * H;
-  if (D <= 128 && wgs <= 512) p.waves = 8;
+  Attn8Plan p{D <= 256 && wgs <= 512 ? 8 : 4, 1};
   const int64_t bytes = max_tokens * 2 * D;
-  if (bytes > (256 << 10) && wgs * p.waves < 4096) {
-    const int64_t fill = 4096 / (wgs * p.waves);
+  if (bytes > (256 << 10) && wgs * p.waves < resident) {
+    const int64_t fill = resident / (wgs * p.waves);
     const int64_t most = max_tokens / 32 / (p.waves * 2);
     p.splits = (int)(fill < most ? fill : most);
     if (p.splits < 1) p.splits = 1;
@@ -511,8 +518,8 @@ static void launch_attention_8bit(const Attn8Args &a, int waves, hipStream_t str
   const dim3 grid((unsigned)xcd_grid(a.num_groups * a.splits, a.H));
 #define VFL_ATTN8(NW) \
   attention_8bit_kernel<DT, NS, PARTS, NW><<<grid, dim3(64 * NW), 0, stream>>>(a)
-  if constexpr (NS == 8) VFL_ATTN8(2);
-  else if (NS <= 2 && waves == 8) { if constexpr (NS <= 2) VFL_ATTN8(8); }
+  if constexpr (NS == 8) VFL_ATTN8(4);
+  else if (waves == 8) VFL_ATTN8(8);
   else VFL_ATTN8(4);
 #undef VFL_ATTN8
 }
