@@ -487,13 +487,14 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
   }
 }
 
-// Waves of a workgroup and workgroups of a context.  Few workgroups take eight waves (head size
-// 64, 16 heads, to 1024 tokens: 128 rows in groups of 4 10.1, one group 7.1; 1024 workgroups want
-// four, 18.5 against 19.9 us with eight).  A context of more than 256 KB is split where that
-// fills waves which the card would hold and leaves each 64 tokens: the join costs 4.6 us, about
-// what one workgroup streams 256 KB in.  Measured: 2 rows of 17001 and 39999 tokens x 8 heads of
-// 128, 16 splits 27.0 us, 8 27.6, 32 28.6, none 675; heads of 256, 64 groups to 1024 tokens, no
-// split 23.0 us, four 30.6.
+// Waves of a workgroup and workgroups of a context.  A workgroup a CU or fewer takes eight waves
+// (eight against four, us: 12 of 590 tokens 5.6 / 6.4, 256 of 256 to 1024, fp32, 8.6 / 9.5; 384
+// of 100 to 1000 9.4 / 9.0, 1024 of 256 to 1024 19.9 / 18.5); wide heads, whose waves hold more
+// and are fewer on a CU, up to two (320 of 192 dims 21.4 / 26.5).  A context of more than 192 KB is
+// split where four parts or more fill waves that the card would hold and leave each 64 tokens; the
+// join costs 4.6 us (512 workgroups of 128 dims to 1024 tokens 24.9 in two parts, 20.5 whole; 16 heads of 64, one group: 1024 tokens 8.8 split, 7.0 whole; 2048 8.8 / 10.3; 4096
+// 9.1 / 16.4; 2 rows of 17001 and 39999 tokens x 8 heads of 128 27.0 in 16 parts, 27.6 in 8, 28.6
+// in 32).
 struct Attn8Plan {
   int waves, splits;
 };
@@ -502,13 +503,13 @@ inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens
   // waves of a launch that the card holds at once, by the registers that a head of D takes
   const int64_t resident = 256 * (D <= 128 ? 16 : D <= 192 ? 12 : D <= 256 ? 8 : 4);
   const int64_t wgs = num_groups * H;
-  Attn8Plan p{D <= 256 && wgs <= 512 ? 8 : 4, 1};
+  Attn8Plan p{D <= 256 && wgs <= (D <= 64 ? 256 : 512) ? 8 : 4, 1};
   const int64_t bytes = max_tokens * 2 * D;
-  if (bytes > (256 << 10) && wgs * p.waves < resident) {
+  if (bytes > (192 << 10) && wgs * p.waves < resident) {
     const int64_t fill = resident / (wgs * p.waves);
     const int64_t most = max_tokens / 32 / (p.waves * 2);
-    p.splits = (int)(fill < most ? fill : most);
-    if (p.splits < 1) p.splits = 1;
+    const int64_t parts = fill < most ? fill : most;
+    if (parts >= 4) p.splits = (int)parts;
   }
   return p;
 }
