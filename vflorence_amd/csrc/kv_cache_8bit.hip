@@ -39,34 +39,116 @@ int check_8bit_cache(const char *who, int dtype, int num_heads, int head_dim, in
   return VFL_OK;
 }
 
-// N consecutive elements as fp32 (16-byte loads, 8-byte ones for four 16-bit elements,
+// N consecutive elements as words of memory (16-byte loads, 8-byte ones for four 16-bit elements,
 // where the rows are aligned for them).
 template <int DT, bool ALIGNED, int N>
-__device__ __forceinline__ void load_elems(const typename Elem<DT>::T *p, float *f) {
+__device__ __forceinline__ void load_raw(const typename Elem<DT>::T *p, uint32_t *w) {
+  constexpr int WORDS = N * (int)sizeof(typename Elem<DT>::T) / 4;
   if constexpr (!ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (DT == VFL_FLOAT32) f[i] = p[i];
-      else f[i] = Mfma<DT>::widen(p[i]);
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (DT == VFL_FLOAT32) w[i] = __float_as_uint(p[i]);
+      else w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
     }
-  } else if constexpr (DT == VFL_FLOAT32 || N % 8 == 0) {
+  } else if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; i += Elem<DT>::VEC)
-      unpack16<DT>(*reinterpret_cast<const uint4 *>(p + i), f + i);
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 u = reinterpret_cast<const uint4 *>(p)[i / 4];
+      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+    }
   } else {
-    static_assert(N == 4, "a 16-bit quad");
+    static_assert(WORDS == 2, "a 16-bit quad");
     const uint2 u = *reinterpret_cast<const uint2 *>(p);
-    f[0] = Mfma<DT>::widen_lo(u.x), f[1] = Mfma<DT>::widen_hi(u.x);
-    f[2] = Mfma<DT>::widen_lo(u.y), f[3] = Mfma<DT>::widen_hi(u.y);
+    w[0] = u.x, w[1] = u.y;
   }
 }
 
-// |x|, or 0 for an infinity or a NaN (which `x` then becomes).
-__device__ __forceinline__ float finite_abs(float &x) {
-  const float a = fabsf(x);
-  if (a < INFINITY) return a;
-  x = __uint_as_float(0x7fc00000u);
-  return 0.f;
+// Magnitudes are compared as patterns without their sign, which order like the values, an
+// infinity and then NaN above them all; 16-bit ones two at a time.
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+template <int DT> struct Pattern {
+  static constexpr bool PAIRS = DT != VFL_FLOAT32;
+  static constexpr uint32_t MAGNITUDE = PAIRS ? 0x7fff7fffu : 0x7fffffffu;
+  static constexpr uint32_t INF = DT == VFL_FLOAT32    ? 0x7f800000u
+                                  : DT == VFL_BFLOAT16 ? 0x7f80u
+                                                       : 0x7c00u;
+
+  static __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+    if constexpr (!PAIRS) return max(a, b);
+    else
+      return __builtin_bit_cast(uint32_t,
+                                __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a),
+                                                          __builtin_bit_cast(ushort2_t, b)));
+  }
+  template <int WORDS>
+  static __device__ __forceinline__ void add(uint32_t &m, const uint32_t (&w)[WORDS]) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) m = largest(m, w[i] & MAGNITUDE);
+  }
+  // the same, what is not finite left out
+  template <int WORDS>
+  static __device__ __forceinline__ void add_finite(uint32_t &m, const uint32_t (&w)[WORDS]) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      uint32_t x = w[i] & MAGNITUDE;
+      if constexpr (PAIRS) {
+        if ((x & 0xffffu) >= INF) x &= 0xffff0000u;
+        if ((x >> 16) >= INF) x &= 0xffffu;
+      } else if (x >= INF) {
+        x = 0;
+      }
+      m = largest(m, x);
+    }
+  }
+  // over the wave, of both halves of a pair
+  static __device__ __forceinline__ uint32_t over_wave(uint32_t m) {
+    if constexpr (PAIRS) m = max(m >> 16, m & 0xffffu);
+    int x = row_max16((int)m);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((int)a[0], (int)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return (uint32_t)max((int)b[0], (int)b[1]);
+  }
+  static __device__ __forceinline__ float value(uint32_t pattern) {
+    if constexpr (PAIRS) return Mfma<DT>::widen(pattern);
+    else return __uint_as_float(pattern);
+  }
+};
+
+// Four elements (as words of memory) over `scale`, a power of two whose exponent the conversion
+// takes off, rounded to nearest even; an infinity or a NaN becomes NaN.
+typedef short short2_t __attribute__((ext_vector_type(2)));
+template <int DT> __device__ __forceinline__ uint32_t e4m3_pack(const uint32_t *w, float scale) {
+  short2_t r = {0, 0};
+  if constexpr (DT == VFL_FLOAT32) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __uint_as_float(w[0]), __uint_as_float(w[1]),
+                                                 scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __uint_as_float(w[2]), __uint_as_float(w[3]),
+                                                 scale, true);
+  } else if constexpr (DT == VFL_BFLOAT16) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w[0]), scale,
+                                                  false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, w[1]), scale,
+                                                  true);
+  } else {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, w[0]), scale,
+                                                 false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2_t, w[1]), scale,
+                                                 true);
+  }
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// Rows of four bytes to columns: word i of the result holds byte i of every word.
+__device__ __forceinline__ void transpose_bytes(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // w0.0 w1.0 w0.1 w1.1
+  const uint32_t b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);  // w0.2 w1.2 w0.3 w1.3
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
 // A workgroup takes the runs that begin among `window` tokens (up to 32), for one head; its NS
@@ -81,7 +163,9 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     uint8_t *__restrict__ vc, float *__restrict__ scales, const int64_t *__restrict__ slots,
     int T, int H, int D, int num_blocks, int window) {
   constexpr int BS = 16 * PARTS;
-  __shared__ float s_max[2][NS];
+  using P = Pattern<DT>;
+  constexpr int KW = 16 * (int)sizeof(typename Elem<DT>::T) / 4, VW = KW / 4;
+  __shared__ uint32_t s_max[2][NS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int64_t pos;
@@ -129,7 +213,7 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
     float *sc = scales + 2 * ((int64_t)blk * H + h);
     const float old_k = fresh ? 0.f : sc[0], old_v = fresh ? 0.f : sc[1];
 
-    float kx[PARTS][16], vx[PARTS][4][4];
+    uint32_t kx[PARTS][KW], vx[PARTS][4][VW];
     int ks[PARTS], vs[PARTS][4];
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
@@ -141,21 +225,13 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
         if (!v_in) vs[p][j] = -1;
       }
     }
-    float km = 0.f, vm = 0.f;
     auto k_row = [&](int p, int i) {
-      load_elems<DT, ALIGNED, 16>(key + (t + i) * k_st + h * k_sh + (k_in ? kd : 0), kx[p]);
+      load_raw<DT, ALIGNED, 16>(key + (t + i) * k_st + h * k_sh + (k_in ? kd : 0), kx[p]);
     };
     auto v_row = [&](int p, int j, int i) {
-      load_elems<DT, ALIGNED, 4>(value + (t + i) * v_st + h * v_sh + (v_in ? vd : 0), vx[p][j]);
+      load_raw<DT, ALIGNED, 4>(value + (t + i) * v_st + h * v_sh + (v_in ? vd : 0), vx[p][j]);
     };
-    auto k_max = [&](int p) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) km = fmaxf(km, finite_abs(kx[p][i]));
-    };
-    auto v_max = [&](int p, int j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vm = fmaxf(vm, finite_abs(vx[p][j][i]));
-    };
+    uint32_t km = 0, vm = 0;
     if (n > 1) {
       // every lane reads some row that is taken (what repeats changes no maximum): a load under
       // a condition would wait for the one before
@@ -167,9 +243,9 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
       }
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        k_max(p);
+        P::add(km, kx[p]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v_max(p, j);
+        for (int j = 0; j < 4; ++j) P::add(vm, vx[p][j]);
       }
     } else {
       // one token: the few lanes that hold it (256 rows x 16 heads 5.4 against 7.2 us)
@@ -177,29 +253,41 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
       for (int p = 0; p < PARTS; ++p) {
         if (ks[p] >= 0) {
           k_row(p, 0);
-          k_max(p);
+          P::add(km, kx[p]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (vs[p][j] >= 0) {
             v_row(p, j, 0);
-            v_max(p, j);
+            P::add(vm, vx[p][j]);
           }
       }
     }
-    km = wave_max64(km);
-    vm = wave_max64(vm);
+    km = P::over_wave(km);
+    vm = P::over_wave(vm);
+    if (max(km, vm) >= P::INF) {  // wave-uniform, rare: the finite values alone
+      km = vm = 0;
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) {
+        if (n > 1 || ks[p] >= 0) P::add_finite(km, kx[p]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n > 1 || vs[p][j] >= 0) P::add_finite(vm, vx[p][j]);
+      }
+      km = P::over_wave(km);
+      vm = P::over_wave(vm);
+    }
     if constexpr (NS > 1) {
       __syncthreads();  // the previous run's maxima have been read
       if (lane == 0) s_max[0][wave] = km, s_max[1][wave] = vm;
       __syncthreads();  // and every wave has read the old scales
 #pragma unroll
-      for (int w = 0; w < NS; ++w) km = fmaxf(km, s_max[0][w]), vm = fmaxf(vm, s_max[1][w]);
+      for (int w = 0; w < NS; ++w) km = max(km, s_max[0][w]), vm = max(vm, s_max[1][w]);
     }
-    const float new_k = fmaxf(old_k, e4m3_scale(km)), new_v = fmaxf(old_v, e4m3_scale(vm));
+    const float new_k = fmaxf(old_k, e4m3_scale(P::value(km)));
+    const float new_v = fmaxf(old_v, e4m3_scale(P::value(vm)));
     const bool all_k = fresh || new_k != old_k, all_v = fresh || new_v != old_v;
-    const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
-    const float ratio_k = old_k * inv_k, ratio_v = old_v * inv_v;
+    const float ratio_k = old_k / new_k, ratio_v = old_v / new_v;
 
     const int64_t tile = ((int64_t)blk * H + h) * (BS * D);
     uint8_t *kt = kc + tile, *vt = vc + tile;
@@ -210,9 +298,7 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
         uint32_t w[4] = {0, 0, 0, 0};
         if (ks[p] >= 0) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) kx[p][i] *= inv_k;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = e4m3_pack(kx[p] + 4 * i);
+          for (int i = 0; i < 4; ++i) w[i] = e4m3_pack<DT>(kx[p] + i * VW, new_k);
         } else if (!fresh) {
           const uint4 u = *row;
           w[0] = e4m3_rescale(u.x, ratio_k), w[1] = e4m3_rescale(u.y, ratio_k);
@@ -232,17 +318,15 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
             for (int i = 0; i < 4; ++i) w[i] = e4m3_rescale(w[i], ratio_v);
           }
         }
+        uint32_t u[4], taken = 0;  // the bytes of the tokens that the run brings
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (vs[p][j] < 0) continue;
-          float f[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] = vx[p][j][i] * inv_v;
-          const uint32_t u = e4m3_pack(f);  // dim i's value of token j
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = (w[i] & ~(0xffu << (8 * j))) | (((u >> (8 * i)) & 0xffu) << (8 * j));
+          u[j] = e4m3_pack<DT>(vx[p][j], new_v);
+          if (vs[p][j] >= 0) taken |= 0xffu << (8 * j);
         }
+        transpose_bytes(u);  // dim i's values of the four tokens
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] & ~taken) | (u[i] & taken);
         *group = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
