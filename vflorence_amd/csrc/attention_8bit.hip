@@ -16,6 +16,19 @@
 // Queries go in as bf16 terms, which hold all of their bits: one of bf16, two of fp16, three of
 // fp32.  Weights as two terms, 2^-17 relative, or three for fp32 outputs, 2^-25: below the
 // output's rounding.  Their sum is the same product with a row of ones.
+//
+// What bounds it: HBM where there is enough to read (64 groups of 4 rows x 16 heads of 64, 2048
+// tokens each: 46 us, 5.8 TB/s; 256 to 1024 tokens, 85 MB: 18.0 us, of which 5.1 are the launch
+// and five dependent loads -- arguments, order, group, length and block ids, pages -- and the
+// merge).  Vector operations take half of the time (about 145 per 32 tokens, 64 dims: 32
+// conversions, 8 exponentials, 24 that split the weights), matrix products a sixth.  What each
+// step gave, us, the same 256 to 1024 tokens / 93 single rows to 1000 tokens, fp16 / 2 rows to
+// 39999 tokens:
+//   loads under conditions, each waited for        23.0 / 28.0 / 675
+//   buffer loads one iteration ahead, splits       19.6 / 23.7 / 49
+//   descriptors in scalar registers, a faster join 18.6 / 21.0 / 30.6
+//   scales in the conversions, weights summed by
+//   matrix products, non-temporal loads            18.0 / 21.6 / 27.0
 #include <math.h>
 #include <stdio.h>
 

@@ -12,10 +12,13 @@
 // grows with the number of appends, which any other scale would cost.  Infinities and NaN
 // become NaN and leave the scale alone.
 //
-// What bounds it: prompts HBM (64 prompts of 256 to 1024 tokens x 16 heads, bf16: 54.6 us,
-// 4.6 TB/s read and written); steps their chain of slots, rows and stores (256 rows x 16 heads
-// 5.2 us, 4 x 12 3.3 us).  The heads of a block run on one XCD, whose L2 then writes the block's
-// line of scales whole.
+// What bounds it: prompts HBM (64 prompts of 256 to 1024 tokens x 16 heads, bf16: 53.0 us, 4.8
+// TB/s read and written, of a copy's 5.1); steps their chain of slots, rows and stores (256 rows
+// x 16 heads 4.7 us, 4 x 12 3.0 us).  A wave takes a block's tokens of a head, so that a tile is
+// written whole; the heads of a block run on one XCD, whose L2 then writes the block's line of
+// scales whole.  Magnitudes are compared as 16-bit patterns, two at a time, and the conversion
+// takes the scale's exponent off: the same prompts ran in 57.0 us with values widened, compared
+// and multiplied one by one (two thirds of the time in vector operations).
 #include <stdio.h>
 
 #include "e4m3.h"
@@ -248,7 +251,7 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
         for (int j = 0; j < 4; ++j) P::add(vm, vx[p][j]);
       }
     } else {
-      // one token: the few lanes that hold it (256 rows x 16 heads 5.4 against 7.2 us)
+      // one token: the few lanes that hold it (all lanes: 256 rows x 16 heads 7.2 us, not 5.2)
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
         if (ks[p] >= 0) {
@@ -354,10 +357,9 @@ static void launch_append_steps(int steps, dim3 grid, hipStream_t stream, A... a
 // Tokens whose runs a workgroup takes.  A decode step's tokens are runs of their own and want
 // a workgroup each; a prompt's fill blocks.  The host does not see which they are: calls of up
 // to 512 tokens (the most rows of a step that the projections take) get one, longer ones a
-// block's.  Windows of 1 and of 16, us, bf16: steps of 256 and 512 rows x 16 heads 5.2 / 23.7 and
-// 7.6 / 25.2, of 2048 rows 23 / 36; a prompt of 590 tokens x 12 heads 7.4 / 3.5, 64 prompts of
-// 256 to 1024 tokens x 16 heads 177 / 54.6; the same in blocks of 32, windows of 16 and 32, 63.5
-// / 54.8.
+// block's.  Windows of 1 and of 16, us, bf16: steps of 256 and 512 rows x 16 heads 4.7 / 19.8 and
+// 6.7 / 21.0, of 2048 rows 18.9 / 31.5; a prompt of 590 tokens x 12 heads 6.1 / 3.1, 64 prompts
+// of 256 to 1024 tokens x 16 heads 159 / 52.9.
 inline int append_window(int64_t T, int BS) { return T <= 512 ? 1 : BS; }
 
 template <int DT>
