@@ -1,13 +1,14 @@
 /*
  * vflorence_amd.h -- C ABI of the MI355X (gfx950) decode-step attention library and the
  * decoder-step kernels around it (residual + LayerNorm, log-softmax + rules + top-k,
- * the decoder's projections for a decode step's rows).
+ * the decoder's projections for a decode step's rows, token scores).
  *
  * Every entry point takes plain device pointers, element strides and sizes, and a
  * hipStream_t passed as `void *` (NULL = the legacy default stream).  No entry point
- * allocates device memory; the one that needs scratch space (vfl_copy_blocks with
- * overlapping pairs) takes it from the caller, or from a buffer the library holds in
- * each GPU's memory (vfl_copy_blocks_noalloc).  All work is enqueued asynchronously
+ * allocates device memory; those that need scratch space (vfl_copy_blocks with overlapping
+ * pairs, vfl_attention_with_kv_cache_8bit over long tables, vfl_token_logprobs over long
+ * rows) take it from the caller, vfl_copy_blocks_noalloc from a buffer the library holds
+ * in each GPU's memory.  All work is enqueued asynchronously
  * on `stream`, in call order, so a caller that issues copy_blocks ->
  * reshape_and_cache -> attention_with_kv_cache on one stream gets the reference's
  * ordering.
