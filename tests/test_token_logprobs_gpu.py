@@ -128,6 +128,23 @@ def test_rows_without_a_distribution(vocab, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [31, 5001, 50265, 130001])
+@pytest.mark.parametrize("left", [0, 1, 3])
+def test_rows_of_nan(dtype, vocab, left):
+    """All NaN but for fewer values than k: every place of the alternatives is written."""
+    k = 6
+    logits, tokens = case(3, vocab, dtype)
+    score(logits, tokens, k)  # (whose memory the next call's results may take)
+    logits[1] = math.nan
+    logits[1, vocab - left :] = 1.0
+    logprobs, entropy, top, ids = score(logits, tokens, k)
+    assert logprobs[1].isnan().all() and entropy[1].isnan()
+    assert top[1].isnan().all() and (ids[1] == -1).all()
+    keep = [0, 2]
+    check(logits[keep], tokens[keep], k, [t[keep] for t in (logprobs, entropy, top, ids)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [9, 50265, 130001])
 def test_given_tokens(dtype, vocab):
     """Several tokens a row, the first and last ones, the same one twice, ones outside."""

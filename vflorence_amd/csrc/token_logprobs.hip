@@ -426,10 +426,14 @@ __global__ __launch_bounds__(TLP_JOIN_NT) void token_logprobs_join_kernel(
     o.logprobs[row * o.num_tokens + i] =
         bad || t < 0 || t >= vocab ? NAN : norm.logprob(logit<DT>(x[t]));
   }
+  if (bad) {  // (its segments may have fewer than k candidates, whose ranks leave gaps)
+    if (tid < k) o.top[row * k + tid] = NAN, o.ids[row * k + tid] = -1;
+    return;
+  }
   __syncthreads();
   rank_candidates(s_cv, s_ci, count, tid >> 6, TLP_JOIN_NT / 64, k, [&](int rank, float v, int id) {
-    o.top[row * k + rank] = bad ? NAN : norm.logprob(v);
-    o.ids[row * k + rank] = bad ? -1 : id;
+    o.top[row * k + rank] = norm.logprob(v);
+    o.ids[row * k + rank] = id;
   });
 }
 
