@@ -508,14 +508,15 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * Caches held in 8 bits: K and V pools of e4m3 elements (OCP FP8: 448 the largest, no
  * infinities) in the 16-bit pools' shape and layout, and one fp32 scale per (block, head) for
  * each, kv_scales [num_blocks][num_heads][2] (K's, V's), a power of two, or 0 where nothing was
- * written.  An element stands for itself times its block's and head's scale.  Pools 16-byte aligned; dtype is that of the 32- or 16-bit
- * operands beside them.  No vllm_cpu_attn counterpart.
+ * written.  An element stands for itself times its block's and head's scale.  Pools 16-byte
+ * aligned; dtype is that of the 32- or 16-bit operands beside them.  No vllm_cpu_attn
+ * counterpart.
  *
  * vfl_reshape_and_cache_8bit: vfl_reshape_and_cache into such a cache, same slots and strides.
  * Consecutive tokens whose slots lie in one block are a run (of a slot that comes twice in it,
- * the later token); a block's tokens must form one run of the call, and a block belong to one sequence (a second run in the call, or a call
- * that overlaps this one on another stream, would race for the block's scale).  Per run
- * and head, for K and for V,
+ * the later token); a block's tokens must form one run of the call, and a block belong to one
+ * sequence (a second run in the call, or a call that overlaps this one on another stream,
+ * would race for the block's scale).  Per run and head, for K and for V,
  *   new = max(old, the smallest power of two with max |x| / new <= 448)   (2^-100 at least)
  * where max is over the run's finite values and old = 0 when the run holds the block's first
  * slot: the block then starts over, and its other slots become 0.  Else they become rnd(q *
@@ -524,7 +525,7 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * for each block_size tokens and 64 dims) are refused.
  *
  * vfl_attention_with_kv_cache_8bit: vfl_attention_with_kv_cache over such a cache; groups
- * (group_start) are rows sharing one table, at most 8 of them, block_table lists
+ * (group_start) are rows sharing one table and length, at most 8 of them, block_table lists
  * max_blocks_per_seq blocks a row (2^30 tokens at most; longer contexts are clamped to that).
  * query and out share dtype; out contiguous, and either query itself or apart from it; scale
  * finite.  Sums and softmax in fp32, the weights kept to 2^-17 (fp32:
@@ -554,8 +555,7 @@ int vfl_attention_with_kv_cache_8bit(const void *query, int64_t query_stride_tok
 /*
  * Log probabilities of given tokens, entropy and best alternatives (no vllm_cpu_attn
  * counterpart).  Per row r of `logits` ([rows][vocab], row stride in elements, 0 for one row
- * repeated; fewer than 2^22 rows), with
- * p = softmax of the row in fp32:
+ * repeated; fewer than 2^22 rows), with p = softmax of the row in fp32:
  *   logprobs[r][i] = log p(tokens[r][i]) for i < num_tokens (NaN for a token outside
  *                    [0, vocab)); tokens DEVICE int64 [rows][num_tokens]
  *   entropy[r]     = -sum p log p

@@ -20,8 +20,8 @@
 // What bounds it: HBM where there is enough to read (64 groups of 4 rows x 16 heads of 64, 2048
 // tokens each: 46 us, 5.8 TB/s; 256 to 1024 tokens, 85 MB: 18.0 us, of which 5.1 are the launch
 // and five dependent loads -- arguments, order, group, length and block ids, pages -- and the
-// merge).  Vector operations take half of the time (about 145 per 32 tokens, 64 dims: 32
-// conversions, 8 exponentials, 24 that split the weights), matrix products a sixth.  What each
+// merge).  Vector operations take 42% of the cycles (about 145 per 32 tokens, 64 dims: 32
+// conversions, 8 exponentials, 24 that split the weights), matrix products 11%.  What each
 // step gave, us, the same 256 to 1024 tokens / 93 single rows to 1000 tokens, fp16 / 2 rows to
 // 39999 tokens:
 //   loads under conditions, each waited for        23.0 / 28.0 / 675
@@ -505,9 +505,9 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
 // of 100 to 1000 9.4 / 9.0, 1024 of 256 to 1024 19.9 / 18.5); wide heads, whose waves hold more
 // and are fewer on a CU, up to two (320 of 192 dims 21.4 / 26.5).  A context of more than 192 KB is
 // split where four parts or more fill waves that the card would hold and leave each 64 tokens; the
-// join costs 4.6 us (512 workgroups of 128 dims to 1024 tokens 24.9 in two parts, 20.5 whole; 16 heads of 64, one group: 1024 tokens 8.8 split, 7.0 whole; 2048 8.8 / 10.3; 4096
-// 9.1 / 16.4; 2 rows of 17001 and 39999 tokens x 8 heads of 128 27.0 in 16 parts, 27.6 in 8, 28.6
-// in 32).
+// join costs 4.6 us (512 workgroups of 128 dims to 1024 tokens 24.9 in two parts, 20.5 whole; 16
+// heads of 64, one group: 1024 tokens 8.8 split, 7.0 whole; 2048 8.8 / 10.3; 4096 9.1 / 16.4; 2
+// rows of 17001 and 39999 tokens x 8 heads of 128 27.0 in 16 parts, 27.6 in 8, 28.6 in 32).
 struct Attn8Plan {
   int waves, splits;
 };

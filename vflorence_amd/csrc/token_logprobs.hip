@@ -144,9 +144,9 @@ struct LogprobOut {
 // A row, or with SPLIT one segment of it, lives in the registers of NT threads, NV vectors
 // of 16 bytes each, read once.
 //
-// What bounds it: many rows the vector work, about 10 operations a value and the exponential
-// at a quarter of their rate (4.3 us of a row's 5.8 on its CU), two workgroups of 64 VGPRs a
-// CU overlapping it with the other's loads; few rows their own chain of loads,
+// What bounds it: many rows the vector work, 17 operations a value with k = 5 (one of them
+// the exponential, at a quarter of their rate), two workgroups of 64 VGPRs a CU overlapping
+// it with the other's loads; few rows their own chain of loads,
 // exponentials and picks.  Device time, us: 4096 x 50265 bf16 k = 5 93 (4.4 TB/s), k = 0 82
 // (5.0); 256 x 50265 k = 0 8.5; 4 x 51289 k = 8 8.5; 93 x 51289 fp32 k = 20 10.7.  What
 // the steps gave (the same cases): loads that no condition holds back 106 -> 93, 10.4 ->

@@ -912,12 +912,13 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
     """``attention_with_kv_cache`` over an 8-bit cache (``kv_cache_8bit``), into ``out``.
 
     query: [N, H, D] in float32, bfloat16 or float16, any token and head strides; out: a
-    contiguous tensor of its shape and dtype, ``query`` itself or apart from it.  Row r attends to the first ``seq_lens[r]``
-    tokens (int32, as many as the table lists at most) of the blocks ``block_table[r]`` (int32
-    [N, max_blocks]) lists; a block id outside the pool contributes nothing, and a row
-    without tokens is zero.  Of ``scheduler_metadata`` the row groups (``group_start``,
-    ``group_order``) are used: a group that shares its table is read once for all of its
-    rows, one whose rows keep their own tables runs row by row."""
+    contiguous tensor of its shape and dtype, ``query`` itself or apart from it.  Row r attends
+    to the first ``seq_lens[r]`` tokens (int32, as many as the table lists at most) of the
+    blocks that ``block_table[r]`` (int32 [N, max_blocks]) lists; a block id outside the pool
+    contributes nothing, and a row without tokens is zero.  Of ``scheduler_metadata`` the row
+    groups (``group_start``, ``group_order``) are used: a group that shares its table (and
+    length) is read once for all of its rows, one whose rows keep their own tables runs row
+    by row."""
     num_blocks, num_heads, block_size, head_dim = _check_8bit_cache(k_cache, v_cache, kv_scales)
     if query.dim() != 3 or query.stride(2) != 1 or query.shape[1:] != (num_heads, head_dim):
         raise ValueError(f"query must be [N, {num_heads}, {head_dim}] with a contiguous last "
