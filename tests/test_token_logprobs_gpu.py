@@ -255,3 +255,74 @@ def test_graph_stream_and_gradient():
     with torch.no_grad():
         score(leaf, tokens, 0)
     assert score(logits[:0], tokens[:0], 3)[2].shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [31, 5001, 50265, 130001])
+@pytest.mark.parametrize("level", [65535.5, 65600.0, 1e6, 3e7, 1e9, 3e9, 5e9, 1e10, 1e12, 1e20,
+                                   1e30, 9e37])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_rows_of_any_magnitude(dtype, vocab, level, sign):
+    """Maxima whose product with log2 e no longer holds units: uniform rows, neighbouring
+    values, low values among and before ordinary ones, one value far above the others."""
+    logits, tokens = case(8, vocab, dtype)
+    noise = logits.float().clone()
+    level = float(torch.tensor(sign * level).to(dtype))
+    half = torch.arange(vocab, device=DEV) < vocab // 2
+    logits[0] = level
+    logits[1] = (level + noise[1]).to(dtype)  # steps of the type about the level
+    logits[2, half] = -math.inf
+    logits[2, ~half] = level
+    logits[3, tokens[3]] = level
+    logits[4] = (noise[4] * (level / 4)).to(dtype)
+    logits[5] = torch.where(half, -abs(level), noise[5]).to(dtype)
+    logits[6] = torch.where(noise[6] > 0, -abs(level), noise[6]).to(dtype)
+    logits[7] = -abs(level)
+    logits[7, tokens[7]] = 1.0
+    for k in (5, 0):
+        got = score(logits, tokens, k)
+        check(logits, tokens, k, got)
+    assert abs(float(got[1][0]) - math.log(vocab)) < 1e-5
+
+
+@pytest.mark.parametrize("vocab", [31, 5001, 50265, 130001])
+@pytest.mark.parametrize("level", [1e10, -1e10])
+def test_large_rows_without_a_distribution(vocab, level):
+    logits, tokens = case(4, vocab, torch.float32)
+    logits[:] = level
+    logits[1, vocab - 1] = math.nan
+    logits[2, 4] = math.inf
+    logprobs, entropy, top, ids = score(logits, tokens, 6)
+    lost = torch.tensor([False, True, True, False], device=DEV)
+    assert torch.equal(logprobs.isnan(), lost) and torch.equal(entropy.isnan(), lost)
+    assert torch.equal(top.isnan(), lost[:, None].expand(4, 6))
+    assert torch.equal(ids == -1, lost[:, None].expand(4, 6))
+    keep = ~lost
+    check(logits[keep], tokens[keep], 6, [t[keep] for t in (logprobs, entropy, top, ids)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [31, 5001, 50265, 130001])
+@pytest.mark.parametrize("gap", [3.0, 8.0, 12.0, 15.0])
+def test_confident_rows(dtype, vocab, gap):
+    """One token with nearly all of the weight, whose log probability is close to 0; two others
+    have the rest, w <= 2 e^-3 < 0.1 of it, and a thread may see any of the low ones first.  A
+    weight's exponent is rounded about its thread's reference (which lags by 16 in log2 at most)
+    and about the maximum, 31 * 2^-23 of the weight at most, and the exponential is good to 2^-22;
+    the largest term is 1.  So 1 + w is off by 0.1 (2^-22 + 31 * 2^-23) and three roundings of
+    2^-24 (the division by the largest term, two sums), its log by 2^-23 of itself more."""
+    gen = torch.Generator().manual_seed(int(gap) + vocab)
+    logits = torch.full((6, vocab), -200.0)
+    tokens = torch.randint(0, vocab, (6,), generator=gen)
+    for r in range(6):
+        others = torch.randperm(vocab, generator=gen)[:2]
+        logits[r, others] = 4.0 * r - gap - torch.rand(2, generator=gen)
+        logits[r, tokens[r]] = 4.0 * r
+    logits, tokens = logits.to(dtype).to(DEV), tokens.to(DEV)
+    got = score(logits, tokens, 1)
+    want = torch.log_softmax(logits.double(), 1).gather(1, tokens[:, None])
+    bound = 0.1 * (2.0**-22 + 31 * 2.0**-23) + 3 * 2.0**-24 + 0.1 * 2.0**-23
+    for have in (got[0], got[2][:, 0]):
+        off = (have.double() - want[:, 0]).abs().max()
+        print(f"error / bound {float(off / bound):.3f}", flush=True)
+        assert off <= bound

@@ -18,14 +18,18 @@ constexpr int TLP_MAX_VOCAB = 1 << 20;
 constexpr int TLP_CAP = 512;        // candidates for the alternatives kept in LDS
 constexpr int TLP_MAX_SEGMENTS = 64;
 constexpr float TLP_FLOOR = -1e4f;  // exp2() is 0 long before
-constexpr float TLP_NONE = -3e38f;  // reference of a thread that has seen no value
-// A row whose maximum lies past this has weight on the values equal to it alone (their
-// neighbours are 2^100 away), and its products with log2 e overflow: taken apart.
-constexpr float TLP_EXTREME = 1e38f;
-constexpr float TLP_SLACK = 16.f;  // log2 units a reference may lag behind: sums stay < 2^33
+// A thread's reference is max * log2 e, rounded: every term carries that rounding, 2^-8 at most up
+// to this maximum, and the step to differences from the maximum itself takes it off again.  Rows
+// (or segments) whose maximum lies further from 0 would carry more, exp2's whole range from
+// 2^32 on: they are summed in a second read, from the differences.
+constexpr float TLP_FAR = 65536.f;
+constexpr float TLP_NONE = -1e5f;  // a thread's first reference: below every such maximum's
+// log2 units a reference may lag behind.  A thread's terms are up to 2^16, its sum of up to 112
+// below 2^23; about the maximum a row's 2^20 terms sum to 2^20 at most.
+constexpr float TLP_SLACK = 16.f;
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 
-// Sums of exp2(x log2 e - c) and of its product with the exponent.
+// A thread's sums of exp2(x log2 e - c) and of its product with the exponent.
 struct Sums {
   float c, s, w;
 
@@ -38,20 +42,41 @@ struct Sums {
   }
 };
 
+// The same of exp2((x - r) log2 e), r a value no less than any of the x.
+struct Stats {
+  float r, s, w;
+
+  // A thread's sums about r: divided by the term that r has in them (or would have), so that
+  // its own term becomes 1.
+  __device__ __forceinline__ Stats(const Sums &a, float r) : r(r), s(a.s), w(a.w) {
+    if (s == 0.f) return;  // (no value: the reference is none)
+    const float t = fmaf(r, LOG2E_F, -a.c), e = fast_exp2(t);
+    w = e < INFINITY ? fmaf(-t, s, w) / e : 0.f;
+    s /= e;
+  }
+  __device__ __forceinline__ Stats(float r, float s, float w) : r(r), s(s), w(w) {}
+
+  __device__ __forceinline__ void move(float to) {
+    if (s == 0.f) return;  // (nothing: r may be -inf)
+    const float d = (r - to) * LOG2E_F, f = fast_exp2(d);
+    w = f == 0.f ? 0.f : f * fmaf(d, s, w);
+    s *= f;
+    r = to;
+  }
+};
+
 // Sum over the wave, the first lane's for every lane: a product before the first addition is
 // fused into it, which then rounds differently on the two lanes of a pair.
 __device__ __forceinline__ float wave_total(float x) {
   return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(group_sum<64>(x))));
 }
 
-// A row's normaliser and what it makes of a value.
+// A row's normaliser, about its maximum, and what it makes of a value.
 struct Normaliser {
-  float c, log2_s, mx;
-  bool extreme;
+  float mx, log2_s;
 
   __device__ __forceinline__ float logprob(float x) const {
-    if (extreme || fabsf(x) > TLP_EXTREME) return (x - mx) - LN2_F * log2_s;
-    return LN2_F * (fmaf(x, LOG2E_F, -c) - log2_s);
+    return fmaf(-LN2_F, log2_s, x - mx);
   }
 };
 
@@ -125,9 +150,9 @@ __device__ __forceinline__ void rank_candidates(const float *cv, const int *ci, 
   }
 }
 
-// One segment's sums and maximum, kept for the join.
-struct Partial {
-  float c, s, w, mx;
+// One segment's maximum and sums about it, kept for the join.
+struct alignas(16) Partial {
+  float mx, s, w;
 };
 
 // Where a workgroup's results go: a row's final figures, or a segment's for the join.
@@ -217,8 +242,8 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
     if (__builtin_amdgcn_ballot_w64(need) != 0) sums.move(need ? to : sums.c);
   };
   auto add = [&](float v, float &s, float &w) {
-    // one fused step, the same for a row's given tokens: what c lost in rounding is lost by
-    // every term alike and cancels.  exp2(-inf) = 0 must not meet its -inf.
+    // one fused step: what c lost in rounding every term carries alike.  exp2(-inf) = 0 must
+    // not meet its -inf.
     const float t = fmaf(v, LOG2E_F, -sums.c), e = fast_exp2(t);
     s += e;
     w = fmaf(fmaxf(t, TLP_FLOOR), e, w);
@@ -254,9 +279,10 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
     g = fmaxf(g, dpp<DPP_ROW_MIRROR>(g));
   }
   if (tid % GL == 0) s_group[tid / GL] = g;
-  sums.move(wave_max64(sums.c));
-  const float ws = group_sum<64>(sums.s), ww = group_sum<64>(sums.w);
-  if (lane == 0) s_red[0][wave] = sums.c, s_red[1][wave] = ws, s_red[2][wave] = ww;
+  const float wmx = wave_max64(tmax);
+  const Stats own(sums, wmx);
+  const float ws = group_sum<64>(own.s), ww = group_sum<64>(own.w);
+  if (lane == 0) s_red[0][wave] = wmx, s_red[1][wave] = ws, s_red[2][wave] = ww;
   __syncthreads();
   g = s_group[lane];
   const float mx = wave_max64(g);
@@ -282,35 +308,31 @@ __global__ __launch_bounds__(NT, OCC) void token_logprobs_kernel(
     }
   }
   // the waves' sums, joined by every wave for itself
-  Sums all{TLP_NONE, 0.f, 0.f};
-  if (lane < NWAVE) all = Sums{s_red[0][lane], s_red[1][lane], s_red[2][lane]};
-  all.move(wave_max64(all.c));
+  Stats all{mx, 0.f, 0.f};
+  if (lane < NWAVE) all = Stats{s_red[0][lane], s_red[1][lane], s_red[2][lane]};
+  all.move(mx);
   float S = wave_total(all.s), W = wave_total(all.w);
-  const bool extreme = fabsf(mx) > TLP_EXTREME && fabsf(mx) < INFINITY;
-  if (extreme) {  // its sum is the number of values that equal the maximum
-    int level = 0;
-    bool nan = false;
+  if (fabsf(mx) > TLP_FAR && fabsf(mx) < INFINITY) {  // workgroup-uniform
+    float s = 0.f, w = 0.f;
 #pragma nounroll
     for (int i = tid; i < n; i += NT) {
-      const float v = logit<DT>(x[i]);
-      level += v == mx;
-      nan |= v != v;
+      const float t = (logit<DT>(x[i]) - mx) * LOG2E_F, e = fast_exp2(t);
+      s += e;
+      w = fmaf(fmaxf(t, TLP_FLOOR), e, w);
     }
-    for (int d = 1; d < 64; d *= 2) level += __shfl_xor(level, d);
-    nan = __syncthreads_or(nan);
-    if (lane == 0) s_bi[wave] = level;
+    s = group_sum<64>(s), w = group_sum<64>(w);
+    __syncthreads();  // the waves' sums have been read
+    if (lane == 0) s_red[1][wave] = s, s_red[2][wave] = w;
     __syncthreads();
-    level = 0;
-    for (int w = 0; w < NWAVE; ++w) level += s_bi[w];
-    S = nan ? NAN : (float)level, W = 0.f;
-    __syncthreads();  // s_bi may be written again
+    S = wave_total(lane < NWAVE ? s_red[1][lane] : 0.f);
+    W = wave_total(lane < NWAVE ? s_red[2][lane] : 0.f);
   }
   // a NaN, +inf or an empty row leaves S NaN or 0
   const bool bad = !SPLIT && !(S > 0.f);
-  const Normaliser norm{all.c, log2f(S), mx, extreme};
+  const Normaliser norm{mx, log2f(S)};
   const int64_t seg = SPLIT ? row * gridDim.y + blockIdx.y : row;
   if constexpr (SPLIT) {
-    if (tid == 0) o.part[seg] = Partial{all.c, S, W, mx};
+    if (tid == 0) o.part[seg] = Partial{mx, S, W};
   } else {
     if (tid == 0) o.entropy[row] = bad ? NAN : LN2_F * (norm.log2_s - W / S);
     for (int i = tid; i < o.num_tokens; i += NT) {
@@ -407,18 +429,14 @@ __global__ __launch_bounds__(TLP_JOIN_NT) void token_logprobs_join_kernel(
   const int tid = threadIdx.x, lane = tid & 63, k = o.k, count = segments * k;
   for (int i = tid; i < count; i += TLP_JOIN_NT)
     s_cv[i] = o.cand[row * count + i], s_ci[i] = o.cand_id[row * count + i];
-  Partial p{TLP_NONE, 0.f, 0.f, NEG_INF_F};
+  Partial p{NEG_INF_F, 0.f, 0.f};
   if (lane < segments) p = o.part[row * segments + lane];
   const float mx = wave_max64(p.mx);
-  const bool extreme = fabsf(mx) > TLP_EXTREME && fabsf(mx) < INFINITY;
-  // a segment that counted its values at an extreme maximum has weight 0 elsewhere
-  const bool counted = fabsf(p.mx) > TLP_EXTREME && fabsf(p.mx) < INFINITY;
-  const bool apart = p.s == p.s && (extreme ? p.mx != mx : counted);
-  Sums all{apart || extreme ? TLP_NONE : p.c, apart ? 0.f : p.s, apart ? 0.f : p.w};
-  all.move(wave_max64(all.c));
+  Stats all{p.mx, p.s, p.w};
+  all.move(mx);
   const float S = wave_total(all.s), W = wave_total(all.w);
   const bool bad = !(S > 0.f);
-  const Normaliser norm{all.c, log2f(S), mx, extreme};
+  const Normaliser norm{mx, log2f(S)};
   if (tid == 0) o.entropy[row] = bad ? NAN : LN2_F * (norm.log2_s - W / S);
   const typename Elem<DT>::T *x = logits + row * stride;
   for (int i = tid; i < o.num_tokens; i += TLP_JOIN_NT) {
