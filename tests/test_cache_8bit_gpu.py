@@ -585,3 +585,34 @@ def test_decode_together():
         assert torch.equal(ids, order[:, :3])
         assert (top.double() - logp.gather(1, ids)).abs().max() < 4e-6
     same_cache(want_cross, cross)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,beams,dim", [([300, 64, 17, 1, 0], 1, 64), ([5003], 3, 64),
+                                            ([90, 33], 4, 128)])
+@pytest.mark.parametrize("power,scale", [(10, 0.125), (26, 0.125), (34, -0.3), (60, 0.125),
+                                         (100, -0.3), (0, 1e30), (0, -3e38), (100, 1e-35),
+                                         (110, 0.0), (118, 1e-42)])
+def test_attention_scores_of_any_size(dtype, lens, beams, dim, power, scale):
+    """Scores so large that their product with log2 e holds no units, whole and split: whole
+    numbers times 2^power, which fp32 sums hold exactly (below 2^24 and 2^128), so that equal
+    ones share the weight and a score's own error (the bound's `size`) is 0.  A difference times
+    the scale is rounded twice, 2^-23 of an exponent that adds weight only below 32."""
+    from vflorence_amd import hip_attn
+
+    query, cache, row_lens, tables, dev, starts = paged_case(power, dtype, dim, 16, lens, beams)
+    gen = torch.Generator().manual_seed(power)
+    query.copy_(torch.randint(-2, 3, query.shape, generator=gen))
+    cache[0].copy_(torch.randint(-4, 5, cache[0].shape, generator=gen).float().to(E4M3))
+    cache[2][..., 0] = 2.0**power
+    cache[2][::3, :, 0] = 2.0**(power - 1)
+    out = torch.full_like(query, 7.0)
+    hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=scale,
+                                          block_table=dev[1],
+                                          scheduler_metadata=metadata(query, 16, beams, starts))
+    want, weight, size = attend(query, Cache.of(*cache).values(), row_lens, tables, scale)
+    tol = attend_tolerance(dtype, dim, max(lens), want, weight, torch.zeros_like(size))
+    tol = tol + 32 * 2.0**-22 * weight
+    worst = ((out.cpu().double() - want).abs() / tol).max()
+    print(f"error / bound {float(worst):.3f}", flush=True)
+    assert worst <= 1, float(worst)

@@ -174,7 +174,7 @@ struct Attn8Args {
 };
 
 constexpr int ATTN8_COLS = 8;  // rows of a group
-constexpr float NO_SCORE = -3e38f;
+constexpr float NO_SCORE = -3.402823466e38f;  // the least finite score
 
 // Maximum across the four 16-lane rows, a NaN passed on.
 __device__ __forceinline__ float rows_maximum4(float x) {
@@ -268,7 +268,9 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   // the sum of the weights, of the row `col`: the same products with a row of ones for V
   floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
   const uint4 ones = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  float m = NO_SCORE;  // below every score: the first one moves it
+  // A row's reference, an unscaled score; weights are exp2((score - m) * scale_log2).  (A product
+  // m * scale_log2 would lose its units from 2^24 on, and exp2's whole range from 2^32.)
+  float m = NEG_INF_F;  // the first score moves it
 
   // A part's tile is read through a buffer descriptor that ends with its last token: what lies
   // behind, or an id outside the pool, or dims past the head, reads as 0 without a branch.
@@ -344,10 +346,10 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
         __builtin_elementwise_maximum(
             __builtin_elementwise_maximum(__builtin_elementwise_maximum(y[0][3], y[1][0]), y[1][1]),
             __builtin_elementwise_maximum(y[1][2], y[1][3])));
-    mb = rows_maximum4(mb) * a.scale_log2;
-    const bool need = mb > m + RESCALE_SLACK_LOG2;
+    mb = rows_maximum4(mb);
+    const bool need = (mb - m) * a.scale_log2 > RESCALE_SLACK_LOG2;
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
-      const float corr = need ? fast_exp2(m - mb) : 1.f;
+      const float corr = need ? fast_exp2((m - mb) * a.scale_log2) : 1.f;
       sum *= corr;
 #pragma unroll
       for (int s = 0; s < NS; ++s)
@@ -355,11 +357,12 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
         for (int c = 0; c < 4; ++c) acc[s][c] *= corr;
       m = need ? mb : m;
     }
+    const float ref = __builtin_elementwise_maximum(m, NO_SCORE);  // (-inf - -inf is no score)
     float w[2][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[u][j] = fast_exp2(fmaf(y[u][j], a.scale_log2, -m));
+      for (int j = 0; j < 4; ++j) w[u][j] = fast_exp2((y[u][j] - ref) * a.scale_log2);
     uint4 pop[PT];
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
@@ -429,7 +432,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           s_acc[wave][64 * s + 16 * rg + 4 * j + c][col] = acc[s][c][j];
-    if (rg == 0) s_ml[wave][0][col] = m, s_ml[wave][1][col] = sum[0];
+    if (rg == 0) s_ml[wave][0][col] = fmaxf(m, NO_SCORE), s_ml[wave][1][col] = sum[0];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < nrows * D; i += 64 * NW) {
@@ -440,7 +443,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
     float S = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = fast_exp2(s_ml[w][0][r] - M);
+      const float f = fast_exp2((s_ml[w][0][r] - M) * a.scale_log2);
       S = fmaf(s_ml[w][1][r], f, S);
       o = fmaf(s_acc[w][d][r], f, o);
     }
@@ -477,7 +480,8 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
     for (int s = team; s < a.splits; s += teams) {
       const float2 x = ml[s];
       const float4 v = acc[(int64_t)s * quads];
-      const float to = fmaxf(M, x.x), f = fast_exp2(M - to), e = fast_exp2(x.x - to);
+      const float to = fmaxf(M, x.x);
+      const float f = fast_exp2((M - to) * a.scale_log2), e = fast_exp2((x.x - to) * a.scale_log2);
       S = S * f + x.y * e;
       o.x = o.x * f + v.x * e, o.y = o.y * f + v.y * e;
       o.z = o.z * f + v.z * e, o.w = o.w * f + v.w * e;
@@ -492,7 +496,7 @@ __global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn
     for (int t = 0; t < teams; ++t) top = fmaxf(top, s_ml[t * quads + d / 4].x);
     for (int t = 0; t < teams; ++t) {
       const float2 x = s_ml[t * quads + d / 4];
-      const float e = fast_exp2(x.x - top);
+      const float e = fast_exp2((x.x - top) * a.scale_log2);
       sum = fmaf(x.y, e, sum);
       y = fmaf((&s_o[t * quads + d / 4].x)[d % 4], e, y);
     }
@@ -617,7 +621,9 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
               (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
               block_table_stride, (int)table, (int)table * block_size, group_start, group_order,
               num_rows, num_groups, num_heads, head_dim, num_blocks,
-              fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f),  // (0 * -inf is no score)
+              // finite and not 0, which would make NaN of an equal or a masked score (the least
+              // denormal in its place moves no weight by more than 2^-21)
+              fminf(fmaxf(fabsf(scale) * 1.4426950408889634f, __FLT_DENORM_MIN__), -NO_SCORE),
               !(scale < 0.f) ? 0u : dtype == VFL_FLOAT32 ? 0x80000000u : 0x80008000u,
               (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
                   query_stride_head % (16 / eb) == 0,
