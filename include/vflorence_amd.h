@@ -513,10 +513,12 @@ int vfl_encoder_attention(const void *q, const void *k, const void *v, int64_t s
  * counterpart.
  *
  * vfl_reshape_and_cache_8bit: vfl_reshape_and_cache into such a cache, same slots and strides.
- * Consecutive tokens whose slots lie in one block are a run (of a slot that comes twice in it,
- * the later token); a block's tokens must form one run of the call, and a block belong to one
- * sequence (a second run in the call, or a call that overlaps this one on another stream,
- * would race for the block's scale).  Per run and head, for K and for V,
+ * Tokens one after another whose slots lie in one block are a run (of a slot that comes twice in
+ * it, the later token); skipped tokens, whose slots lie outside the pool, are as if they were
+ * not in the call and end no run.  A block's tokens must form one run of the call, and a block
+ * belong to one sequence (a second run in the call, behind another block's token, or a call
+ * that overlaps this one on another stream would race for the block's scale).  Per run and
+ * head, for K and for V,
  *   new = max(old, the smallest power of two with max |x| / new <= 448)   (2^-100 at least)
  * where max is over the run's finite values and old = 0 when the run holds the block's first
  * slot: the block then starts over, and its other slots become 0.  Else they become rnd(q *

@@ -153,6 +153,81 @@ def test_append_out_of_order_and_repeated_slots(dim, bs):
     same_cache(want, cache)
 
 
+@pytest.mark.parametrize("bs,dim,dtype", [(16, 64, torch.bfloat16), (32, 64, torch.float16),
+                                          (16, 192, torch.float32)])
+@pytest.mark.parametrize("tail", [0, 600])
+def test_append_skips_tokens_inside_runs(bs, dim, dtype, tail):
+    """Skipped tokens are as if they were not in the call: inside a block's run, before its first
+    and after its last token, more of them than a wave sees at once, and between tokens out of
+    order.  (Were each side of a gap a run of its own, both would write the block's scale.)"""
+    from vflorence_amd import hip_attn
+
+    gen = torch.Generator().manual_seed(bs + dim + tail)
+    blocks, heads = 60, 3
+    past = blocks * bs + 5
+    slots = [-1, past, 0, 1, -1, 2, 5 * bs + 1, -1, past, 5 * bs + 2, -7, 3 * bs]
+    for gap in (1, 14, 15, 16, 17, 62, 63, 64, 65, 127, 128, 200):
+        block = 6 + len(slots) % 3 + 3 * (gap % 7)
+        offsets = torch.randperm(bs, generator=gen)[:5].tolist()
+        if gap % 2:
+            offsets.sort()
+        if any(s // bs == block for s in slots):
+            block = next(b for b in range(30, blocks) if all(s // bs != b for s in slots))
+        slots += [block * bs + offsets[0]] + [-1] * gap + [block * bs + o for o in offsets[1:3]]
+        slots += [past] * (gap % 20) + [block * bs + o for o in offsets[3:]]
+    slots += [-1] * 70
+    if tail:
+        slots = [-1] * tail + slots + [blocks * bs] * tail
+    slots = torch.tensor(slots)
+    cache = random_cache(gen, blocks, heads, bs, dim)
+    want = Cache.of(*cache)
+    key, value = tokens_of(gen, len(slots), heads, dim, dtype, spread=3.0)
+    for t in range(4):  # whole calls of a few tokens, ends skipped or not
+        part = slice(3 * t + tail, 3 * t + 3 + tail)
+        few, mine = slots[part].clone(), [t.clone() for t in cache]
+        hip_attn.reshape_and_cache_8bit(key[part], value[part], *mine, few.to(DEV))
+        other = Cache.of(*cache)
+        kept = (few >= 0) & (few < blocks * bs)
+        other.append(key[part][kept.to(DEV)], value[part][kept.to(DEV)], few[kept])
+        same_cache(other, mine)
+    hip_attn.reshape_and_cache_8bit(key, value, *cache, slots.to(DEV))
+    kept = (slots >= 0) & (slots < blocks * bs)
+    want.append(key[kept.to(DEV)], value[kept.to(DEV)], slots[kept])
+    same_cache(want, cache)
+
+
+@pytest.mark.parametrize("count,bs", [(300, 16), (511, 16), (2000, 16), (2000, 32)])
+def test_append_padded_prompts(count, bs):
+    """A padded batch: every prompt's tokens followed by skipped ones, some inside it as well;
+    the same cache as of the call without them, and on every run."""
+    from vflorence_amd import hip_attn
+
+    gen = torch.Generator().manual_seed(count + bs)
+    heads, dim, slots, block = 5, 64, [], 0
+    while len(slots) < count:
+        n, first, gap = (int(torch.randint(lo, hi, (1,), generator=gen))
+                         for lo, hi in ((1, 5 * bs), (0, bs), (0, 150)))
+        for t in range(n):
+            slots += [-1] * int(torch.rand(1, generator=gen) < 0.2) + [block * bs + first + t]
+        slots += [-1] * gap
+        block += (first + n + bs - 1) // bs
+    slots = torch.tensor(slots[:count])
+    cache = random_cache(gen, block, heads, bs, dim)
+    key, value = tokens_of(gen, count, heads, dim, torch.bfloat16, spread=3.0)
+    kept = slots >= 0
+    packed = [t.clone() for t in cache]
+    hip_attn.reshape_and_cache_8bit(key[kept.to(DEV)], value[kept.to(DEV)], *packed,
+                                    slots[kept].to(DEV))
+    want = Cache.of(*cache)
+    want.append(key[kept.to(DEV)], value[kept.to(DEV)], slots[kept])
+    same_cache(want, packed)
+    for _ in range(3):
+        padded = [t.clone() for t in cache]
+        hip_attn.reshape_and_cache_8bit(key, value, *padded, slots.to(DEV))
+        for a, b in zip(padded, packed):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("offset,head_stride,token_stride", [(0, 96, 200), (1, 65, 131),
                                                              (3, 64, 129)])

@@ -1,8 +1,9 @@
 // Appending keys and values to a paged cache held in e4m3, one scale per (block, head) for
 // K and one for V (gfx950).
 //
-// A run is the consecutive tokens of a call whose slots lie in one block (of a slot that comes
-// twice, the later token).  Per run and head
+// A run is the tokens of a call, one after another, whose slots lie in one block (of a slot that
+// comes twice, the later token).  Skipped tokens, whose slots lie outside the pool, are as if they
+// were not in the call: a run goes on behind them.  Per run and head
 //   a = max |x| over the run's finite values,  need = the smallest power of two with
 //   a / need <= 448,  new = max(old, need)  (old = 0 where the run holds the block's offset
 //   0: the block starts over, what it held is dropped)
@@ -188,28 +189,55 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
   const int64_t slot = slots[min(max(tl, 0), T - 1)];
   const int bl = tl >= 0 && tl < T ? block_of(slot) : -1;
   const int off = (int)(slot & (BS - 1));
-  const int before = __shfl_up(bl, 1);
-  uint64_t leaders = __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= window && bl >= 0 &&
-                                                 bl != before);
+  const uint64_t own = ((1ull << window) - 1) << 1;  // the window's lanes
+  const uint64_t past = T - t0 < 63 ? ~0ull << (T - t0 + 1) : 0;  // lanes behind the last token
+  const uint64_t held = __builtin_amdgcn_ballot_w64(bl >= 0);
+  int before = __shfl_up(bl, 1);  // block of the last token that is not skipped
+  if (__builtin_expect((~(held | past) & (own | (t0 > 0))) != 0, 0)) {  // some are
+    const uint64_t lower = held & ((1ull << lane) - 1);
+    int first = -1;  // the block before the wave's first one: 64 tokens at a time
+    if (!(held & 1) && (held & own))
+      for (int end = t0 - 2; end >= 0; end -= 64) {
+        const int b = end >= lane ? block_of(slots[end - lane]) : -1;
+        const uint64_t found = __builtin_amdgcn_ballot_w64(b >= 0);
+        if (found) {
+          first = __builtin_amdgcn_readlane(b, __builtin_ctzll(found));
+          break;
+        }
+      }
+    before = __shfl(bl, lower ? 63 - __builtin_clzll(lower) : 0);
+    if (!lower) before = first;
+  }
+  uint64_t leaders = __builtin_amdgcn_ballot_w64(bl >= 0 && bl != before) & own;
 
   for (; leaders; leaders &= leaders - 1) {
     const int at = __builtin_ctzll(leaders), t = t0 - 1 + at;
     const int blk = __builtin_amdgcn_readlane(bl, at);
-    // lane o: the run's token that takes the block's offset o (its last one), from t on
-    const uint64_t differ = ~(__builtin_amdgcn_ballot_w64(bl == blk) >> at);
-    const int n = differ ? __builtin_ctzll(differ) : 64;
+    // n tokens side by side, and whether the run may go on behind skipped tokens or the wave's
+    const int n0 = __builtin_ctzll(~(__builtin_amdgcn_ballot_w64(bl == blk) >> at));
+    const bool on = at + n0 == 64 || !(((held | past) >> (at + n0)) & 1);
+    // lane o: the run's token that takes the block's offset o (its last one), from t on; n, the
+    // run's tokens; last, its last token (which is always taken)
     const int off0 = __builtin_amdgcn_readlane(off, at);
-    int src = -1, last = n - 1;  // (the last token is always taken)
-    if (at + n < 64 && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
-                                                   off != off0 + lane - at) == 0) {
+    int src = -1, n = n0, last = n0 - 1;
+    if (!on && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
+                                           off != off0 + lane - at) == 0) {
       src = lane >= off0 && lane < off0 + n ? lane - off0 : -1;  // in order
     } else {
-      // any order; of a slot that comes twice the later token is taken
-      for (int i = 0; t + i < T; ++i) {
-        const int64_t s = slots[t + i];
-        if (block_of(s) != blk) break;
-        if ((int)(s & (BS - 1)) == lane) src = i;
-        last = i;
+      uint64_t ends = 0;
+      n = 0;
+      for (int i = 0; !ends; i += 64) {
+        const int64_t s = slots[min(t + i + lane, T - 1)];
+        const int b = t + i + lane < T ? block_of(s) : -1, o = (int)(s & (BS - 1));
+        uint64_t mine = __builtin_amdgcn_ballot_w64(b == blk);
+        ends = __builtin_amdgcn_ballot_w64(t + i + lane >= T || (b >= 0 && b != blk));
+        if (ends) mine &= (ends & -ends) - 1;
+        n += __builtin_popcountll(mine);
+        for (; mine; mine &= mine - 1) {
+          const int j = __builtin_ctzll(mine);
+          if (__builtin_amdgcn_readlane(o, j) == lane) src = i + j;
+          last = i + j;
+        }
       }
     }
     const bool fresh = __builtin_amdgcn_readlane(src, 0) >= 0;
@@ -407,7 +435,7 @@ extern "C" int vfl_reshape_and_cache_8bit(const void *key, const void *value,
   const int st = check_8bit_cache("reshape_and_cache_8bit", dtype, num_heads, head_dim,
                                   block_size, num_blocks);
   if (st != VFL_OK) return st;
-  if (num_tokens < 0 || (num_tokens + XCDS) * num_heads > 2147483647LL) {
+  if (num_tokens < 0 || (num_tokens + 64) * num_heads > 2147483647LL) {
     set_error("reshape_and_cache_8bit: %lld tokens x %d heads", (long long)num_tokens, num_heads);
     return VFL_E_INVALID;
   }

@@ -868,9 +868,11 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
 
     key/value: [T, H, D] in float32, bfloat16 or float16, any token and head strides, a
     contiguous last dimension.  slot_mapping: int64 [T]; a token whose slot is negative or
-    past the pool is skipped.  A block's tokens of one call must follow one another in it
-    (as positions of a sequence do), and a block appended to must belong to one sequence.
-    Of a slot that comes twice in a block's run, the later token is taken.
+    past the pool is skipped, as if it were not in the call.  A block's tokens of one call must
+    follow one another in it (as positions of a sequence do; skipped tokens between them do not
+    count, another block's token does: the block's scale would have two writers), and a block
+    appended to must belong to one sequence.  Of a slot that comes twice in a block's run, the
+    later token is taken.
 
     A block's scale is a power of two that brings its largest value to 448 or less.  It only
     grows: what the block holds is then rescaled, exactly but for values under e4m3's smallest
