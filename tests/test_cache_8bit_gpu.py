@@ -365,6 +365,28 @@ def test_attention_long_contexts(dtype, bs, dim, lens, beams):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bs,dim,heads,lens,beams", [
+    (16, 64, 1, [2555], 1), (16, 64, 5, [20011], 1), (16, 48, 1, [7000, 33, 0], 1),
+    (32, 80, 3, [9001], 3), (16, 128, 1, [5001], 5)])
+def test_attention_odd_number_of_parts(dtype, bs, dim, heads, lens, beams):
+    """Rows x heads x parts of a context odd: the workspace keeps its vectors aligned."""
+    from vflorence_amd import hip_attn
+    from vflorence_amd._lib import lib
+
+    query, cache, row_lens, tables, dev, starts = paged_case(dim, dtype, dim, bs, lens, beams,
+                                                             heads)
+    need = lib.vfl_attention_8bit_workspace(len(row_lens), len(lens), heads, dim, bs,
+                                            dev[1].shape[1])
+    parts = need // (4 * dim + 8)
+    assert parts % 2 and parts > len(row_lens) * heads
+    out = torch.full_like(query, 7.0)
+    hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=dim**-0.5,
+                                          block_table=dev[1],
+                                          scheduler_metadata=metadata(query, bs, beams, starts))
+    close(query, out, Cache.of(*cache), row_lens, tables, dim**-0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bs", [16, 32])
 def test_attention_ignores_what_lies_behind(dtype, bs):
     """NaN elements and NaN scales behind a row's last token, in its last block and in

@@ -147,7 +147,8 @@ __device__ __forceinline__ int clamp_scalar(int x) {
   return r;
 }
 
-// What is added to a softmax when its context is split: [row][head][split].
+// What is added to a softmax when its context is split: [row][head][split].  The sums come first
+// in the workspace: whole 64-byte pieces, 16-byte aligned for any number of parts.
 struct SplitOut {
   float *acc;  // [D]
   float2 *ml;
@@ -637,8 +638,8 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
     }
     a.splits = plan.splits;
     const int64_t parts = num_rows * num_heads * plan.splits;
-    a.part.ml = (float2 *)workspace;
-    a.part.acc = (float *)(a.part.ml + parts);
+    a.part.acc = (float *)workspace;
+    a.part.ml = (float2 *)(a.part.acc + parts * head_dim);
   }
   hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto dt) {
