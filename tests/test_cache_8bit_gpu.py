@@ -713,3 +713,46 @@ def test_attention_scores_of_any_size(dtype, lens, beams, dim, power, scale):
     worst = ((out.cpu().double() - want).abs() / tol).max()
     print(f"error / bound {float(worst):.3f}", flush=True)
     assert worst <= 1, float(worst)
+
+
+def test_refuses_gradients_of_the_cache_and_counts_writes():
+    """Pools and scales that require gradients are refused as queries, keys and values are; what
+    a call writes counts as written, so that autograd sees a saved tensor change."""
+    from vflorence_amd import hip_attn
+
+    query, cache, _, _, dev, _ = paged_case(16, torch.bfloat16, 64, 16, [20, 40])
+    key = torch.ones(2, 2, 64, device=DEV)
+    slots = torch.tensor([3, 20], device=DEV)
+
+    def attend_into(out):
+        hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=0.125,
+                                              block_table=dev[1])
+
+    def append():
+        hip_attn.reshape_and_cache_8bit(key, key, *cache, slots)
+
+    out = torch.empty_like(query)
+    for call, written in ((append, cache), (lambda: attend_into(out), (out,))):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > v for t, v in zip(written, before))
+    for t in cache:
+        t.requires_grad_(True)
+        for call in (append, lambda: attend_into(out)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad():
+                call()
+        t.requires_grad_(False)
+    x = torch.ones(query.shape, device=DEV, requires_grad=True)
+    saved = torch.empty(query.shape, device=DEV)
+    loss = (x * saved).sum()  # saves `saved`
+    hip_attn.attention_with_kv_cache_8bit(query.float(), *cache, saved, dev[0], scale=0.125,
+                                          block_table=dev[1])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # (whose own tensors count no versions)
+        held = hip_attn.kv_cache_8bit(4, 2, 16, 64, DEV)
+        hip_attn.reshape_and_cache_8bit(key, key, *held, slots)
+        other = torch.empty_like(query)
+        attend_into(other)

@@ -846,15 +846,16 @@ def one_gpu(*tensors: torch.Tensor) -> int:
     """The index of the GPU that holds all of the tensors (``_require_gpu``'s errors; integers,
     as device objects cost a small call 2 us)."""
     index = tensors[0].get_device()
-    if index < 0 or any(t.get_device() != index for t in tensors):
-        _require_gpu(*tensors)
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            _require_gpu(*tensors)
     return index
 
 
 def on_device(index: int, function, *args) -> None:
     """A checked C-ABI call on a GPU and its current stream, the last argument (a null stream
     handle, every default stream's, means the current device's)."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         check(function(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
@@ -891,7 +892,8 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
         raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
                          f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
     index = one_gpu(key, value, k_cache, v_cache, kv_scales, slot_mapping)
-    if key.requires_grad or value.requires_grad:
+    if (key.requires_grad or value.requires_grad or k_cache.requires_grad
+            or v_cache.requires_grad or kv_scales.requires_grad):
         refuse_gradients("reshape_and_cache_8bit")
     slot_mapping = slot_mapping.contiguous()
     on_device(index, lib.vfl_reshape_and_cache_8bit, key.data_ptr(), value.data_ptr(),
@@ -899,6 +901,8 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
               k_cache.data_ptr(), v_cache.data_ptr(), kv_scales.data_ptr(),
               slot_mapping.data_ptr(), key.shape[0], num_heads, head_dim, block_size, num_blocks,
               dtype)
+    # autograd's check of saved tensors
+    torch.autograd.graph.increment_version((k_cache, v_cache, kv_scales))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -937,7 +941,8 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
         raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
                          f"{block_table.dtype} {tuple(block_table.shape)}")
     index = one_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
-    if query.requires_grad or out.requires_grad:
+    if (query.requires_grad or out.requires_grad or k_cache.requires_grad
+            or v_cache.requires_grad or kv_scales.requires_grad):
         refuse_gradients("attention_with_kv_cache_8bit")
     width = block_table.shape[1]
     if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
@@ -972,6 +977,7 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
               None if order is None else order.data_ptr(), num_rows, num_groups, num_heads,
               head_dim, block_size, num_blocks, float(scale), dtype,
               workspace.data_ptr() if need else None)
+    torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
 
 
 def cache_pointer_table(caches: list[torch.Tensor]) -> torch.Tensor:
