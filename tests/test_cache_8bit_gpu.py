@@ -495,6 +495,27 @@ def test_attention_any_finite_scale(dtype, scale):
                                                   block_table=dev[1])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_largest_queries(dtype):
+    """One dim of a query at its type's largest value, of either sign, over small keys: the weight
+    lies on the tokens whose key has the largest product with it, which share it."""
+    from vflorence_amd import hip_attn
+
+    query, cache, lens, tables, dev, _ = paged_case(17, dtype, 64, 16, [300, 64, 17, 1])
+    gen = torch.Generator().manual_seed(17)
+    query.zero_()
+    query[:, :, 5] = torch.finfo(dtype).max
+    query[1, :, 5] *= -1
+    cache[0].copy_(torch.randint(-4, 5, cache[0].shape, generator=gen).float().to(E4M3))
+    cache[2][..., 0] = 2.0**-8  # (fp16: products a hundred apart and more)
+    out = torch.empty_like(query)
+    hip_attn.attention_with_kv_cache_8bit(query, *cache, out, dev[0], scale=1.0,
+                                          block_table=dev[1])
+    want, weight, size = attend(query, Cache.of(*cache).values(), lens, tables, 1.0)
+    tol = attend_tolerance(dtype, 64, 300, want, weight, torch.zeros_like(size))
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("length", [45, 6000])
 def test_attention_in_place_and_broadcast_tables(length):
     """The output written over the query; rows that share one expanded table and length; a

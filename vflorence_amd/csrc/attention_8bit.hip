@@ -44,9 +44,20 @@ template <int DT> struct Terms {
 
 using Bf16 = Mfma<VFL_BFLOAT16>;
 
-// bf16 terms of four floats, largest first; f is left with the remainder.
-__device__ __forceinline__ uint2 take_bf16(float (&f)[4]) {
-  const uint2 w = make_uint2(Bf16::narrow2(f[0], f[1]), Bf16::narrow2(f[2], f[3]));
+// bf16 terms of four floats, largest first; f is left with the remainder.  Queries are cut, weights
+// rounded: a cut term holds 8 bits and the next ones start behind it, so two hold all of fp16 and
+// three all of fp32 either way, and the largest fp32 values, which would round to infinity,
+// stay finite; of two or three terms that do not hold everything rounding leaves half as much.
+template <bool ROUND> __device__ __forceinline__ uint2 take_bf16(float (&f)[4]) {
+  uint2 w;
+  if constexpr (ROUND) {
+    w = make_uint2(Bf16::narrow2(f[0], f[1]), Bf16::narrow2(f[2], f[3]));
+  } else {
+    constexpr uint32_t HIGH_HALVES = 0x07060302u;
+    w = make_uint2(
+        __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), HIGH_HALVES),
+        __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), HIGH_HALVES));
+  }
   f[0] -= Bf16::widen_lo(w.x), f[1] -= Bf16::widen_hi(w.x);
   f[2] -= Bf16::widen_lo(w.y), f[3] -= Bf16::widen_hi(w.y);
   return w;
@@ -367,7 +378,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
     uint4 pop[PT];
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
-      const uint2 p0 = take_bf16(w[0]), p1 = take_bf16(w[1]);
+      const uint2 p0 = take_bf16<true>(w[0]), p1 = take_bf16<true>(w[1]);
       pop[t] = make_uint4(p0.x, p0.y, p1.x, p1.y);
     }
 #pragma unroll
@@ -406,7 +417,7 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
           float f0[4] = {f[0], f[1], f[2], f[3]}, f1[4] = {f[4], f[5], f[6], f[7]};
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            const uint2 lo = take_bf16(f0), hi = take_bf16(f1);
+            const uint2 lo = take_bf16<false>(f0), hi = take_bf16<false>(f1);
             qop[s][e][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
           }
         }
