@@ -20,15 +20,16 @@
 // What bounds it: HBM where there is enough to read (64 groups of 4 rows x 16 heads of 64, 2048
 // tokens each: 46 us, 5.8 TB/s; 256 to 1024 tokens, 85 MB: 18.0 us, of which 5.1 are the launch
 // and five dependent loads -- arguments, order, group, length and block ids, pages -- and the
-// merge).  Vector operations take 42% of the cycles (about 145 per 32 tokens, 64 dims: 32
-// conversions, 8 exponentials, 24 that split the weights), matrix products 11%.  What each
-// step gave, us, the same 256 to 1024 tokens / 93 single rows to 1000 tokens, fp16 / 2 rows to
-// 39999 tokens:
+// merge).  The vector units are busy for 7.2 us of these (about 147 operations per 32 tokens, 64
+// dims: 32 conversions, 16 differences and products of the softmax, 8 exponentials, 24 that
+// split the weights), the matrix units for 1.9 (cycles at 2.4 GHz).  What each step gave, us,
+// the same 256 to 1024 tokens / 93 single rows to 1000 tokens, fp16 / 2 rows to 39999 tokens:
 //   loads under conditions, each waited for        23.0 / 28.0 / 675
 //   buffer loads one iteration ahead, splits       19.6 / 23.7 / 49
 //   descriptors in scalar registers, a faster join 18.6 / 21.0 / 30.6
 //   scales in the conversions, weights summed by
 //   matrix products, non-temporal loads            18.0 / 21.6 / 27.0
+//   weights from differences of unscaled scores    18.2 / 21.8 / 27.8
 #include <math.h>
 #include <stdio.h>
 

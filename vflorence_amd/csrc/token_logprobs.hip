@@ -24,8 +24,8 @@ constexpr float TLP_FLOOR = -1e4f;  // exp2() is 0 long before
 // 2^32 on: they are summed in a second read, from the differences.
 constexpr float TLP_FAR = 65536.f;
 constexpr float TLP_NONE = -1e5f;  // a thread's first reference: below every such maximum's
-// log2 units a reference may lag behind.  A thread's terms are up to 2^16, its sum of up to 112
-// below 2^23; about the maximum a row's 2^20 terms sum to 2^20 at most.
+// log2 units a reference may lag behind.  A thread's terms are up to 2^16, its sum of up to 57
+// below 2^22; about the maximum a row's 2^20 terms sum to 2^20 at most.
 constexpr float TLP_SLACK = 16.f;
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 
@@ -172,8 +172,8 @@ struct LogprobOut {
 // What bounds it: many rows the vector work, 17 operations a value with k = 5 (one of them
 // the exponential, at a quarter of their rate), two workgroups of 64 VGPRs a CU overlapping
 // it with the other's loads; few rows their own chain of loads,
-// exponentials and picks.  Device time, us: 4096 x 50265 bf16 k = 5 93 (4.4 TB/s), k = 0 82
-// (5.0); 256 x 50265 k = 0 8.5; 4 x 51289 k = 8 8.5; 93 x 51289 fp32 k = 20 10.7.  What
+// exponentials and picks.  Device time, us: 4096 x 50265 bf16 k = 5 92 (4.5 TB/s), k = 0 81
+// (5.1); 256 x 50265 k = 0 8.2; 4 x 51289 k = 8 8.5; 93 x 51289 fp32 k = 20 10.6.  What
 // the steps gave (the same cases): loads that no condition holds back 106 -> 93, 10.4 ->
 // 8.5; ranks by ballot and packed compares for the alternatives k = 8 10.0 -> 8.5, k = 20
 // 13.1 -> 10.7.
