@@ -196,6 +196,26 @@ def test_append_skips_tokens_inside_runs(bs, dim, dtype, tail):
     same_cache(want, cache)
 
 
+@pytest.mark.parametrize("bs", [16, 32])
+@pytest.mark.parametrize("gap", [448, 479, 480, 481, 511, 512, 513, 543, 544, 1055, 1056, 5000])
+def test_append_runs_over_long_gaps(bs, gap):
+    """Runs and ends of runs on either side of more skipped tokens than one look ahead covers, and
+    a call that ends with them."""
+    from vflorence_amd import hip_attn
+
+    gen = torch.Generator().manual_seed(gap)
+    slots = [-1] * gap + [2 * bs + 3] + [-1] * gap + [2 * bs + 9, 2 * bs + 1] + [-1] * gap
+    slots += [5 * bs + 4, 7 * bs] + [-1] * gap + [7 * bs + 1, 3 * bs + 2] + [-1] * gap
+    slots = torch.tensor(slots)
+    cache = random_cache(gen, 9, 2, bs, 64)
+    want = Cache.of(*cache)
+    key, value = tokens_of(gen, len(slots), 2, 64, torch.bfloat16, spread=3.0)
+    hip_attn.reshape_and_cache_8bit(key, value, *cache, slots.to(DEV))
+    kept = slots >= 0
+    want.append(key[kept.to(DEV)], value[kept.to(DEV)], slots[kept])
+    same_cache(want, cache)
+
+
 @pytest.mark.parametrize("count,bs", [(300, 16), (511, 16), (2000, 16), (2000, 32)])
 def test_append_padded_prompts(count, bs):
     """A padded batch: every prompt's tokens followed by skipped ones, some inside it as well;

@@ -181,64 +181,95 @@ __global__ __launch_bounds__(64 * NS) void append_8bit_kernel(
   const int kd = 64 * wave + 16 * (lane & 3), vd = 64 * wave + 4 * (lane & 15);
   const bool k_in = kd < D, v_in = vd < D;
 
-  // Lane l: block and offset of token t0 - 1 + l (block -1: skipped, or no token).  One load
-  // covers the window, the token before it and the rest of its last run.
-  auto block_of = [&](int64_t slot) {
-    return slot >= 0 && slot < (int64_t)num_blocks * BS ? (int)(slot / BS) : -1;
-  };
-  const int tl = t0 - 1 + lane;
+  // Lane l: block and offset of token t0 - back + l (block -1: skipped, or no token).  One load
+  // covers the window, what lies before it and the rest of its last run.
+  constexpr int SHIFT = PARTS == 1 ? 4 : 5;
+  const uint64_t pool = (uint64_t)num_blocks << SHIFT;  // slots
+  auto block_of = [&](int64_t slot) { return (uint64_t)slot < pool ? (int)(slot >> SHIFT) : -1; };
+  const int back = window < 32 ? 32 - window : 1;
+  const int tl = t0 - back + lane;
   const int64_t slot = slots[min(max(tl, 0), T - 1)];
-  const int bl = tl >= 0 && tl < T ? block_of(slot) : -1;
+  const uint64_t own = ((1ull << window) - 1) << back;  // the window's lanes
+  const uint64_t none = __builtin_amdgcn_ballot_w64((unsigned)tl >= (unsigned)T);
+  const int bl = (unsigned)tl < (unsigned)T ? block_of(slot) : -1;
   const int off = (int)(slot & (BS - 1));
-  const uint64_t own = ((1ull << window) - 1) << 1;  // the window's lanes
-  const uint64_t past = T - t0 < 63 ? ~0ull << (T - t0 + 1) : 0;  // lanes behind the last token
   const uint64_t held = __builtin_amdgcn_ballot_w64(bl >= 0);
+  // Where many skipped tokens follow one another: the first or last of the tokens from lo up to
+  // hi (SCAN of them at most) that is not, or -1; eight loads in flight.  (16 heads: 1000 tokens
+  // before 7192 skipped ones 9.5 us, 25 with one load; every other one of 256 rows skipped 4.8.)
+  constexpr int SCAN = 512;
+  auto find_held = [&](int lo, int hi, auto backwards) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(slots + lo), 0, __builtin_amdgcn_readfirstlane((hi - lo) * 8), 0x00020000);
+    uint64_t x[SCAN / 64];
+#pragma unroll
+    for (int c = 0; c < SCAN / 64; ++c)
+      x[c] = __builtin_bit_cast(
+          uint64_t, __builtin_amdgcn_raw_buffer_load_b64(r, lane * 8 + c * 512, 0, 0));
+    int found = -1;
+#pragma unroll
+    for (int i = 0; i < SCAN / 64; ++i) {  // the one to find comes last
+      const int c = backwards.value ? i : SCAN / 64 - 1 - i;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(64 * c + lane < hi - lo && x[c] < pool);
+      if (m) found = 64 * c + (backwards.value ? 63 - __builtin_clzll(m) : __builtin_ctzll(m));
+    }
+    return found < 0 ? -1 : lo + found;
+  };
   int before = __shfl_up(bl, 1);  // block of the last token that is not skipped
-  if (__builtin_expect((~(held | past) & (own | (t0 > 0))) != 0, 0)) {  // some are
+  if (__builtin_expect((~(held | none) & (own | own >> 1)) != 0, 0)) {  // some are
     const uint64_t lower = held & ((1ull << lane) - 1);
-    int first = -1;  // the block before the wave's first one: 64 tokens at a time
-    if (!(held & 1) && (held & own))
-      for (int end = t0 - 2; end >= 0; end -= 64) {
-        const int b = end >= lane ? block_of(slots[end - lane]) : -1;
-        const uint64_t found = __builtin_amdgcn_ballot_w64(b >= 0);
-        if (found) {
-          first = __builtin_amdgcn_readlane(b, __builtin_ctzll(found));
-          break;
-        }
-      }
     before = __shfl(bl, lower ? 63 - __builtin_clzll(lower) : 0);
-    if (!lower) before = first;
+    if ((held & own) && !(held & ((1ull << back) - 1))) {  // before the wave's first one
+      int token = -1;
+      for (int hi = t0 - back; token < 0 && hi > 0; hi -= SCAN)
+        token = find_held(max(hi - SCAN, 0), hi, std::true_type{});
+      const int first = token < 0 ? -1 : block_of(slots[token]);
+      if (!lower) before = first;
+    }
   }
   uint64_t leaders = __builtin_amdgcn_ballot_w64(bl >= 0 && bl != before) & own;
 
   for (; leaders; leaders &= leaders - 1) {
-    const int at = __builtin_ctzll(leaders), t = t0 - 1 + at;
+    const int at = __builtin_ctzll(leaders), t = t0 - back + at;
     const int blk = __builtin_amdgcn_readlane(bl, at);
     // n tokens side by side, and whether the run may go on behind skipped tokens or the wave's
-    const int n0 = __builtin_ctzll(~(__builtin_amdgcn_ballot_w64(bl == blk) >> at));
-    const bool on = at + n0 == 64 || !(((held | past) >> (at + n0)) & 1);
-    // lane o: the run's token that takes the block's offset o (its last one), from t on; n, the
-    // run's tokens; last, its last token (which is always taken)
+    const uint64_t same = __builtin_amdgcn_ballot_w64(bl == blk);
+    int n = __builtin_ctzll(~(same >> at));
+    const bool on = at + n == 64 || !(((held | none) >> (at + n)) & 1);
+    // lane o: the run's token that takes the block's offset o (its last one), from t on; last, the
+    // run's last token (which is always taken)
     const int off0 = __builtin_amdgcn_readlane(off, at);
-    int src = -1, n = n0, last = n0 - 1;
-    if (!on && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
-                                           off != off0 + lane - at) == 0) {
+    int src = -1, last = n - 1;
+    if (__builtin_expect(!on && __builtin_amdgcn_ballot_w64(lane > at && lane < at + n &&
+                                                            off != off0 + lane - at) == 0,
+                         1)) {
       src = lane >= off0 && lane < off0 + n ? lane - off0 : -1;  // in order
     } else {
-      uint64_t ends = 0;
+      // which of the tokens i, i + 1, .. (offsets o of lanes `from` on) lie in the block, and
+      // which end the run
+      uint64_t mine = same >> at, ends = ((held | none) & ~same) >> at;
+      int o = off, from = at, i = 0;
       n = 0;
-      for (int i = 0; !ends; i += 64) {
-        const int64_t s = slots[min(t + i + lane, T - 1)];
-        const int b = t + i + lane < T ? block_of(s) : -1, o = (int)(s & (BS - 1));
-        uint64_t mine = __builtin_amdgcn_ballot_w64(b == blk);
-        ends = __builtin_amdgcn_ballot_w64(t + i + lane >= T || (b >= 0 && b != blk));
+      while (true) {
         if (ends) mine &= (ends & -ends) - 1;
         n += __builtin_popcountll(mine);
         for (; mine; mine &= mine - 1) {
           const int j = __builtin_ctzll(mine);
-          if (__builtin_amdgcn_readlane(o, j) == lane) src = i + j;
+          if (__builtin_amdgcn_readlane(o, from + j) == lane) src = i + j;
           last = i + j;
         }
+        if (ends) break;
+        int next = -1;
+        for (int lo = t + i + 64 - from; next < 0 && lo < T; lo += SCAN)
+          next = find_held(lo, min(lo + SCAN, T), std::false_type{});
+        if (next < 0) break;
+        i = next - t;
+        from = 0;
+        const int64_t x = slots[min(next + lane, T - 1)];
+        const int b = next + lane < T ? block_of(x) : -2;
+        o = (int)(x & (BS - 1));
+        mine = __builtin_amdgcn_ballot_w64(b == blk);
+        ends = __builtin_amdgcn_ballot_w64(b != blk && b != -1);
       }
     }
     const bool fresh = __builtin_amdgcn_readlane(src, 0) >= 0;
@@ -436,7 +467,7 @@ extern "C" int vfl_reshape_and_cache_8bit(const void *key, const void *value,
   const int st = check_8bit_cache("reshape_and_cache_8bit", dtype, num_heads, head_dim,
                                   block_size, num_blocks);
   if (st != VFL_OK) return st;
-  if (num_tokens < 0 || (num_tokens + 64) * num_heads > 2147483647LL) {
+  if (num_tokens < 0 || (num_tokens + 1024) * num_heads > 2147483647LL) {
     set_error("reshape_and_cache_8bit: %lld tokens x %d heads", (long long)num_tokens, num_heads);
     return VFL_E_INVALID;
   }
