@@ -15,7 +15,7 @@
 //
 // What bounds it: prompts HBM (64 prompts of 256 to 1024 tokens x 16 heads, bf16: 53.3 us, 4.7
 // TB/s read and written, of a copy's 5.1); steps their chain of slots, rows and stores (256 rows
-// x 16 heads 4.6 us, 4 x 12 3.0 us).  A wave takes a block's tokens of a head, so that a tile is
+// x 16 heads 4.7 us, 4 x 12 3.0 us).  A wave takes a block's tokens of a head, so that a tile is
 // written whole; the heads of a block run on one XCD, whose L2 then writes the block's line of
 // scales whole.  Magnitudes are compared as 16-bit patterns, two at a time, and the conversion
 // takes the scale's exponent off: the same prompts ran in 57.0 us with values widened, compared
