@@ -573,6 +573,87 @@ int vfl_token_logprobs(const void *logits, int64_t row_stride, int64_t rows, int
                        float *entropy, float *top_logprobs, int64_t *top_ids, void *workspace,
                        void *stream);
 
+/*
+ * Caches held in 4 bits: one pool of bytes, [num_blocks][num_heads][block_size][34 * groups] with
+ * groups = ceil(head_dim / 32), 16-byte aligned, for K and V together.  It holds e2m1 codes (OCP FP4: 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6, the fourth bit the sign) and, for each token, head and group of 32
+ * dims, K's and V's, the exponent byte e of a scale 2^(e - 127) (27 .. 252, or 255: the
+ * group's values are NaN; 0 in a pool of zeros).  The order inside a block is the library's.  No
+ * vllm_cpu_attn counterpart.
+ *
+ * vfl_reshape_and_cache_4bit: vfl_reshape_and_cache into such a cache, same slots and strides;
+ * tokens whose slots lie outside the pool are skipped, the others' slots must differ (of two
+ * tokens at one slot each byte is one's or the other's).  Per group
+ *   scale = the smallest power of two with max |x| / scale <= 6   (2^-100 at least, 2^125 at most)
+ * and the codes are rnd(x / scale), to nearest even, past 6 to 6; a group with an infinity or a
+ * NaN is NaN.  What other slots hold is left as it was.
+ *
+ * vfl_gather_cache_4bit: the way back, key[t][h][:] and value[t][h][:] as cache holds them at
+ * slot_mapping[t], rounded to dtype where that does not hold them (fp16 past its range: an
+ * infinity), 0 for a slot outside the pool.
+ *
+ * vfl_attention_with_kv_cache_4bit: vfl_attention_with_kv_cache over such a cache; groups
+ * (group_start) are rows sharing one table and length, at most 8 of them; max_group_size (1 .. 8) is
+ * how many rows the launch takes together, more of a group's run in turn.  block_table
+ * lists max_blocks_per_seq blocks a row (2^30 tokens at most; longer contexts are clamped to
+ * that); a block id outside the pool contributes nothing.  query and out share dtype; out
+ * contiguous, and either query itself or apart from it; scale finite.  Sums and softmax in fp32,
+ * the weights kept to 2^-17 (fp32: 2^-25) through the product with V.  A launch of few rows
+ * over long tables splits their contexts, and a second one joins the parts: workspace is DEVICE
+ * memory, 16-byte aligned, of vfl_attention_4bit_workspace bytes for the call's sizes (0: none
+ * needed); calls that may overlap need one each.
+ */
+int vfl_reshape_and_cache_4bit(const void *key, const void *value, int64_t key_stride_token,
+                               int64_t key_stride_head, int64_t value_stride_token,
+                               int64_t value_stride_head, void *cache,
+                               const int64_t *slot_mapping, int64_t num_tokens, int num_heads,
+                               int head_dim, int block_size, int64_t num_blocks, int dtype,
+                               void *stream);
+int vfl_gather_cache_4bit(const void *cache, const int64_t *slot_mapping, void *key, void *value,
+                          int64_t key_stride_token, int64_t key_stride_head,
+                          int64_t value_stride_token, int64_t value_stride_head,
+                          int64_t num_tokens, int num_heads, int head_dim, int block_size,
+                          int64_t num_blocks, int dtype, void *stream);
+int64_t vfl_attention_4bit_workspace(int64_t num_rows, int64_t num_groups, int num_heads,
+                                     int head_dim, int block_size, int64_t max_blocks_per_seq);
+int vfl_attention_with_kv_cache_4bit(const void *query, int64_t query_stride_token,
+                                     int64_t query_stride_head, const void *cache, void *out,
+                                     const int32_t *seq_lens, const int32_t *block_table,
+                                     int64_t block_table_stride, int64_t max_blocks_per_seq,
+                                     const int32_t *group_start, const int32_t *group_order,
+                                     int64_t num_rows, int64_t num_groups, int max_group_size,
+                                     int num_heads, int head_dim, int block_size,
+                                     int64_t num_blocks, float scale, int dtype, void *workspace,
+                                     void *stream);
+
+/*
+ * Cross-attention of packed runs (scaled_dot_product_attention per sequence, queries and keys
+ * of different lengths; no vllm_cpu_attn counterpart):
+ *   out[r][h] = softmax(scale * query[r][h] key[:][h]^T) value[:][h]
+ * over the keys of r's sequence.  Sequence n has queries query_start_loc[n] ..
+ * query_start_loc[n + 1] - 1 and keys key_start_loc[n] .. key_start_loc[n + 1] - 1 (DEVICE int32
+ * [num_sequences + 1], rising; they are limited to the rows there are).  Rows of no sequence are
+ * neither read nor written; queries without keys get 0.  query [num_queries], key and value
+ * [num_keys] rows of num_heads x head_dim, any strides; out contiguous, query itself or apart from
+ * it, apart from key and value.  head_dim up to 256; scale finite.  Sums and softmax in fp32,
+ * the weights rounded to the type for the second product (fp32: kept to 2^-24).
+ * max_query_len and max_key_len, the longest runs expected, shape the launch (longer ones are
+ * served too).  workspace as above, of vfl_packed_cross_attention_workspace bytes.
+ */
+int64_t vfl_packed_cross_attention_workspace(int64_t num_queries, int64_t num_sequences,
+                                             int num_heads, int head_dim, int64_t max_query_len,
+                                             int64_t max_key_len, int dtype);
+int vfl_packed_cross_attention(const void *query, int64_t query_stride_token,
+                               int64_t query_stride_head, const void *key,
+                               int64_t key_stride_token, int64_t key_stride_head,
+                               const void *value, int64_t value_stride_token,
+                               int64_t value_stride_head, void *out,
+                               const int32_t *query_start_loc, const int32_t *key_start_loc,
+                               int64_t num_queries, int64_t num_keys, int64_t num_sequences,
+                               int num_heads, int head_dim, int64_t max_query_len,
+                               int64_t max_key_len, float scale, int dtype, void *workspace,
+                               void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ("kv_cache.hip", "paged_attention.hip", "attention_dims.hip", "attention_block32.hip",
            "decoder_ops.hip", "decode_linear.hip", "encoder_attention.hip", "kv_cache_8bit.hip",
-           "attention_8bit.hip", "token_logprobs.hip")
+           "attention_8bit.hip", "token_logprobs.hip", "kv_cache_4bit.hip", "attention_4bit.hip",
+           "cross_attention.hip", "cross_attention_f32.hip", "cross_attention_bf16.hip",
+           "cross_attention_f16.hip")
 OUTPUT = os.path.join(HERE, "libvflorence_amd.so")
 ARCH = os.environ.get("VFL_OFFLOAD_ARCH", "gfx950")
 

@@ -50,6 +50,12 @@ EXPORTED_SYMBOLS = (
     "vfl_attention_with_kv_cache_8bit",
     "vfl_token_logprobs_workspace",
     "vfl_token_logprobs",
+    "vfl_reshape_and_cache_4bit",
+    "vfl_gather_cache_4bit",
+    "vfl_attention_4bit_workspace",
+    "vfl_attention_with_kv_cache_4bit",
+    "vfl_packed_cross_attention_workspace",
+    "vfl_packed_cross_attention",
 )
 
 
@@ -170,6 +176,26 @@ _SIGNATURES = {
     "vfl_token_logprobs": (
         ctypes.c_int,
         [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "vfl_reshape_and_cache_4bit": (
+        ctypes.c_int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i32, _vp],
+    ),
+    "vfl_gather_cache_4bit": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i32, _vp],
+    ),
+    "vfl_attention_4bit_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i64]),
+    "vfl_attention_with_kv_cache_4bit": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _i32,
+         _i32, _i64, _f32, _i32, _vp, _vp],
+    ),
+    "vfl_packed_cross_attention_workspace": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64, _i32]),
+    "vfl_packed_cross_attention": (
+        ctypes.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32,
+         _i32, _i64, _i64, _f32, _i32, _vp, _vp],
     ),
 }
 

@@ -34,42 +34,9 @@
 #include <stdio.h>
 
 #include "e4m3.h"
+#include "split_softmax.h"
 
 namespace vfl {
-
-// bf16 terms of a query and of a weight
-template <int DT> struct Terms {
-  static constexpr int Q = DT == VFL_FLOAT32 ? 3 : DT == VFL_FLOAT16 ? 2 : 1;
-  static constexpr int P = DT == VFL_FLOAT32 ? 3 : 2;
-};
-
-using Bf16 = Mfma<VFL_BFLOAT16>;
-
-// bf16 terms of four floats, largest first; f is left with the remainder.  Queries are cut, weights
-// rounded: a cut term holds 8 bits and the next ones start behind it, so two hold all of fp16 and
-// three all of fp32 either way, and the largest fp32 values, which would round to infinity,
-// stay finite; of two or three terms that do not hold everything rounding leaves half as much.
-template <bool ROUND> __device__ __forceinline__ uint2 take_bf16(float (&f)[4]) {
-  uint2 w;
-  if constexpr (ROUND) {
-    w = make_uint2(Bf16::narrow2(f[0], f[1]), Bf16::narrow2(f[2], f[3]));
-  } else {
-    constexpr uint32_t HIGH_HALVES = 0x07060302u;
-    w = make_uint2(
-        __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), HIGH_HALVES),
-        __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), HIGH_HALVES));
-  }
-  f[0] -= Bf16::widen_lo(w.x), f[1] -= Bf16::widen_hi(w.x);
-  f[2] -= Bf16::widen_lo(w.y), f[3] -= Bf16::widen_hi(w.y);
-  return w;
-}
-
-template <int DT>
-__device__ __forceinline__ void store_result(typename Elem<DT>::T *p, float S, float o) {
-  const float y = S > 0.f ? o / S : S == S ? 0.f : S;  // NaN scores stay NaN
-  if constexpr (DT == VFL_FLOAT32) *p = y;
-  else *p = (uint16_t)Mfma<DT>::narrow(y);
-}
 
 __device__ __forceinline__ float lane_float(float x, int lane) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
@@ -159,35 +126,20 @@ __device__ __forceinline__ int clamp_scalar(int x) {
   return r;
 }
 
-// What is added to a softmax when its context is split: [row][head][split].  The sums come first
-// in the workspace: whole 64-byte pieces, 16-byte aligned for any number of parts.
-struct SplitOut {
-  float *acc;  // [D]
-  float2 *ml;
-};
-
-struct Attn8Args {
+struct Attn8Args : DecodeRows {
   const void *q;
   int64_t q_st, q_sh;
   const uint8_t *kc, *vc;
   const float *scales;
-  void *out;
   const int32_t *seq_lens, *bt;
   int64_t bt_stride;
   int width, room;  // entries of a table row (one at least), tokens it can list
-  const int32_t *group_start, *group_order;
-  int64_t num_rows, num_groups;
-  int H, D;
   int64_t num_blocks;
-  float scale_log2;  // its magnitude: the query takes the sign
   uint32_t q_sign;   // flips the sign of a word's elements
   bool q_vec;  // every 8 elements of a query are 16-byte aligned
-  int splits;
-  SplitOut part;
 };
 
-constexpr int ATTN8_COLS = 8;  // rows of a group
-constexpr float NO_SCORE = -3.402823466e38f;  // the least finite score
+constexpr int ATTN8_COLS = GROUP_ROWS;
 
 // Maximum across the four 16-lane rows, a NaN passed on.
 __device__ __forceinline__ float rows_maximum4(float x) {
@@ -197,22 +149,6 @@ __device__ __forceinline__ float rows_maximum4(float x) {
   const auto b =
       __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// Rows of the group at dispatch position `pos`, from row0 on (0: no such group).
-__device__ __forceinline__ int group_rows(const Attn8Args &a, int64_t pos, int64_t &row0) {
-  if (pos >= a.num_groups) return 0;
-  int64_t g = pos;
-  if (a.group_order) g = a.group_order[pos];
-  if (g < 0 || g >= a.num_groups) return 0;
-  row0 = g;
-  int n = 1;
-  if (a.group_start) {
-    row0 = a.group_start[g];
-    n = a.group_start[g + 1] - (int)row0;
-  }
-  if (row0 < 0 || row0 >= a.num_rows) return 0;
-  return (int)min((int64_t)min(n, ATTN8_COLS), a.num_rows - row0);
 }
 
 // NS: ceil(D / 64).  PARTS: 16-token parts of a block.  NW waves split a context, and
@@ -470,53 +406,6 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
   }
 }
 
-// The splits of a (row, head) joined: a quarter of D threads, a team, take 4 dims each of
-// every teams-th split, about a maximum of their own, so that maxima and sums come in one round
-// trip; the teams meet in LDS.
-constexpr int ATTN8_JOIN_NT = 256;
-template <int DT>
-__global__ __launch_bounds__(ATTN8_JOIN_NT) void attention_8bit_join_kernel(Attn8Args a) {
-  using T = typename Elem<DT>::T;
-  __shared__ float4 s_o[ATTN8_JOIN_NT];
-  __shared__ float2 s_ml[ATTN8_JOIN_NT];
-  int64_t row0;
-  if ((int)blockIdx.y >= group_rows(a, blockIdx.x / a.H, row0)) return;
-  const int64_t at = (row0 + blockIdx.y) * a.H + blockIdx.x % a.H;
-  const int tid = threadIdx.x, quads = a.D / 4, teams = ATTN8_JOIN_NT / quads;
-  const int team = tid / quads, quad = tid % quads;
-  const float2 *ml = a.part.ml + at * a.splits;
-  const float4 *acc = reinterpret_cast<const float4 *>(a.part.acc + at * a.splits * a.D) + quad;
-  float M = NO_SCORE, S = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (team < teams) {
-#pragma unroll 4
-    for (int s = team; s < a.splits; s += teams) {
-      const float2 x = ml[s];
-      const float4 v = acc[(int64_t)s * quads];
-      const float to = fmaxf(M, x.x);
-      const float f = fast_exp2((M - to) * a.scale_log2), e = fast_exp2((x.x - to) * a.scale_log2);
-      S = S * f + x.y * e;
-      o.x = o.x * f + v.x * e, o.y = o.y * f + v.y * e;
-      o.z = o.z * f + v.z * e, o.w = o.w * f + v.w * e;
-      M = to;
-    }
-  }
-  s_o[tid] = o;
-  s_ml[tid] = make_float2(M, S);
-  __syncthreads();
-  for (int d = tid; d < a.D; d += ATTN8_JOIN_NT) {
-    float top = NO_SCORE, sum = 0.f, y = 0.f;
-    for (int t = 0; t < teams; ++t) top = fmaxf(top, s_ml[t * quads + d / 4].x);
-    for (int t = 0; t < teams; ++t) {
-      const float2 x = s_ml[t * quads + d / 4];
-      const float e = fast_exp2((x.x - top) * a.scale_log2);
-      sum = fmaf(x.y, e, sum);
-      y = fmaf((&s_o[t * quads + d / 4].x)[d % 4], e, y);
-    }
-    store_result<DT>((T *)a.out + at * a.D + d, sum, y);
-  }
-}
-
 // Waves of a workgroup and workgroups of a context.  A workgroup a CU or fewer takes eight waves
 // (eight against four, us: 12 of 590 tokens 5.6 / 6.4, 256 of 256 to 1024, fp32, 8.6 / 9.5; 384
 // of 100 to 1000 9.4 / 9.0, 1024 of 256 to 1024 19.9 / 18.5); wide heads, whose waves hold more
@@ -566,18 +455,13 @@ static int launch_attention_8bit_steps(const Attn8Args &a, int waves, hipStream_
   }
   int st = launch_status("attention_with_kv_cache_8bit");
   if (st != VFL_OK || a.splits == 1) return st;
-  const unsigned rows = a.group_start ? ATTN8_COLS : 1;
-  attention_8bit_join_kernel<DT>
-      <<<dim3((unsigned)(a.num_groups * a.H), rows), dim3(ATTN8_JOIN_NT), 0, stream>>>(a);
+  launch_join_rows<DT>(a, stream);
   return launch_status("attention_with_kv_cache_8bit");
 }
 
 }  // namespace vfl
 
 using namespace vfl;
-
-// Bytes a (row, head) of one split takes in the workspace.
-static int64_t attn8_part_bytes(int head_dim) { return head_dim * 4 + 8; }
 
 extern "C" int64_t vfl_attention_8bit_workspace(int64_t num_rows, int64_t num_groups,
                                                 int num_heads, int head_dim, int block_size,
@@ -587,7 +471,7 @@ extern "C" int64_t vfl_attention_8bit_workspace(int64_t num_rows, int64_t num_gr
     return 0;
   const Attn8Plan p =
       attn8_plan(num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
-  return p.splits > 1 ? num_rows * num_heads * p.splits * attn8_part_bytes(head_dim) : 0;
+  return p.splits > 1 ? num_rows * num_heads * p.splits * split_part_bytes(head_dim) : 0;
 }
 
 extern "C" int vfl_attention_with_kv_cache_8bit(
@@ -630,17 +514,21 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
   }
   // an empty pool holds nothing: every row is zero
   const int64_t table = num_blocks ? max_blocks_per_seq : 0;
-  Attn8Args a{query, query_stride_token, query_stride_head, (const uint8_t *)k_cache,
-              (const uint8_t *)v_cache, kv_scales, out, seq_lens, block_table,
-              block_table_stride, (int)table, (int)table * block_size, group_start, group_order,
-              num_rows, num_groups, num_heads, head_dim, num_blocks,
-              // finite and not 0, which would make NaN of an equal or a masked score (the least
-              // denormal in its place moves no weight by more than 2^-21)
-              fminf(fmaxf(fabsf(scale) * 1.4426950408889634f, __FLT_DENORM_MIN__), -NO_SCORE),
-              !(scale < 0.f) ? 0u : dtype == VFL_FLOAT32 ? 0x80000000u : 0x80008000u,
-              (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
-                  query_stride_head % (16 / eb) == 0,
-              1, {nullptr, nullptr}};
+  Attn8Args a;
+  a.out = out;
+  a.group_start = group_start, a.group_order = group_order;
+  a.num_rows = num_rows, a.num_groups = num_groups;
+  a.H = num_heads, a.D = head_dim;
+  a.scale_log2 = decode_scale_log2(scale);
+  a.splits = 1, a.part = {nullptr, nullptr};
+  a.q = query, a.q_st = query_stride_token, a.q_sh = query_stride_head;
+  a.kc = (const uint8_t *)k_cache, a.vc = (const uint8_t *)v_cache, a.scales = kv_scales;
+  a.seq_lens = seq_lens, a.bt = block_table, a.bt_stride = block_table_stride;
+  a.width = (int)table, a.room = (int)table * block_size;
+  a.num_blocks = num_blocks;
+  a.q_sign = !(scale < 0.f) ? 0u : dtype == VFL_FLOAT32 ? 0x80000000u : 0x80008000u;
+  a.q_vec = (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
+            query_stride_head % (16 / eb) == 0;
   if (table == 0) a.bt = seq_lens, a.bt_stride = 0, a.width = 1;  // read, and not used
   const Attn8Plan plan = attn8_plan(num_groups, num_heads, head_dim, table * block_size);
   if (plan.splits > 1) {

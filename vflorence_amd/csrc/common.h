@@ -63,6 +63,9 @@ __device__ __forceinline__ void xcd_position(unsigned id, unsigned H, int64_t &p
   pos = (int64_t)XCDS * (j / H) + id % XCDS;
 }
 
+// Whether a launch stays below the runtime's 2^32 threads a dimension.
+inline bool grid_fits(int64_t groups, int threads) { return groups * threads < (1LL << 32); }
+
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 

@@ -1,0 +1,7 @@
+// Packed cross-attention of fp32 operands (a file a type: they compile side by side).
+#define VFL_CROSS_KERNEL
+#include "cross_attention.h"
+
+int vfl::launch_cross_f32(const CrossArgs &a, int ks, hipStream_t stream) {
+  return launch_cross<VFL_FLOAT32>(a, ks, stream);
+}

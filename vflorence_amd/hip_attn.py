@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import operator
 from dataclasses import dataclass, field
 
@@ -905,6 +906,52 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
     torch.autograd.graph.increment_version((k_cache, v_cache, kv_scales))
 
 
+def _check_paged_rows(query: torch.Tensor, out: torch.Tensor, seq_lens: torch.Tensor,
+                      block_table: torch.Tensor, *caches: torch.Tensor):
+    """Checks what a decode attention takes beside its caches; ``(block_table, seq_lens)`` as the
+    kernels read them."""
+    num_rows = query.shape[0]
+    if out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of query's shape and dtype")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (num_rows,):
+        raise ValueError(f"seq_lens must be int32 [{num_rows}], got {seq_lens.dtype} "
+                         f"{tuple(seq_lens.shape)}")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2
+            or block_table.shape[0] != num_rows):
+        raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
+                         f"{block_table.dtype} {tuple(block_table.shape)}")
+    one_gpu(query, *caches, out, seq_lens, block_table)
+    width = block_table.shape[1]
+    if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
+                                                      and num_rows > 1):
+        block_table = block_table.contiguous()
+    return block_table, seq_lens.contiguous()
+
+
+def _shared_groups(sm: SchedulerMetadata | None, query: torch.Tensor, block_size: int):
+    """``(group_start, group_order, groups, rows of a group at most)`` of the row groups that
+    share a table; every row its own group where they do not."""
+    num_rows, num_heads, head_dim = query.shape
+    if sm is None:
+        return None, None, num_rows, 1
+    if (sm.num_heads, sm.head_dim, sm.block_size) != (num_heads, head_dim, block_size):
+        raise ValueError("scheduler_metadata was made for another cache: "
+                         f"H={sm.num_heads}, D={sm.head_dim}, block_size={sm.block_size}")
+    if sm.group_plan is not None and sm.group_plan.folded:
+        raise ValueError("a group plan with copy-on-write folded in is for "
+                         "self_attention_with_kv_write alone")
+    if sm.own_tables and sm.group_start is not None:
+        return None, None, num_rows, 1
+    start, order = sm.group_start, sm.group_order
+    if start is not None:
+        one_gpu(query, start)
+        start = start.contiguous()
+    if order is not None:
+        one_gpu(query, order)
+        order = order.contiguous()
+    return start, order, sm.num_groups, sm.max_group_size
+
+
 @functools.lru_cache(maxsize=4096)
 def _attention_8bit_workspace(*sizes: int) -> int:
     return lib.vfl_attention_8bit_workspace(*sizes)
@@ -931,42 +978,13 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                          f"dimension, got {tuple(query.shape)}")
     num_rows = query.shape[0]
     dtype = _dtype_code(query.dtype)
-    if out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
-        raise ValueError("out must be a contiguous tensor of query's shape and dtype")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (num_rows,):
-        raise ValueError(f"seq_lens must be int32 [{num_rows}], got {seq_lens.dtype} "
-                         f"{tuple(seq_lens.shape)}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2
-            or block_table.shape[0] != num_rows):
-        raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
-                         f"{block_table.dtype} {tuple(block_table.shape)}")
-    index = one_gpu(query, k_cache, v_cache, kv_scales, out, seq_lens, block_table)
+    block_table, seq_lens = _check_paged_rows(query, out, seq_lens, block_table, k_cache, v_cache,
+                                              kv_scales)
     if (query.requires_grad or out.requires_grad or k_cache.requires_grad
             or v_cache.requires_grad or kv_scales.requires_grad):
         refuse_gradients("attention_with_kv_cache_8bit")
-    width = block_table.shape[1]
-    if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
-                                                      and num_rows > 1):
-        block_table = block_table.contiguous()
-    seq_lens = seq_lens.contiguous()
-    start = order = None
-    num_groups = num_rows
-    sm = scheduler_metadata
-    if sm is not None:
-        if (sm.num_heads, sm.head_dim, sm.block_size) != (num_heads, head_dim, block_size):
-            raise ValueError("scheduler_metadata was made for another cache: "
-                             f"H={sm.num_heads}, D={sm.head_dim}, block_size={sm.block_size}")
-        if sm.group_plan is not None and sm.group_plan.folded:
-            raise ValueError("a group plan with copy-on-write folded in is for "
-                             "self_attention_with_kv_write alone")
-        if not sm.own_tables or sm.group_start is None:
-            start, order, num_groups = sm.group_start, sm.group_order, sm.num_groups
-        if start is not None:
-            one_gpu(query, start)
-            start = start.contiguous()
-        if order is not None:
-            one_gpu(query, order)
-            order = order.contiguous()
+    index, width = query.get_device(), block_table.shape[1]
+    start, order, num_groups, _ = _shared_groups(scheduler_metadata, query, block_size)
     need = _attention_8bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     on_device(index, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
@@ -977,6 +995,246 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
               None if order is None else order.data_ptr(), num_rows, num_groups, num_heads,
               head_dim, block_size, num_blocks, float(scale), dtype,
               workspace.data_ptr() if need else None)
+    torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
+
+
+# ---------------------------------------------------------------------------
+# caches held in 4 bits
+# ---------------------------------------------------------------------------
+CACHE_4BIT_GROUP = 32  # dims that share a scale
+
+
+def _bytes_per_token_4bit(head_dim: int) -> int:
+    """Bytes of a token and head in a 4-bit cache: K's and V's codes and scales."""
+    return 34 * -(-head_dim // CACHE_4BIT_GROUP)
+
+
+def kv_cache_4bit(num_blocks: int, num_heads: int, block_size: int, head_dim: int,
+                  device) -> torch.Tensor:
+    """A zero-filled paged cache in 4 bits, K and V in one pool: ``torch.uint8`` ``[num_blocks, H,
+    block_size, 34 * ceil(D / 32)]``.  A value is an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4 or 6 and
+    a sign) times the scale of its token, head and 32 dims, a power of two.  The order of the
+    bytes inside a block is the library's (``kv_cache_4bit_values`` gives the values);
+    ``copy_blocks([cache], ...)`` copies blocks whole."""
+    if head_dim not in SUPPORTED_HEAD_DIMS or block_size not in SUPPORTED_BLOCK_SIZES:
+        raise ValueError(f"no gfx950 kernel for block_size={block_size} head_dim={head_dim}; "
+                         f"supported head_dim {sorted(SUPPORTED_HEAD_DIMS)}, block_size "
+                         f"{sorted(SUPPORTED_BLOCK_SIZES)}")
+    return torch.zeros(num_blocks, num_heads, block_size, _bytes_per_token_4bit(head_dim),
+                       dtype=torch.uint8, device=device)
+
+
+def kv_cache_4bit_values(cache: torch.Tensor,
+                         head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The float32 keys and values that a 4-bit cache stands for, ``[num_blocks, H, block_size,
+    D]`` in token order."""
+    num_blocks, heads, block_size, _ = _check_4bit_cache(cache, head_dim)
+    groups, parts = -(-head_dim // CACHE_4BIT_GROUP), block_size // 16
+    flat, size = cache.view(num_blocks, -1), heads * parts * groups * 256
+    shape = (num_blocks, heads, parts, groups, 16, 16)
+    keys = flat[:, :size].view(shape)  # tokens, then bytes of two dims side by side
+    values = flat[:, size:2 * size].view(shape).transpose(-1, -2)  # dims 16 apart, token last
+    scales = flat[:, 2 * size:].view(num_blocks, heads, parts, 4, 2, groups, 4)
+    scales = scales.permute(4, 0, 1, 2, 5, 3, 6).reshape(2, *shape[:-1]).int()
+    steps = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=cache.device)
+    look = torch.cat([steps, -steps])
+    found = []
+    for codes, e in ((torch.stack([keys & 15, keys >> 4], dim=-1).flatten(-2), scales[0]),
+                     (torch.cat([values & 15, values >> 4], dim=-1), scales[1])):
+        scale = (e << 23).view(torch.float32).masked_fill(e == 255, math.nan)
+        x = (look[codes.int()] * scale[..., None]).transpose(3, 4)  # tokens before groups
+        found.append(x.reshape(num_blocks, heads, block_size, groups * 32)[..., :head_dim])
+    return found[0], found[1]
+
+
+def _check_4bit_cache(cache: torch.Tensor, head_dim: int):
+    if cache.dim() != 4 or cache.dtype != torch.uint8 or not cache.is_contiguous():
+        raise ValueError("a 4-bit cache is a contiguous torch.uint8 tensor [num_blocks, H, "
+                         f"block_size, bytes], got {cache.dtype} {tuple(cache.shape)}")
+    shape = cache.shape
+    if shape[2] not in SUPPORTED_BLOCK_SIZES or head_dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"block_size={shape[2]}, head_dim={head_dim} has no attention kernel; "
+                         f"supported: {sorted(SUPPORTED_BLOCK_SIZES)}, "
+                         f"{sorted(SUPPORTED_HEAD_DIMS)}")
+    if shape[3] != _bytes_per_token_4bit(head_dim):
+        raise ValueError(f"a 4-bit cache of head_dim={head_dim} has "
+                         f"{_bytes_per_token_4bit(head_dim)} bytes a token, this one {shape[3]}")
+    return shape
+
+
+def _check_4bit_rows(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
+                     slot_mapping: torch.Tensor):
+    """The sizes, dtype code and device index of keys and values beside a 4-bit cache."""
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError(f"key/value must be [T, H, D] of one shape, got {tuple(key.shape)}, "
+                         f"{tuple(value.shape)}")
+    num_blocks, num_heads, block_size, _ = _check_4bit_cache(cache, key.shape[2])
+    if key.shape[1] != num_heads:
+        raise ValueError(f"key/value have {key.shape[1]} heads, the cache {num_heads}")
+    if key.dtype != value.dtype:
+        raise ValueError("key and value must share one dtype")
+    dtype = _dtype_code(key.dtype)
+    if key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("key/value need a contiguous last dimension")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],):
+        raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
+                         f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
+    return num_blocks, num_heads, block_size, dtype, one_gpu(key, value, cache, slot_mapping)
+
+
+def reshape_and_cache_4bit(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
+                           slot_mapping: torch.Tensor) -> None:
+    """``reshape_and_cache`` into a 4-bit cache (``kv_cache_4bit``), in place.
+
+    key/value: [T, H, D] in float32, bfloat16 or float16, any token and head strides, a
+    contiguous last dimension.  slot_mapping: int64 [T]; a token whose slot is negative or past
+    the pool is skipped, and the other slots must differ from one another.  What other slots
+    hold is left as it was.
+
+    Each 32 dims of a token's head have a scale of their own, the smallest power of two that
+    brings their largest magnitude to 6 or less, so every value is rounded once, to nearest, and
+    a later token changes no earlier one.  Dims that share a scale with an infinity or a NaN
+    are held as NaN."""
+    num_blocks, num_heads, block_size, dtype, index = _check_4bit_rows(key, value, cache,
+                                                                       slot_mapping)
+    if key.requires_grad or value.requires_grad:
+        refuse_gradients("reshape_and_cache_4bit")
+    slot_mapping = slot_mapping.contiguous()
+    on_device(index, lib.vfl_reshape_and_cache_4bit, key.data_ptr(), value.data_ptr(),
+              key.stride(0), key.stride(1), value.stride(0), value.stride(1), cache.data_ptr(),
+              slot_mapping.data_ptr(), key.shape[0], num_heads, key.shape[2], block_size,
+              num_blocks, dtype)
+    torch.autograd.graph.increment_version((cache,))  # autograd's check of saved tensors
+
+
+def gather_cache_4bit(cache: torch.Tensor, slot_mapping: torch.Tensor, key: torch.Tensor,
+                      value: torch.Tensor) -> None:
+    """The way back from ``reshape_and_cache_4bit``: ``key[t]`` and ``value[t]`` ([T, H, D] in
+    float32, bfloat16 or float16, any strides that give every element a place of its own, a
+    contiguous last dimension) become what ``cache`` holds at ``slot_mapping[t]`` (int64 [T], in
+    any order), and 0 for a slot that is negative or past the pool."""
+    num_blocks, num_heads, block_size, dtype, index = _check_4bit_rows(key, value, cache,
+                                                                       slot_mapping)
+    for t in (key, value):
+        if any(step == 0 and size > 1 for step, size in zip(t.stride(), t.shape)):
+            raise ValueError("key and value are written: expanded tensors do not do")
+    if key.requires_grad or value.requires_grad:
+        refuse_gradients("gather_cache_4bit")
+    slot_mapping = slot_mapping.contiguous()
+    on_device(index, lib.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(),
+              key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0),
+              value.stride(1), key.shape[0], num_heads, key.shape[2], block_size, num_blocks,
+              dtype)
+    torch.autograd.graph.increment_version((key, value))  # autograd's check of saved tensors
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_4bit_workspace(*sizes: int) -> int:
+    return lib.vfl_attention_4bit_workspace(*sizes)
+
+
+def attention_with_kv_cache_4bit(query: torch.Tensor, cache: torch.Tensor, out: torch.Tensor,
+                                 seq_lens: torch.Tensor, *, scale: float,
+                                 block_table: torch.Tensor,
+                                 scheduler_metadata: SchedulerMetadata | None = None) -> None:
+    """``attention_with_kv_cache`` over a 4-bit cache (``kv_cache_4bit``), into ``out``.
+
+    query: [N, H, D] in float32, bfloat16 or float16, any token and head strides; out: a
+    contiguous tensor of its shape and dtype, ``query`` itself or apart from it.  Row r attends
+    to the first ``seq_lens[r]`` tokens (int32, as many as the table lists at most) of the
+    blocks that ``block_table[r]`` (int32 [N, max_blocks]) lists; a block id outside the pool
+    contributes nothing, and a row without tokens is zero.  Of ``scheduler_metadata`` the row
+    groups (``group_start``, ``group_order``, ``max_group_size``) are used: a group that shares
+    its table (and length) is read once for all of its rows, one whose rows keep their own
+    tables runs row by row."""
+    if query.dim() != 3 or query.stride(2) != 1:
+        raise ValueError("query must be [N, H, D] with a contiguous last dimension, got "
+                         f"{tuple(query.shape)}")
+    num_rows, num_heads, head_dim = query.shape
+    num_blocks, cache_heads, block_size, _ = _check_4bit_cache(cache, head_dim)
+    if cache_heads != num_heads:
+        raise ValueError(f"query has {num_heads} heads, the cache {cache_heads}")
+    dtype = _dtype_code(query.dtype)
+    block_table, seq_lens = _check_paged_rows(query, out, seq_lens, block_table, cache)
+    if query.requires_grad or out.requires_grad:
+        refuse_gradients("attention_with_kv_cache_4bit")
+    index, width = query.get_device(), block_table.shape[1]
+    start, order, num_groups, most = _shared_groups(scheduler_metadata, query, block_size)
+    need = _attention_4bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    on_device(index, lib.vfl_attention_with_kv_cache_4bit, query.data_ptr(), query.stride(0),
+              query.stride(1), cache.data_ptr(), out.data_ptr(), seq_lens.data_ptr(),
+              block_table.data_ptr(), block_table.stride(0) if num_rows > 1 else width, width,
+              None if start is None else start.data_ptr(),
+              None if order is None else order.data_ptr(), num_rows, num_groups, most, num_heads,
+              head_dim, block_size, num_blocks, float(scale), dtype,
+              workspace.data_ptr() if need else None)
+    torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
+
+
+# ---------------------------------------------------------------------------
+# cross-attention of packed runs
+# ---------------------------------------------------------------------------
+CROSS_HEAD_DIMS = frozenset(d for d in SUPPORTED_HEAD_DIMS if d <= 256)
+
+
+@functools.lru_cache(maxsize=4096)
+def _cross_workspace(*sizes: int) -> int:
+    return lib.vfl_packed_cross_attention_workspace(*sizes)
+
+
+def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                           out: torch.Tensor, query_start_loc: torch.Tensor,
+                           key_start_loc: torch.Tensor, *, scale: float, max_query_len: int,
+                           max_key_len: int) -> None:
+    """Attention of packed sequences of queries, each over keys and values of its own and of
+    another length: a decoder's prompt or a given text over its encoder states.
+
+    query: [T, H, D], key and value: [S, H, D], all float32, bfloat16 or float16, any token and
+    head strides, a contiguous last dimension, head sizes up to 256.  Sequence n has queries
+    ``query_start_loc[n]`` to ``query_start_loc[n + 1] - 1`` and keys ``key_start_loc[n]`` to
+    ``key_start_loc[n + 1] - 1`` (int32 [sequences + 1], rising, on the GPU).  Of ``out``, a
+    contiguous tensor of query's shape and dtype, ``query`` itself or apart from it, the rows of
+    the sequences are written, 0 where one has no keys; rows of none are left as they were.
+    ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch and
+    change no result."""
+    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape \
+            or query.shape[1:] != key.shape[1:]:
+        raise ValueError("query must be [T, H, D], key and value [S, H, D], got "
+                         f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
+    num_queries, num_heads, head_dim = query.shape
+    if head_dim not in CROSS_HEAD_DIMS:
+        raise ValueError(f"head_dim {head_dim} has no kernel; supported: "
+                         f"{sorted(CROSS_HEAD_DIMS)}")
+    if not query.dtype == key.dtype == value.dtype == out.dtype:
+        raise ValueError("query, key, value and out must share one dtype")
+    dtype = _dtype_code(query.dtype)
+    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
+        raise ValueError("query, key and value need a contiguous last dimension")
+    if out.shape != query.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of query's shape")
+    if (query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1
+            or query_start_loc.numel() < 1 or key_start_loc.dtype != torch.int32
+            or key_start_loc.shape != query_start_loc.shape):
+        raise ValueError("query_start_loc and key_start_loc must be int32 [sequences + 1], got "
+                         f"{query_start_loc.dtype} {tuple(query_start_loc.shape)}, "
+                         f"{key_start_loc.dtype} {tuple(key_start_loc.shape)}")
+    max_query_len, max_key_len = operator.index(max_query_len), operator.index(max_key_len)
+    if max_query_len < 0 or max_key_len < 0:
+        raise ValueError(f"longest runs of {max_query_len} queries and {max_key_len} keys")
+    index = one_gpu(query, key, value, out, query_start_loc, key_start_loc)
+    if (query.requires_grad or key.requires_grad or value.requires_grad or out.requires_grad):
+        refuse_gradients("packed_cross_attention")
+    query_start_loc, key_start_loc = query_start_loc.contiguous(), key_start_loc.contiguous()
+    sequences = query_start_loc.numel() - 1
+    longest = (min(max_query_len, num_queries), min(max_key_len, key.shape[0]))
+    need = _cross_workspace(num_queries, sequences, num_heads, head_dim, *longest, dtype)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    on_device(index, lib.vfl_packed_cross_attention, query.data_ptr(), query.stride(0),
+              query.stride(1), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
+              value.stride(0), value.stride(1), out.data_ptr(), query_start_loc.data_ptr(),
+              key_start_loc.data_ptr(), num_queries, key.shape[0], sequences, num_heads, head_dim,
+              *longest, float(scale), dtype, workspace.data_ptr() if need else None)
     torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
 
 
