@@ -8,8 +8,8 @@
 // them (half-wave hf of step s holds keys 16 s + 4 hf + 0..3 and 16 s + 8 + 4 hf + 0..3).  V lies
 // in LDS as it came, key by key, and is turned by the transposing reads.
 //
-// 16-bit inputs go in as they are, the weights rounded to that type (fp16's times 2^14, which keeps
-// those down to 2^-28 of the largest clear of its subnormals; the others' times 2^-20).  fp32 goes in as three bf16 terms
+// 16-bit inputs go in as they are, the weights rounded to that type (fp16's times 2^7, which keeps
+// those down to 2^-21 of the reference clear of its subnormals; the others' times 2^-20).  fp32 goes in as three bf16 terms
 // each, rounded, of whose nine products the six largest are taken: the others are 2^-26 of the whole
 // or less.
 #pragma once
@@ -30,21 +30,32 @@ struct CrossArgs {
   const int32_t *q_start, *k_start;  // [sequences + 1]
   int64_t num_queries, num_keys;     // rows of q and out, of k and v
   int sequences, H, D;
-  int tiles;         // query tiles of a sequence in the launch (more run in turn)
   float scale_log2;  // its magnitude: the query takes the sign
   bool negative;
-  bool vec;          // every 8 elements of q, k and v are 16-byte aligned
+  bool spread;       // workgroups go to any XCD
   bool out_vec;      // every 4 elements of out are aligned
   int splits;
   SplitOut part;
 };
 
+constexpr int CROSS_MAX_STRIDE = 1 << 22;  // elements between keys
+
 int launch_cross_f32(const CrossArgs &a, int ks, hipStream_t stream);
 int launch_cross_bf16(const CrossArgs &a, int ks, hipStream_t stream);
 int launch_cross_f16(const CrossArgs &a, int ks, hipStream_t stream);
 
-// Key groups that a launch may take (their tiles have to fit the LDS).
-inline int cross_most_groups(bool f32, int DG) { return !f32 || DG <= 2 ? 4 : DG <= 4 ? 2 : 1; }
+// Key groups that a launch may take (their tiles have to fit the LDS, and what the tiles' rows take
+// on their way the registers).
+constexpr int cross_most_groups(bool f32, int DG) {
+  return f32 ? (DG <= 2 ? 4 : DG <= 4 ? 2 : 1) : (DG <= 4 ? 4 : 2);
+}
+
+// Workgroups of a launch.
+inline int64_t cross_grid(int64_t num_queries, int64_t sequences, int H, int ks, int splits,
+                          bool spread) {
+  const int64_t places = num_queries / (128 / ks) + sequences;
+  return places * (spread ? H : (H + XCDS - 1) / XCDS * XCDS) * splits;
+}
 
 #ifdef VFL_CROSS_KERNEL
 namespace {
@@ -82,6 +93,22 @@ __device__ __forceinline__ void half_pair(float x, float &a, float &b) {
   b = __uint_as_float(s[1]);
 }
 
+// Two weights rounded to nearest even and packed, and the sum of a pair and c.
+template <int DT> __device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (DT == VFL_FLOAT16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{a, b}, f16x2_t));
+  else
+    return Bf16::narrow2(a, b);
+}
+template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float c) {
+  if constexpr (DT == VFL_FLOAT16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w),
+                                  __builtin_bit_cast(f16x2_t, 0x3c003c00u), c, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
+                                           __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
+}
+
 // Of 16 lanes, lane 4 i + c points to 4 elements of row i; lane n gets the four rows' element n
 // of the 16 that the lanes point to.
 __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
@@ -91,6 +118,7 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
 }
 
 // Shape of a launch: heads of up to 32 DG dims, KS key groups of 4 / KS waves.
+constexpr int WAVES = 4;
 template <int DT, int DG, int KS> struct CrossShape {
   static constexpr bool F32 = DT == VFL_FLOAT32;
   static constexpr int PLANES = F32 ? 3 : 1;   // bf16 terms
@@ -99,49 +127,90 @@ template <int DT, int DG, int KS> struct CrossShape {
   static constexpr int PLANE = KT * STRIDE;
   static constexpr int TILE = 2 * PLANES * PLANE;  // K, then V
   static constexpr int BUFS = 2 * KS * TILE <= 160 * 1024 ? 2 : 1;
-  static constexpr int GW = 4 / KS;            // waves of a key group
+  static constexpr int NW = WAVES;
+  static constexpr int GW = NW / KS;           // waves of a key group
   static constexpr int QT = 32 * GW;           // queries of a workgroup
   static constexpr int GT = 64 * GW;           // threads of a key group
   static constexpr int PIECES = KT * DG * 4;   // of 8 elements, of K or V
   static constexpr int CH = (PIECES + GT - 1) / GT;  // a thread's
+  static constexpr int OCC = !F32 && DG <= 2 && KS == 1 ? 3 : 1;  // waves of a SIMD at least
   static_assert(BUFS * KS * TILE <= 160 * 1024, "the tiles fit the LDS");
 };
 
+// A tile of queries: from `first` on of sequence n's nq (nq: none), which begin at row qa
+// and see the nk keys from row ka on.
+struct Tile {
+  int n, first, nq, nk;
+  int64_t qa, ka;
+};
+
+// Sequence n's tiles take the launch's places from floor(its first row / QT) + n on, as many as
+// there are to the next one's: never fewer than its queries fill, and no more than one to a
+// sequence beyond the rows' own.  A wave looks 64 sequences up at a time.
+template <int QT> __device__ __forceinline__ Tile find_tile(const CrossArgs &a, int place) {
+  const int lane = __lane_id();
+  const int rows = (int)a.num_queries, keys = (int)a.num_keys;
+  int lo = 0, span = a.sequences;
+  while (span > 63) {
+    const int step = (span + 63) / 64, n = lo + lane * step;
+    const bool in = lane * step < span;
+    const int q = min(max(a.q_start[in ? n : lo], 0), rows);
+    const uint64_t below = __builtin_amdgcn_ballot_w64(in && q / QT + n <= place);
+    const int i = max((int)__builtin_popcountll(below) - 1, 0);
+    lo += i * step;
+    span = min(step, span - i * step);
+  }
+  const int n = min(lo + lane, a.sequences);
+  const int q = min(max(a.q_start[n], 0), rows), k = min(max(a.k_start[n], 0), keys);
+  const uint64_t below = __builtin_amdgcn_ballot_w64(lane < span && q / QT + n <= place);
+  const int i = max((int)__builtin_popcountll(below) - 1, 0);  // (span is 63 at most)
+  const int qa = __builtin_amdgcn_readlane(q, i), qb = __builtin_amdgcn_readlane(q, i + 1);
+  const int ka = __builtin_amdgcn_readlane(k, i), kb = __builtin_amdgcn_readlane(k, i + 1);
+  const int nq = max(qb - qa, 0);
+  const int64_t first = (int64_t)(place - (qa / QT + lo + i)) * QT;
+  return Tile{lo + i, first < 0 || first >= nq ? nq : (int)first, nq, max(kb - ka, 0), qa, ka};
+}
+
 template <int DT, int DG, int KS>
-__global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
+__global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cross_attention_kernel(
+    CrossArgs a) {
   using S = CrossShape<DT, DG, KS>;
   using T = typename Elem<DT>::T;
   constexpr int PLANES = S::PLANES, KT = S::KT, STRIDE = S::STRIDE, GW = S::GW, GT = S::GT;
   constexpr int CH = S::CH, BUFS = S::BUFS, QT = S::QT;
-  constexpr int KB = KT / 32;                        // 32-key blocks of a tile
+  constexpr int KB = KT / 32;                        // 32 keys' worth of a tile
   constexpr int RAW = S::F32 ? 2 : 1;                // 16-byte words of 8 elements
   constexpr int MDT = S::F32 ? VFL_BFLOAT16 : DT;    // the products' type
   constexpr int PART = 16 * DG + 2;                  // a lane's partial result
-  // of a row's largest weight: fp16's small weights stay normal numbers; sums of up to 2^20 of the
-  // other types' largest values stay finite
-  constexpr float WEIGHT_LOG2 = DT == VFL_FLOAT16 ? 14.f : -20.f;
+  // of the weight of a row's reference: fp16's small weights stay normal numbers, those that pass
+  // the reference by the slack finite; sums of up to 2^12 of the other types' largest values stay
+  // finite
+  constexpr float WEIGHT_LOG2 = DT == VFL_FLOAT16 ? 15.f - RESCALE_SLACK_LOG2 : -20.f;
+  // a lane's sum at which a reference moves (a weight that fp16 does not hold is infinite)
+  constexpr float MOST_SUM = DT == VFL_FLOAT16 ? 0x1p15f : 0x1p-12f;
+  static_assert(RESCALE_SLACK_LOG2 == 8.f, "MOST_SUM is 2^(WEIGHT_LOG2 + slack)");
   __shared__ __align__(16) uint8_t s_tile[BUFS * KS * S::TILE];
   static_assert((KS - 1) * GW * 64 * PART * 4 <= (int)sizeof(s_tile),
                 "the partial outputs fit the tile buffers");
 
   // A (sequence, head)'s query tiles run on one XCD, which then reads its K/V once: ids go to XCDs
-  // round robin, so they are laid out as 8 pairs x tiles x splits.
-  const int per = a.tiles * a.splits;
-  const int64_t u = blockIdx.x;
-  const int64_t pair = 8 * (u / 8 / per) + u % 8;
-  if (pair >= (int64_t)a.sequences * a.H) return;
-  const int within = (int)(u / 8 % per);
-  const int split = within % a.splits;
-  const int n = (int)(pair / a.H), h = (int)(pair % a.H);
-  const int D = a.D;
-  const int64_t qa = min(max((int64_t)a.q_start[n], (int64_t)0), a.num_queries);
-  const int nq = (int)(min(max((int64_t)a.q_start[n + 1], qa), a.num_queries) - qa);
-  const int64_t ka = min(max((int64_t)a.k_start[n], (int64_t)0), a.num_keys);
-  const int nk = (int)(min(max((int64_t)a.k_start[n + 1], ka), a.num_keys) - ka);
+  // round robin, and XCD x takes the heads h of sequence n with (n H + h) % 8 = x.  A launch that
+  // the card holds at once goes anywhere: its heads may not fill the XCDs evenly.
+  const int lane = threadIdx.x & 63;
+  const unsigned ways = a.spread ? 1 : XCDS;
+  const unsigned heads = (a.H + ways - 1) / ways;
+  const unsigned item = blockIdx.x / ways;
+  const int split = (int)(item % a.splits);
+  const Tile at = find_tile<QT>(a, (int)(item / a.splits / heads));
+  const int h = (int)((blockIdx.x - (unsigned)at.n * (unsigned)a.H) % ways
+                      + item / a.splits % heads * ways);
+  if (at.first >= at.nq || h >= a.H) return;
+  const int D = a.D, nq = at.nq, nk = at.nk;
+  const int64_t qa = at.qa, ka = at.ka;
   const T *k = (const T *)a.k + ka * a.k_st + h * a.k_sh;
   const T *v = (const T *)a.v + ka * a.v_st + h * a.v_sh;
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = wave / GW, gw = wave % GW;  // key group, wave within it
   const int gt = threadIdx.x % GT;
   const int col = lane & 31, hf = lane >> 5;
@@ -154,25 +223,21 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
   const int ntiles = (int)((int64_t)all * (split + 1) / a.splits) - tile_first;
   const int steps = (ntiles + KS - 1) / KS;
 
+  // Pieces of rows past the run or of dims past the head are read from the last row's or the head's
+  // first ones, so that no load stands under a condition, and stored as zeros.
   uint4 kr[CH][RAW], vr[CH][RAW];
-  auto read8 = [&](const T *p, bool in, uint4 (&r)[RAW]) {
-#pragma unroll
-    for (int i = 0; i < RAW; ++i) {
-      r[i] = make_uint4(0, 0, 0, 0);
-      if (in) {
-        if (a.vec) r[i] = reinterpret_cast<const uint4 *>(p)[i];
-        else r[i] = load16_unaligned<DT>(p + 4 * i);
-      }
-    }
-  };
-  auto load = [&](int t) {  // keys past the run and dims past the head are zeros
+  auto load = [&](int t) {
+    const int first = min((tile_first + t) * KT, nk - 1);
+    const T *kt = k + first * a.k_st, *vt = v + first * a.v_st;
+    const unsigned most = (unsigned)(nk - 1 - first);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int idx = gt + GT * i, d = 8 * (idx % (4 * DG));
-      const int64_t key = (int64_t)(tile_first + t) * KT + idx / (4 * DG);
-      const bool in = key < nk && d < D && idx < S::PIECES;
-      read8(k + key * a.k_st + d, in, kr[i]);
-      read8(v + key * a.v_st + d, in, vr[i]);
+      const unsigned idx = gt + GT * i, row = min(idx / (4 * DG), most);
+      const unsigned d = 8 * (idx % (4 * DG)) < (unsigned)D ? 8 * (idx % (4 * DG)) : 0;
+      const uint4 *kp = reinterpret_cast<const uint4 *>(kt + (row * (unsigned)a.k_st + d));
+      const uint4 *vp = reinterpret_cast<const uint4 *>(vt + (row * (unsigned)a.v_st + d));
+#pragma unroll
+      for (int j = 0; j < RAW; ++j) kr[i][j] = kp[j], vr[i][j] = vp[j];
     }
   };
   auto put = [&](uint8_t *to, const uint4 (&r)[RAW]) {
@@ -189,8 +254,18 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
       }
     }
   };
-  auto store = [&](int buf) {
+  auto store = [&](int t, int buf) {
     uint8_t *kt = tile0 + buf * BUF, *vt = kt + PLANES * S::PLANE;
+    const int left = nk - (tile_first + t) * KT;  // rows of the tile that are keys
+    if (left < KT || D != 32 * DG) {  // uniform
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int idx = gt + GT * i;
+        if (idx / (4 * DG) >= left || 8 * (idx % (4 * DG)) >= D)
+#pragma unroll
+          for (int j = 0; j < RAW; ++j) kr[i][j] = vr[i][j] = make_uint4(0, 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int idx = gt + GT * i, at = idx / (4 * DG) * STRIDE + idx % (4 * DG) * 16;
@@ -201,15 +276,18 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
     }
   };
 
-  for (int tile = within / a.splits; tile * QT < nq; tile += a.tiles) {
-    const int query = tile * QT + 32 * gw + col;
-    uint4 qop[2 * DG][PLANES];
-#pragma unroll
-    for (int kk = 0; kk < 2 * DG; ++kk) {
+  {
+    const int query = at.first + 32 * gw + col;
+    const bool active = at.first + 32 * gw < nq;  // (of the wave) some query is one
+    const T *qp = (const T *)a.q + (qa + min(query, nq - 1)) * a.q_st + h * a.q_sh;
+    auto read_query = [&](int kk, uint4 (&to)[PLANES]) {  // dims 16 kk + 8 hf .. + 7
       const int d = 16 * kk + 8 * hf;
-      const T *p = (const T *)a.q + (qa + min(query, nq - 1)) * a.q_st + h * a.q_sh + d;
       uint4 r[RAW];
-      read8(p, d < D, r);
+#pragma unroll
+      for (int i = 0; i < RAW; ++i) {
+        r[i] = make_uint4(0, 0, 0, 0);
+        if (16 * kk < D) r[i] = reinterpret_cast<const uint4 *>(qp + d)[i];  // uniform
+      }
       if (a.negative) {
         const uint32_t sign = S::F32 ? 0x80000000u : 0x80008000u;
 #pragma unroll
@@ -222,11 +300,18 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
 #pragma unroll
         for (int t = 0; t < PLANES; ++t) {
           const uint2 lo = take_rounded(f0, t == 0), hi = take_rounded(f1, t == 0);
-          qop[kk][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          to[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
       } else {
-        qop[kk][0] = r[0];
+        to[0] = r[0];
       }
+    };
+    // (wide fp32 queries' terms would not fit the registers: they are read again for each tile)
+    constexpr bool HOLD = !S::F32 || DG <= 4;
+    uint4 qop[HOLD ? 2 * DG : 1][PLANES];
+    if constexpr (HOLD) {
+#pragma unroll
+      for (int kk = 0; kk < 2 * DG; ++kk) read_query(kk, qop[kk]);
     }
 
     floatx16_t o[DG];
@@ -234,136 +319,184 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
     for (int b = 0; b < DG; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+    // A row's reference m is a score; weights are 2^((score - m) scale + WEIGHT_LOG2).
     float m = NO_SCORE, l = 0.f;
+    float ms = 0.f;     // m * scale - WEIGHT_LOG2
+    bool fresh = true;  // (of the wave) no row has one yet
+    bool wide = false;  // (of the wave) some row's ms loses its units
 
-    auto attend = [&](int t, int buf) {
-      const uint8_t *kt = tile0 + buf * BUF, *vt = kt + PLANES * S::PLANE;
-      floatx16_t s[KB];
+    // 32 keys from row 32 b of the buffer on; ragged: `left` of them
+    auto attend_block = [&](int left, int b, int buf, auto ragged) {
+      const uint8_t *kt = tile0 + buf * BUF + 32 * b * STRIDE, *vt = kt + PLANES * S::PLANE;
+      auto scores = [&]() {
+        floatx16_t s;
+        if constexpr (S::F32) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int b = 0; b < KB; ++b) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 2 * DG; ++kk) {
-          const uint8_t *at = kt + (32 * b + col) * STRIDE + (2 * kk + hf) * 16;
+          const uint8_t *at = kt + col * STRIDE + (2 * kk + hf) * 16;
+          if constexpr (!HOLD) read_query(kk, qop[0]);
+          const auto &qk = qop[HOLD ? kk : 0];
 #pragma unroll
           for (int p = PLANES - 1; p >= 0; --p) {
             const uint4 kop = *reinterpret_cast<const uint4 *>(at + p * S::PLANE);
 #pragma unroll
-            for (int t = PLANES - 1 - p; t >= 0; --t) s[b] = mfma32<MDT>(kop, qop[kk][t], s[b]);
+            for (int t = PLANES - 1 - p; t >= 0; --t) s = mfma32<MDT>(kop, qk[t], s);
           }
         }
-      }
-      const int left = nk - (tile_first + t) * KT;
-      if (left < KT) {
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
+        if constexpr (S::F32) __builtin_amdgcn_s_setprio(0);
+        if (decltype(ragged)::value && left < 32) {  // uniform
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (32 * b + 8 * (i / 4) + 4 * hf + i % 4 >= left) s[b][i] = NEG_INF_F;
-      }
-      float mx = NO_SCORE;
+            s[i] = 8 * (i / 4) + i % 4 < left - 4 * hf ? s[i] : NEG_INF_F;
+        }
+        return s;
+      };
+      // a lane's weights as the second product takes them, and their sum as it sees them
+      uint4 pop[2][PLANES];
+      float sum;
+      auto take = [&](floatx16_t &s) {
+        sum = 0.f;
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
+        for (int st = 0; st < 2; ++st) {
+          float p0[4], p1[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-      float ma, mb;
-      half_pair(mx, ma, mb);
-      mx = fmaxf(ma, mb);
-      const bool need = mx > m;
-      if (__builtin_amdgcn_ballot_w64(need) != 0) {
-        const float corr = need ? fast_exp2((m - mx) * a.scale_log2) : 1.f;
-        l *= corr;
+          for (int i = 0; i < 4; ++i) p0[i] = s[8 * st + i], p1[i] = s[8 * st + 4 + i];
+          if constexpr (S::F32) {
 #pragma unroll
-        for (int b = 0; b < DG; ++b)
+            for (int i = 0; i < 4; ++i) sum += p0[i] + p1[i];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[b][i] *= corr;
-        m = need ? mx : m;
-      }
-      const float ms = m * a.scale_log2 - WEIGHT_LOG2;
+            for (int t = 0; t < PLANES; ++t) {
+              const uint2 lo = take_bf16<true>(p0), hi = take_bf16<true>(p1);
+              pop[st][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+          } else {
+            pop[st][0] = make_uint4(narrow2<DT>(p0[0], p0[1]), narrow2<DT>(p0[2], p0[3]),
+                                    narrow2<DT>(p1[0], p1[1]), narrow2<DT>(p1[2], p1[3]));
+            sum = add_pair<DT>(pop[st][0].x, sum);
+            sum = add_pair<DT>(pop[st][0].y, sum);
+            sum = add_pair<DT>(pop[st][0].z, sum);
+            sum = add_pair<DT>(pop[st][0].w, sum);
+          }
+        }
+      };
+      // Weights about the references as they stand, without a look at the scores' maxima: a weight
+      // that passes its reference by more than the slack shows in its lane's sum.
       // One operation a weight where the product m * scale keeps its units to 2^-8 (what it is
-      // rounded by is the same for every weight of the row), two where it does not: by row, so
-      // that none hangs on its neighbours
-      const bool small = fabsf(ms) <= 65536.f;
-      if (__builtin_amdgcn_ballot_w64(!small) == 0) {
+      // rounded by is the same for every weight of the row), two where it does not: by row, so that
+      // none hangs on its neighbours.
+      auto weights = [&](floatx16_t &s) {
+        if (!wide) {
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = fast_exp2(fmaf(s[b][i], a.scale_log2, -ms));
-      } else {
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
+          for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale_log2, -ms));
+        } else {
+          const bool one = fabsf(ms) <= 65536.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float one = fmaf(s[b][i], a.scale_log2, -ms);
-            const float two = fmaf(s[b][i] - m, a.scale_log2, WEIGHT_LOG2);
-            s[b][i] = fast_exp2(small ? one : two);
+            const float x = fmaf(s[i], a.scale_log2, -ms);
+            const float y = fmaf(s[i] - m, a.scale_log2, WEIGHT_LOG2);
+            s[i] = fast_exp2(one ? x : y);
           }
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int st = 0; st < KT / 16; ++st) {
-        const int e = 8 * (st & 1);
-        float p0[4], p1[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p0[i] = s[st >> 1][e + i], p1[i] = s[st >> 1][e + 4 + i];
-        uint4 pop[PLANES];
-        if constexpr (S::F32) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum += p0[i] + p1[i];
-#pragma unroll
-          for (int t = 0; t < PLANES; ++t) {
-            const uint2 lo = take_bf16<true>(p0), hi = take_bf16<true>(p1);
-            pop[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-          }
-        } else {
-          // the normaliser sums the weights as they are, which the product sees rounded
-          pop[0] = make_uint4(Mfma<DT>::narrow2(p0[0], p0[1]), Mfma<DT>::narrow2(p0[2], p0[3]),
-                              Mfma<DT>::narrow2(p1[0], p1[1]), Mfma<DT>::narrow2(p1[2], p1[3]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum += p0[i] + p1[i];
         }
+        take(s);
+      };
+      if (!fresh) {
+        floatx16_t s = scores();
+        weights(s);
+      }
+      if (fresh || __builtin_amdgcn_ballot_w64(!(sum <= MOST_SUM)) != 0) {
+        // rows whose own sums pass the slack move, whatever stands beside them
+        bool need = true;
+        if (!fresh) {
+          float sa, sb;
+          half_pair(sum, sa, sb);
+          need = !(sa <= MOST_SUM && sb <= MOST_SUM);
+        }
+        floatx16_t s = scores();
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        float ma, mb;
+        half_pair(mx, ma, mb);
+        mx = fmaxf(ma, mb);
+        if (!fresh) {
+          const float corr = need ? fast_exp2((m - mx) * a.scale_log2) : 1.f;
+          l *= corr;
+#pragma unroll
+          for (int d = 0; d < DG; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+        }
+        m = need ? mx : m;
+        ms = fmaf(m, a.scale_log2, -WEIGHT_LOG2);
+        fresh = false;
+        wide = __builtin_amdgcn_ballot_w64(!(fabsf(ms) <= 65536.f)) != 0;
+        weights(s);
+      }
+      l += sum;
+      // (waves in their products go first, so that others' vector work runs beside them: fp32, whose
+      // products take most of the time, 68 against 65 us)
+      if constexpr (S::F32) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
         // 16 lanes: four keys, 16 dims
         const int key = 16 * st + 4 * hf + (lane & 15) / 4;
         const uint8_t *vp = vt + key * STRIDE + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
-        for (int b = 0; b < DG; ++b) {
+        for (int d = 0; d < DG; ++d) {
 #pragma unroll
           for (int p = PLANES - 1; p >= 0; --p) {
-            const uint2 v0 = read_turned(vp + p * S::PLANE + 64 * b);
-            const uint2 v1 = read_turned(vp + p * S::PLANE + 64 * b + 8 * STRIDE);
+            const uint2 v0 = read_turned(vp + p * S::PLANE + 64 * d);
+            const uint2 v1 = read_turned(vp + p * S::PLANE + 64 * d + 8 * STRIDE);
             const uint4 vop = make_uint4(v0.x, v0.y, v1.x, v1.y);
 #pragma unroll
-            for (int t = PLANES - 1 - p; t >= 0; --t) o[b] = mfma32<MDT>(vop, pop[t], o[b]);
+            for (int t = PLANES - 1 - p; t >= 0; --t) o[d] = mfma32<MDT>(vop, pop[st][t], o[d]);
           }
         }
       }
-      l += sum;
+      if constexpr (S::F32) __builtin_amdgcn_s_setprio(0);
+    };
+
+    auto attend = [&](int buf) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b) attend_block(32, b, buf, std::false_type{});
+    };
+    auto attend_last = [&](int t, int buf) {  // of the run's last tile some rows may be no keys
+      const int left = nk - (tile_first + t) * KT;
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+        if (left > 32 * b) attend_block(left - 32 * b, b, buf, std::true_type{});
     };
 
     // Step t: the group's tile of step t is in buffer t % BUFS, the next one's rows in flight.
-    load(grp);
+    // (all but the last step's are whole tiles of every group)
+    if (steps > 0) load(grp);
     if constexpr (BUFS == 2) {
-      store(0);
+      if (steps > 0) store(grp, 0);
       if (steps > 1) load(KS + grp);
       __syncthreads();
-      for (int t = 0; t < steps; ++t) {
-        if (t + 1 < steps) {
-          store((t + 1) & 1);
-          if (t + 2 < steps) load((t + 2) * KS + grp);
-        }
-        if (t * KS + grp < ntiles) attend(t * KS + grp, t & 1);
+#pragma unroll 1
+      for (int t = 0; t < steps - 1; ++t) {
+        store((t + 1) * KS + grp, (t + 1) & 1);
+        if (t + 2 < steps) load((t + 2) * KS + grp);
+        if (active) attend(t & 1);
         __syncthreads();
       }
     } else {
+#pragma unroll 1
       for (int t = 0; t < steps; ++t) {
-        store(0);
+        store(t * KS + grp, 0);
         __syncthreads();
-        if (t + 1 < steps) load((t + 1) * KS + grp);
-        if (t * KS + grp < ntiles) attend(t * KS + grp, 0);
+        if (t + 1 >= steps) break;
+        load((t + 1) * KS + grp);
+        if (active) attend(0);
         __syncthreads();
       }
     }
+    const int last = (steps - 1) * KS + grp;
+    if (active && steps > 0 && last < ntiles) attend_last(last, BUFS == 2 ? (steps - 1) & 1 : 0);
+    __syncthreads();
     // both halves of a column hold the same reference and other keys
     {
       float la, lb;
@@ -406,7 +539,6 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
         }
         m = M;
       }
-      __syncthreads();  // the next tile's stores follow
     }
     if (grp == 0 && query < nq) {
       const int64_t at = (qa + query) * a.H + h;
@@ -423,56 +555,103 @@ __global__ __launch_bounds__(256) void cross_attention_kernel(CrossArgs a) {
           }
         if (hf == 0) a.part.ml[at * a.splits + split] = make_float2(m, l);
       } else {
-        T *dst = (T *)a.out + at * D;
+        T *dst = (T *)a.out + at * D + 4 * hf;
         // no keys, or scores of -inf alone: 0; NaN scores stay NaN
         const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+        auto write = [&](auto aligned) {
 #pragma unroll
-        for (int b = 0; b < DG; ++b)
+          for (int b = 0; b < DG; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = 32 * b + 8 * i + 4 * hf;
-            if (d >= D) continue;
-            float y[4];
+            for (int i = 0; i < 4; ++i) {
+              if (i >= 2 && 32 * b + 16 >= D) continue;  // (head sizes are multiples of 16; uniform)
+              if (32 * b >= D) continue;
+              T *to = dst + 32 * b + 8 * i;
+              float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = o[b][4 * i + j] * inv;
-            if constexpr (S::F32) {
-              if (a.out_vec) *reinterpret_cast<float4 *>(dst + d) = make_float4(y[0], y[1], y[2], y[3]);
-              else dst[d] = y[0], dst[d + 1] = y[1], dst[d + 2] = y[2], dst[d + 3] = y[3];
-            } else {
-              const uint32_t w0 = Mfma<DT>::narrow2(y[0], y[1]), w1 = Mfma<DT>::narrow2(y[2], y[3]);
-              if (a.out_vec) {
-                *reinterpret_cast<uint2 *>(dst + d) = make_uint2(w0, w1);
+              for (int j = 0; j < 4; ++j) y[j] = o[b][4 * i + j] * inv;
+              if constexpr (S::F32) {
+                if constexpr (decltype(aligned)::value)
+                  *reinterpret_cast<float4 *>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                else to[0] = y[0], to[1] = y[1], to[2] = y[2], to[3] = y[3];
               } else {
-                dst[d] = (uint16_t)w0, dst[d + 1] = (uint16_t)(w0 >> 16);
-                dst[d + 2] = (uint16_t)w1, dst[d + 3] = (uint16_t)(w1 >> 16);
+                const uint32_t w0 = narrow2<DT>(y[0], y[1]), w1 = narrow2<DT>(y[2], y[3]);
+                if constexpr (decltype(aligned)::value) {
+                  *reinterpret_cast<uint2 *>(to) = make_uint2(w0, w1);
+                } else {
+                  to[0] = (uint16_t)w0, to[1] = (uint16_t)(w0 >> 16);
+                  to[2] = (uint16_t)w1, to[3] = (uint16_t)(w1 >> 16);
+                }
               }
             }
-          }
+        };
+        if (a.out_vec) write(std::true_type{});
+        else write(std::false_type{});
       }
     }
   }
 }
 
-// One workgroup a (sequence, head) and query of the sequence.
-template <int DT> __global__ __launch_bounds__(JOIN_NT) void cross_join_kernel(CrossArgs a) {
-  const int n = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
-  const int64_t qa = min(max((int64_t)a.q_start[n], (int64_t)0), a.num_queries);
-  const int64_t qb = min(max((int64_t)a.q_start[n + 1], qa), a.num_queries);
-  for (int64_t r = qa + blockIdx.y; r < qb; r += gridDim.y) {
-    const int64_t at = r * a.H + h;
-    join_splits<DT>(a.out, a.part, at, at * a.D, a.D, a.splits, a.scale_log2);
-    __syncthreads();
+// Whether a row is one of a sequence's.
+__device__ __forceinline__ bool in_sequence(const CrossArgs &a, int row) {
+  int lo = 0, hi = a.sequences;  // the last sequence that begins at or before the row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (a.q_start[mid] <= row) lo = mid;
+    else hi = mid;
   }
+  return row >= a.q_start[lo] && row < a.q_start[lo + 1];
+}
+
+// The splits of each (query, head) joined: of many a workgroup takes one (query, head), of few a
+// thread four dims.  (50 queries x 8 heads of 128 in 32 parts, with the attention: 43 / 55 us;
+// 590 x 12 of 64 in two 26 / 21.)
+constexpr int CROSS_JOIN_NT = 256;
+constexpr int CROSS_JOIN_FEW = 8;
+template <int DT> __global__ __launch_bounds__(JOIN_NT) void cross_join_many_kernel(CrossArgs a) {
+  const int64_t at = blockIdx.x;
+  if (!in_sequence(a, (int)(at / a.H))) return;
+  join_splits<DT>(a.out, a.part, at, at * a.D, a.D, a.splits, a.scale_log2);
+}
+template <int DT> __global__ __launch_bounds__(CROSS_JOIN_NT) void cross_join_few_kernel(CrossArgs a) {
+  using T = typename Elem<DT>::T;
+  const int quads = a.D / 4;
+  const int64_t i = (int64_t)blockIdx.x * CROSS_JOIN_NT + threadIdx.x;
+  const int64_t at = i / quads;  // query * H + head
+  const int row = (int)(at / a.H), d = (int)(i % quads) * 4;
+  if (row >= a.num_queries || !in_sequence(a, row)) return;
+  const float2 *ml = a.part.ml + at * a.splits;
+  const float *acc = a.part.acc + at * a.splits * a.D + d;
+  float2 x[CROSS_JOIN_FEW];
+  float4 v[CROSS_JOIN_FEW];
+#pragma unroll
+  for (int s = 0; s < CROSS_JOIN_FEW; ++s) {
+    const int at_split = min(s, a.splits - 1);
+    x[s] = ml[at_split];
+    v[s] = *reinterpret_cast<const float4 *>(acc + (int64_t)at_split * a.D);
+  }
+  float M = x[0].x;
+#pragma unroll
+  for (int s = 1; s < CROSS_JOIN_FEW; ++s) M = fmaxf(M, x[s].x);
+  float S = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < CROSS_JOIN_FEW; ++s) {
+    if (s >= a.splits) break;
+    const float e = fast_exp2((x[s].x - M) * a.scale_log2);
+    S = fmaf(x[s].y, e, S);
+    o[0] = fmaf(v[s].x, e, o[0]), o[1] = fmaf(v[s].y, e, o[1]);
+    o[2] = fmaf(v[s].z, e, o[2]), o[3] = fmaf(v[s].w, e, o[3]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store_result<DT>((T *)a.out + at * a.D + d + j, S, o[j]);
 }
 
 template <int DT, int DG, int KS> void launch_cross_shape(const CrossArgs &a, hipStream_t stream) {
-  const int64_t pairs = (int64_t)a.sequences * a.H;
-  const dim3 grid((unsigned)((pairs + 7) / 8 * 8 * a.tiles * a.splits));
-  cross_attention_kernel<DT, DG, KS><<<grid, dim3(256), 0, stream>>>(a);
+  const dim3 grid((unsigned)cross_grid(a.num_queries, a.sequences, a.H, KS, a.splits, a.spread));
+  cross_attention_kernel<DT, DG, KS><<<grid, dim3(64 * WAVES), 0, stream>>>(a);
 }
 
 template <int DT, int DG> void launch_cross_groups(const CrossArgs &a, int ks, hipStream_t stream) {
-  constexpr int MOST = DT != VFL_FLOAT32 || DG <= 2 ? 4 : DG <= 4 ? 2 : 1;  // cross_most_groups
+  constexpr int MOST = cross_most_groups(DT == VFL_FLOAT32, DG);
   if constexpr (MOST >= 4) {
     if (ks == 4) return launch_cross_shape<DT, DG, 4>(a, stream);
   }
@@ -494,9 +673,14 @@ template <int DT> int launch_cross(const CrossArgs &a, int ks, hipStream_t strea
   }
   const int st = launch_status("packed_cross_attention");
   if (st != VFL_OK || a.splits == 1) return st;
-  const unsigned rows = (unsigned)min((int64_t)65535, (int64_t)a.num_queries);
-  cross_join_kernel<DT>
-      <<<dim3((unsigned)(a.sequences * a.H), rows), dim3(JOIN_NT), 0, stream>>>(a);
+  const int64_t units = a.num_queries * a.H;
+  if (a.splits > CROSS_JOIN_FEW) {
+    cross_join_many_kernel<DT><<<dim3((unsigned)units), dim3(JOIN_NT), 0, stream>>>(a);
+  } else {
+    const int64_t threads = units * (a.D / 4);
+    cross_join_few_kernel<DT><<<dim3((unsigned)((threads + CROSS_JOIN_NT - 1) / CROSS_JOIN_NT)),
+                                dim3(CROSS_JOIN_NT), 0, stream>>>(a);
+  }
   return launch_status("packed_cross_attention");
 }
 

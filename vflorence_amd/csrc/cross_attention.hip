@@ -8,27 +8,43 @@ namespace {
 
 // Key groups of a workgroup and workgroups of a run of keys.
 struct CrossPlan {
-  int ks, tiles, splits;
+  int ks, splits;
+  bool spread;
 };
 
-CrossPlan cross_plan(int64_t sequences, int H, int D, bool f32, int64_t max_queries,
-                     int64_t max_keys) {
+// us, 16 heads of 64 over 256 to 1024 keys if not said otherwise, bf16:
+// - more key groups are the faster ones where tiles of 128 queries are few or would stay mostly
+//   empty.  One / two / four groups: 8 runs of 60 to 128 queries 19.7 / 13.4 / 18.1, 590 queries x 12
+//   heads over 590 keys 13.8 / 10.1 / 16.7, 64 runs of 40 to 64 45.0 / 39.8 / 74.8; yet 64 of 60 to
+//   128 49.1 / 54.4 / 124, 16 of 31 to 257 26.5 / 28.8 / 48.5; 9 queries x 12 heads over 590 keys
+//   12.6 / 9.4 / 8.9.  fp32, whose tiles take a CU's LDS in two groups: 8 runs of 60 to 128 56.8 / 38.3
+//   / 48.1, but 64 of 20 to 32 110 / 128 / 120, 16 of 31 to 257 67.8 / 86.4 / 116.
+// - runs of keys are split where that leaves no more workgroups than two a CU (fp32: one): 8 runs
+//   of 20 to 32 queries over 1000 to 2000 keys whole 22.9, in four parts 17.9, in eight 20.7; fp32 4
+//   of 60 to 64 whole 63.6, in four 26.6, in eight 30.4; more than 16 parts cost the join more
+//   (2 runs of 17 and 33 over 17001 and 39999 keys, fp16, 8 heads of 128: 16 parts 45.4, 32 49.6).
+// - launches of up to two workgroups a CU go to any XCD: 12 heads, fp32, 590 queries in two parts
+//   21.2, a head to an XCD 33.6.
+CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool f32,
+                     int64_t max_queries, int64_t max_keys) {
   const int DG = (D + 31) / 32;
-  CrossPlan p{1, 1, 1};
-  if (max_queries < 1) max_queries = 1;
-  const int64_t wide = sequences * H * ((max_queries + 127) / 128);
-  p.ks = max_queries <= 32 || wide <= 32 ? 4 : max_queries <= 64 || wide <= 192 ? 2 : 1;
+  CrossPlan p{1, 1, false};
+  auto workgroups = [&](int ks) {  // that hold queries, at most
+    const int64_t qt = 128 / ks, tiles = (max_queries + qt - 1) / qt;
+    const int64_t by_length = sequences * (tiles > 1 ? tiles : 1);
+    const int64_t by_rows = num_queries / qt + sequences;
+    return (by_length < by_rows ? by_length : by_rows) * H;
+  };
+  if (max_queries <= 32 && workgroups(1) <= 64) p.ks = 4;
+  else if ((!f32 && max_queries <= 64) || workgroups(1) <= 256) p.ks = 2;
   const int most = cross_most_groups(f32, DG);
   if (p.ks > most) p.ks = most;
   while (p.ks > 1 && 64 * (p.ks / 2) >= max_keys) p.ks /= 2;
-  const int64_t qt = 128 / p.ks;
-  p.tiles = (int)((max_queries + qt - 1) / qt);
-  const int64_t wgs = sequences * H * p.tiles;
-  if (wgs < 256 && max_keys > 2048) {
-    const int64_t fill = 512 / wgs, parts = max_keys / (256 * p.ks);
-    const int64_t s = fill < parts ? fill : parts;
-    if (s >= 2) p.splits = (int)s;
-  }
+  const int64_t wgs = workgroups(p.ks);
+  const int64_t fill = (f32 ? 256 : 512) / wgs, parts = max_keys / (f32 ? 64 : 256 * p.ks);
+  const int64_t most_parts = fill < parts ? fill : parts;
+  if (most_parts >= 2) p.splits = most_parts < 16 ? (int)most_parts : 16;
+  p.spread = wgs * p.splits <= 512;
   return p;
 }
 
@@ -43,8 +59,8 @@ extern "C" int64_t vfl_packed_cross_attention_workspace(int64_t num_queries, int
                                                         int64_t max_query_len,
                                                         int64_t max_key_len, int dtype) {
   if (num_queries <= 0 || num_sequences <= 0 || num_heads <= 0 || head_dim <= 0) return 0;
-  const CrossPlan p = cross_plan(num_sequences, num_heads, head_dim, dtype == VFL_FLOAT32,
-                                 max_query_len, max_key_len);
+  const CrossPlan p = cross_plan(num_queries, num_sequences, num_heads, head_dim,
+                                 dtype == VFL_FLOAT32, max_query_len, max_key_len);
   return p.splits > 1 ? num_queries * num_heads * p.splits * split_part_bytes(head_dim) : 0;
 }
 
@@ -83,16 +99,27 @@ extern "C" int vfl_packed_cross_attention(
     return VFL_E_INVALID;
   }
   const int eb = elem_bytes(dtype);
-  if ((uintptr_t)query % eb || (uintptr_t)key % eb || (uintptr_t)value % eb ||
-      (uintptr_t)out % eb || (uintptr_t)workspace % 16) {
-    set_error("%s: misaligned pointer (workspace 16 bytes, others their element)", who);
+  if (((uintptr_t)query | (uintptr_t)key | (uintptr_t)value | (uintptr_t)workspace) % 16 ||
+      (uintptr_t)out % eb ||
+      (query_stride_token | query_stride_head | key_stride_token | key_stride_head |
+       value_stride_token | value_stride_head) % (16 / eb)) {
+    set_error("%s: misaligned rows (query, key, value, their strides and workspace 16 bytes, out "
+              "its element)", who);
     return VFL_E_INVALID;
   }
-  const CrossPlan plan = cross_plan(num_sequences, num_heads, head_dim, dtype == VFL_FLOAT32,
-                                    max_query_len, max_key_len);
-  if (!grid_fits((num_sequences * num_heads + 7) / 8 * 8 * plan.tiles * plan.splits, 256)) {
-    set_error("%s: %lld sequences x %d heads x %d tiles exceed a launch", who,
-              (long long)num_sequences, num_heads, plan.tiles);
+  // (a tile's rows are addressed by 32-bit offsets)
+  if (key_stride_token < 0 || value_stride_token < 0 || key_stride_token > CROSS_MAX_STRIDE ||
+      value_stride_token > CROSS_MAX_STRIDE) {
+    set_error("%s: key and value token strides %lld, %lld (0 to %d)", who,
+              (long long)key_stride_token, (long long)value_stride_token, CROSS_MAX_STRIDE);
+    return VFL_E_INVALID;
+  }
+  const CrossPlan plan = cross_plan(num_queries, num_sequences, num_heads, head_dim,
+                                    dtype == VFL_FLOAT32, max_query_len, max_key_len);
+  if (!grid_fits(cross_grid(num_queries, num_sequences, num_heads, plan.ks, plan.splits, plan.spread),
+                 256)) {
+    set_error("%s: %lld queries of %lld sequences x %d heads exceed a launch", who,
+              (long long)num_queries, (long long)num_sequences, num_heads);
     return VFL_E_INVALID;
   }
   CrossArgs a;
@@ -104,12 +131,8 @@ extern "C" int vfl_packed_cross_attention(
   a.q_start = query_start_loc, a.k_start = key_start_loc;
   a.num_queries = num_queries, a.num_keys = num_keys;
   a.sequences = (int)num_sequences, a.H = num_heads, a.D = head_dim;
-  a.tiles = plan.tiles;
   a.scale_log2 = decode_scale_log2(scale);
-  a.negative = scale < 0.f;
-  const int64_t vec = 16 / eb;
-  a.vec = ((uintptr_t)query | (uintptr_t)key | (uintptr_t)value) % 16 == 0 &&
-          (a.q_st | a.q_sh | a.k_st | a.k_sh | a.v_st | a.v_sh) % vec == 0;
+  a.negative = scale < 0.f, a.spread = plan.spread;
   a.out_vec = (uintptr_t)out % (4 * eb) == 0;
   a.splits = plan.splits, a.part = {nullptr, nullptr};
   if (plan.splits > 1) {

@@ -1183,6 +1183,15 @@ def _cross_workspace(*sizes: int) -> int:
     return lib.vfl_packed_cross_attention_workspace(*sizes)
 
 
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` ([T, H, D], unit last stride) where each head's row is 16-byte aligned and 2^22
+    elements or less from the next token's, or a copy."""
+    token, head, _ = x.stride()
+    if (x.data_ptr() | (token | head) * x.element_size()) & 15 or token > 1 << 22:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
 def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                            out: torch.Tensor, query_start_loc: torch.Tensor,
                            key_start_loc: torch.Tensor, *, scale: float, max_query_len: int,
@@ -1225,6 +1234,8 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     index = one_gpu(query, key, value, out, query_start_loc, key_start_loc)
     if (query.requires_grad or key.requires_grad or value.requires_grad or out.requires_grad):
         refuse_gradients("packed_cross_attention")
+    # the kernel reads 16 bytes at a time; rows that do not allow it are copied
+    query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
     query_start_loc, key_start_loc = query_start_loc.contiguous(), key_start_loc.contiguous()
     sequences = query_start_loc.numel() - 1
     longest = (min(max_query_len, num_queries), min(max_key_len, key.shape[0]))
