@@ -369,24 +369,23 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
   }
 }
 
-// Waves of a workgroup and workgroups of a context.
+// Waves of a workgroup and workgroups of a context.  A context is split where four parts or more
+// fill eight waves a CU and leave each wave 128 tokens; more waves than that, or eight to a
+// workgroup, were the slower ones (2 rows of 17001 and 39999 tokens x 8 heads of 128, us: workgroups
+// of four waves, 4 / 8 / 12 / 16 a CU 18.9 / 17.8 / 19.4 / 20.5, of eight 25.2 / 19.4 / 22.5 / 21.6;
+// one row of 40000 x 16 of 64 16.8 / 14.9 / 15.6 / 15.4).  What is not split takes eight waves where
+// workgroups are few (16 rows of 2000 to 4000 tokens x 16 heads 14.7, four waves 17.6; 1536 workgroups
+// of up to 1000 tokens 18.6, four waves 14.9).
 struct Attn4Plan {
   int waves, splits;
 };
 
 inline Attn4Plan attn4_plan(int64_t num_groups, int H, int D, int64_t max_tokens) {
-  // waves of a launch that the card holds at once, by the registers that a head of D takes
-  const int64_t resident = 256 * (D <= 128 ? 16 : 8);
   const int64_t wgs = num_groups * H;
-  Attn4Plan p{D <= 256 && wgs <= (D <= 64 ? 256 : 512) ? 8 : 4, 1};
-  const int64_t bytes = max_tokens * 2 * D;
-  if (bytes > (192 << 10) && wgs * p.waves < resident) {
-    const int64_t fill = resident / (wgs * p.waves);
-    const int64_t most = max_tokens / 64 / (p.waves * 2);
-    const int64_t parts = fill < most ? fill : most;
-    if (parts >= 4) p.splits = (int)parts;
-  }
-  return p;
+  const int64_t fill = 256 * (D <= 256 ? 8 : 4) / (wgs * 4), most = max_tokens / (4 * 128);
+  const int64_t parts = fill < most ? fill : most;
+  if (parts >= 4) return Attn4Plan{4, (int)parts};
+  return Attn4Plan{D <= 256 && wgs <= (D <= 64 ? 256 : 512) ? 8 : 4, 1};
 }
 
 template <int DT, int G, int ROWS>

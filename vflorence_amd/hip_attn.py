@@ -909,47 +909,46 @@ def reshape_and_cache_8bit(key: torch.Tensor, value: torch.Tensor, k_cache: torc
 def _check_paged_rows(query: torch.Tensor, out: torch.Tensor, seq_lens: torch.Tensor,
                       block_table: torch.Tensor, *caches: torch.Tensor):
     """Checks what a decode attention takes beside its caches; ``(block_table, seq_lens)`` as the
-    kernels read them."""
-    num_rows = query.shape[0]
-    if out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
+    kernels read them, and the index of the GPU that holds all of it."""
+    shape = query.shape
+    if out.dtype != query.dtype or out.shape != shape or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of query's shape and dtype")
+    num_rows = shape[0]
     if seq_lens.dtype != torch.int32 or seq_lens.shape != (num_rows,):
         raise ValueError(f"seq_lens must be int32 [{num_rows}], got {seq_lens.dtype} "
                          f"{tuple(seq_lens.shape)}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2
-            or block_table.shape[0] != num_rows):
+    table = block_table.shape
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != num_rows:
         raise ValueError(f"block_table must be int32 [{num_rows}, max_blocks], got "
-                         f"{block_table.dtype} {tuple(block_table.shape)}")
-    one_gpu(query, *caches, out, seq_lens, block_table)
-    width = block_table.shape[1]
-    if (block_table.stride(1) != 1 and width > 1) or (block_table.stride(0) < width
-                                                      and num_rows > 1):
+                         f"{block_table.dtype} {tuple(table)}")
+    index = one_gpu(query, *caches, out, seq_lens, block_table)
+    step = block_table.stride()
+    if (step[1] != 1 and table[1] > 1) or (step[0] < table[1] and num_rows > 1):
         block_table = block_table.contiguous()
-    return block_table, seq_lens.contiguous()
+    return block_table, seq_lens.contiguous(), index
 
 
-def _shared_groups(sm: SchedulerMetadata | None, query: torch.Tensor, block_size: int):
+def _shared_groups(sm: SchedulerMetadata | None, shape: torch.Size, index: int, block_size: int):
     """``(group_start, group_order, groups, rows of a group at most)`` of the row groups that
-    share a table; every row its own group where they do not."""
-    num_rows, num_heads, head_dim = query.shape
+    share a table, for queries of ``shape`` on GPU ``index``; every row its own group where they
+    do not."""
+    num_rows, num_heads, head_dim = shape
     if sm is None:
         return None, None, num_rows, 1
-    if (sm.num_heads, sm.head_dim, sm.block_size) != (num_heads, head_dim, block_size):
+    if sm.num_heads != num_heads or sm.head_dim != head_dim or sm.block_size != block_size:
         raise ValueError("scheduler_metadata was made for another cache: "
                          f"H={sm.num_heads}, D={sm.head_dim}, block_size={sm.block_size}")
     if sm.group_plan is not None and sm.group_plan.folded:
         raise ValueError("a group plan with copy-on-write folded in is for "
                          "self_attention_with_kv_write alone")
-    if sm.own_tables and sm.group_start is not None:
-        return None, None, num_rows, 1
     start, order = sm.group_start, sm.group_order
-    if start is not None:
-        one_gpu(query, start)
-        start = start.contiguous()
-    if order is not None:
-        one_gpu(query, order)
-        order = order.contiguous()
-    return start, order, sm.num_groups, sm.max_group_size
+    if sm.own_tables and start is not None:
+        return None, None, num_rows, 1
+    for t in (start, order):
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"tensors on different devices: cuda:{index} and {t.device}")
+    return (start if start is None else start.contiguous(),
+            order if order is None else order.contiguous(), sm.num_groups, sm.max_group_size)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -978,13 +977,13 @@ def attention_with_kv_cache_8bit(query: torch.Tensor, k_cache: torch.Tensor,
                          f"dimension, got {tuple(query.shape)}")
     num_rows = query.shape[0]
     dtype = _dtype_code(query.dtype)
-    block_table, seq_lens = _check_paged_rows(query, out, seq_lens, block_table, k_cache, v_cache,
-                                              kv_scales)
+    block_table, seq_lens, index = _check_paged_rows(query, out, seq_lens, block_table, k_cache,
+                                                     v_cache, kv_scales)
     if (query.requires_grad or out.requires_grad or k_cache.requires_grad
             or v_cache.requires_grad or kv_scales.requires_grad):
         refuse_gradients("attention_with_kv_cache_8bit")
-    index, width = query.get_device(), block_table.shape[1]
-    start, order, num_groups, _ = _shared_groups(scheduler_metadata, query, block_size)
+    width = block_table.shape[1]
+    start, order, num_groups, _ = _shared_groups(scheduler_metadata, query.shape, index, block_size)
     need = _attention_8bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     on_device(index, lib.vfl_attention_with_kv_cache_8bit, query.data_ptr(), query.stride(0),
@@ -1028,7 +1027,7 @@ def kv_cache_4bit_values(cache: torch.Tensor,
                          head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
     """The float32 keys and values that a 4-bit cache stands for, ``[num_blocks, H, block_size,
     D]`` in token order."""
-    num_blocks, heads, block_size, _ = _check_4bit_cache(cache, head_dim)
+    num_blocks, heads, block_size = _check_4bit_cache(cache, head_dim)
     groups, parts = -(-head_dim // CACHE_4BIT_GROUP), block_size // 16
     flat, size = cache.view(num_blocks, -1), heads * parts * groups * 256
     shape = (num_blocks, heads, parts, groups, 16, 16)
@@ -1047,11 +1046,12 @@ def kv_cache_4bit_values(cache: torch.Tensor,
     return found[0], found[1]
 
 
-def _check_4bit_cache(cache: torch.Tensor, head_dim: int):
-    if cache.dim() != 4 or cache.dtype != torch.uint8 or not cache.is_contiguous():
-        raise ValueError("a 4-bit cache is a contiguous torch.uint8 tensor [num_blocks, H, "
-                         f"block_size, bytes], got {cache.dtype} {tuple(cache.shape)}")
-    shape = cache.shape
+@functools.lru_cache(maxsize=4096)
+def _cache_4bit_sizes(shape: torch.Size, head_dim: int) -> tuple[int, int, int]:
+    """``(num_blocks, heads, block_size)`` of a 4-bit cache's shape, checked."""
+    if len(shape) != 4:
+        raise ValueError("a 4-bit cache is a torch.uint8 tensor [num_blocks, H, block_size, "
+                         f"bytes], got {tuple(shape)}")
     if shape[2] not in SUPPORTED_BLOCK_SIZES or head_dim not in SUPPORTED_HEAD_DIMS:
         raise ValueError(f"block_size={shape[2]}, head_dim={head_dim} has no attention kernel; "
                          f"supported: {sorted(SUPPORTED_BLOCK_SIZES)}, "
@@ -1059,27 +1059,40 @@ def _check_4bit_cache(cache: torch.Tensor, head_dim: int):
     if shape[3] != _bytes_per_token_4bit(head_dim):
         raise ValueError(f"a 4-bit cache of head_dim={head_dim} has "
                          f"{_bytes_per_token_4bit(head_dim)} bytes a token, this one {shape[3]}")
-    return shape
+    return shape[:3]
+
+
+def _check_4bit_cache(cache: torch.Tensor, head_dim: int) -> tuple[int, int, int]:
+    if cache.dtype != torch.uint8 or not cache.is_contiguous():
+        raise ValueError("a 4-bit cache is a contiguous torch.uint8 tensor, got "
+                         f"{cache.dtype} {tuple(cache.shape)}")
+    return _cache_4bit_sizes(cache.shape, head_dim)
 
 
 def _check_4bit_rows(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
                      slot_mapping: torch.Tensor):
-    """The sizes, dtype code and device index of keys and values beside a 4-bit cache."""
-    if key.dim() != 3 or value.shape != key.shape:
+    """What ``reshape_and_cache_4bit`` and ``gather_cache_4bit`` share: sizes, strides, dtype code
+    and device index of keys and values beside a 4-bit cache."""
+    shape = key.shape
+    if len(shape) != 3 or value.shape != shape:
         raise ValueError(f"key/value must be [T, H, D] of one shape, got {tuple(key.shape)}, "
                          f"{tuple(value.shape)}")
-    num_blocks, num_heads, block_size, _ = _check_4bit_cache(cache, key.shape[2])
-    if key.shape[1] != num_heads:
-        raise ValueError(f"key/value have {key.shape[1]} heads, the cache {num_heads}")
-    if key.dtype != value.dtype:
+    tokens, heads, head_dim = shape
+    num_blocks, num_heads, block_size = _check_4bit_cache(cache, head_dim)
+    if heads != num_heads:
+        raise ValueError(f"key/value have {heads} heads, the cache {num_heads}")
+    dtype = key.dtype
+    if dtype != value.dtype:
         raise ValueError("key and value must share one dtype")
-    dtype = _dtype_code(key.dtype)
-    if key.stride(2) != 1 or value.stride(2) != 1:
+    code = _dtype_code(dtype)
+    strides = (*key.stride(), *value.stride())
+    if strides[2] != 1 or strides[5] != 1:
         raise ValueError("key/value need a contiguous last dimension")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],):
-        raise ValueError(f"slot_mapping must be int64 [{key.shape[0]}], got "
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (tokens,):
+        raise ValueError(f"slot_mapping must be int64 [{tokens}], got "
                          f"{slot_mapping.dtype} {tuple(slot_mapping.shape)}")
-    return num_blocks, num_heads, block_size, dtype, one_gpu(key, value, cache, slot_mapping)
+    return (shape, num_blocks, block_size, strides, code,
+            one_gpu(key, value, cache, slot_mapping))
 
 
 def reshape_and_cache_4bit(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
@@ -1095,15 +1108,14 @@ def reshape_and_cache_4bit(key: torch.Tensor, value: torch.Tensor, cache: torch.
     brings their largest magnitude to 6 or less, so every value is rounded once, to nearest, and
     a later token changes no earlier one.  Dims that share a scale with an infinity or a NaN
     are held as NaN."""
-    num_blocks, num_heads, block_size, dtype, index = _check_4bit_rows(key, value, cache,
-                                                                       slot_mapping)
+    (tokens, heads, dim), num_blocks, block_size, st, dtype, index = _check_4bit_rows(
+        key, value, cache, slot_mapping)
     if key.requires_grad or value.requires_grad:
         refuse_gradients("reshape_and_cache_4bit")
     slot_mapping = slot_mapping.contiguous()
-    on_device(index, lib.vfl_reshape_and_cache_4bit, key.data_ptr(), value.data_ptr(),
-              key.stride(0), key.stride(1), value.stride(0), value.stride(1), cache.data_ptr(),
-              slot_mapping.data_ptr(), key.shape[0], num_heads, key.shape[2], block_size,
-              num_blocks, dtype)
+    on_device(index, lib.vfl_reshape_and_cache_4bit, key.data_ptr(), value.data_ptr(), st[0],
+              st[1], st[3], st[4], cache.data_ptr(), slot_mapping.data_ptr(), tokens, heads, dim,
+              block_size, num_blocks, dtype)
     torch.autograd.graph.increment_version((cache,))  # autograd's check of saved tensors
 
 
@@ -1113,18 +1125,16 @@ def gather_cache_4bit(cache: torch.Tensor, slot_mapping: torch.Tensor, key: torc
     float32, bfloat16 or float16, any strides that give every element a place of its own, a
     contiguous last dimension) become what ``cache`` holds at ``slot_mapping[t]`` (int64 [T], in
     any order), and 0 for a slot that is negative or past the pool."""
-    num_blocks, num_heads, block_size, dtype, index = _check_4bit_rows(key, value, cache,
-                                                                       slot_mapping)
-    for t in (key, value):
-        if any(step == 0 and size > 1 for step, size in zip(t.stride(), t.shape)):
-            raise ValueError("key and value are written: expanded tensors do not do")
+    (tokens, heads, dim), num_blocks, block_size, st, dtype, index = _check_4bit_rows(
+        key, value, cache, slot_mapping)
+    if (tokens > 1 and not (st[0] and st[3])) or (heads > 1 and not (st[1] and st[4])):
+        raise ValueError("key and value are written: expanded tensors do not do")
     if key.requires_grad or value.requires_grad:
         refuse_gradients("gather_cache_4bit")
     slot_mapping = slot_mapping.contiguous()
     on_device(index, lib.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(),
-              key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0),
-              value.stride(1), key.shape[0], num_heads, key.shape[2], block_size, num_blocks,
-              dtype)
+              key.data_ptr(), value.data_ptr(), st[0], st[1], st[3], st[4], tokens, heads, dim,
+              block_size, num_blocks, dtype)
     torch.autograd.graph.increment_version((key, value))  # autograd's check of saved tensors
 
 
@@ -1147,24 +1157,26 @@ def attention_with_kv_cache_4bit(query: torch.Tensor, cache: torch.Tensor, out: 
     groups (``group_start``, ``group_order``, ``max_group_size``) are used: a group that shares
     its table (and length) is read once for all of its rows, one whose rows keep their own
     tables runs row by row."""
-    if query.dim() != 3 or query.stride(2) != 1:
+    shape = query.shape
+    st = query.stride()
+    if len(shape) != 3 or st[2] != 1:
         raise ValueError("query must be [N, H, D] with a contiguous last dimension, got "
                          f"{tuple(query.shape)}")
-    num_rows, num_heads, head_dim = query.shape
-    num_blocks, cache_heads, block_size, _ = _check_4bit_cache(cache, head_dim)
+    num_rows, num_heads, head_dim = shape
+    num_blocks, cache_heads, block_size = _check_4bit_cache(cache, head_dim)
     if cache_heads != num_heads:
         raise ValueError(f"query has {num_heads} heads, the cache {cache_heads}")
     dtype = _dtype_code(query.dtype)
-    block_table, seq_lens = _check_paged_rows(query, out, seq_lens, block_table, cache)
+    block_table, seq_lens, index = _check_paged_rows(query, out, seq_lens, block_table, cache)
     if query.requires_grad or out.requires_grad:
         refuse_gradients("attention_with_kv_cache_4bit")
-    index, width = query.get_device(), block_table.shape[1]
-    start, order, num_groups, most = _shared_groups(scheduler_metadata, query, block_size)
+    width, table_step = block_table.shape[1], block_table.stride(0)
+    start, order, num_groups, most = _shared_groups(scheduler_metadata, shape, index, block_size)
     need = _attention_4bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    on_device(index, lib.vfl_attention_with_kv_cache_4bit, query.data_ptr(), query.stride(0),
-              query.stride(1), cache.data_ptr(), out.data_ptr(), seq_lens.data_ptr(),
-              block_table.data_ptr(), block_table.stride(0) if num_rows > 1 else width, width,
+    on_device(index, lib.vfl_attention_with_kv_cache_4bit, query.data_ptr(), st[0], st[1],
+              cache.data_ptr(), out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(),
+              table_step if num_rows > 1 else width, width,
               None if start is None else start.data_ptr(),
               None if order is None else order.data_ptr(), num_rows, num_groups, most, num_heads,
               head_dim, block_size, num_blocks, float(scale), dtype,
@@ -1176,20 +1188,12 @@ def attention_with_kv_cache_4bit(query: torch.Tensor, cache: torch.Tensor, out: 
 # cross-attention of packed runs
 # ---------------------------------------------------------------------------
 CROSS_HEAD_DIMS = frozenset(d for d in SUPPORTED_HEAD_DIMS if d <= 256)
+CROSS_MAX_STRIDE = 1 << 22  # elements from a key to the next
 
 
 @functools.lru_cache(maxsize=4096)
 def _cross_workspace(*sizes: int) -> int:
     return lib.vfl_packed_cross_attention_workspace(*sizes)
-
-
-def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` ([T, H, D], unit last stride) where each head's row is 16-byte aligned and 2^22
-    elements or less from the next token's, or a copy."""
-    token, head, _ = x.stride()
-    if (x.data_ptr() | (token | head) * x.element_size()) & 15 or token > 1 << 22:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
 
 
 def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -1207,24 +1211,25 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     the sequences are written, 0 where one has no keys; rows of none are left as they were.
     ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch and
     change no result."""
-    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape \
-            or query.shape[1:] != key.shape[1:]:
+    rows, keys = query.shape, key.shape
+    if len(rows) != 3 or len(keys) != 3 or value.shape != keys or rows[1:] != keys[1:]:
         raise ValueError("query must be [T, H, D], key and value [S, H, D], got "
-                         f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
-    num_queries, num_heads, head_dim = query.shape
+                         f"{tuple(rows)}, {tuple(keys)}, {tuple(value.shape)}")
+    num_queries, num_heads, head_dim = rows
     if head_dim not in CROSS_HEAD_DIMS:
         raise ValueError(f"head_dim {head_dim} has no kernel; supported: "
                          f"{sorted(CROSS_HEAD_DIMS)}")
     if not query.dtype == key.dtype == value.dtype == out.dtype:
         raise ValueError("query, key, value and out must share one dtype")
     dtype = _dtype_code(query.dtype)
-    if query.stride(2) != 1 or key.stride(2) != 1 or value.stride(2) != 1:
+    q_st, k_st, v_st = query.stride(), key.stride(), value.stride()
+    if q_st[2] != 1 or k_st[2] != 1 or v_st[2] != 1:
         raise ValueError("query, key and value need a contiguous last dimension")
-    if out.shape != query.shape or not out.is_contiguous():
+    if out.shape != rows or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of query's shape")
-    if (query_start_loc.dtype != torch.int32 or query_start_loc.dim() != 1
-            or query_start_loc.numel() < 1 or key_start_loc.dtype != torch.int32
-            or key_start_loc.shape != query_start_loc.shape):
+    starts = query_start_loc.shape
+    if (query_start_loc.dtype != torch.int32 or len(starts) != 1 or not starts[0]
+            or key_start_loc.dtype != torch.int32 or key_start_loc.shape != starts):
         raise ValueError("query_start_loc and key_start_loc must be int32 [sequences + 1], got "
                          f"{query_start_loc.dtype} {tuple(query_start_loc.shape)}, "
                          f"{key_start_loc.dtype} {tuple(key_start_loc.shape)}")
@@ -1234,17 +1239,21 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     index = one_gpu(query, key, value, out, query_start_loc, key_start_loc)
     if (query.requires_grad or key.requires_grad or value.requires_grad or out.requires_grad):
         refuse_gradients("packed_cross_attention")
-    # the kernel reads 16 bytes at a time; rows that do not allow it are copied
-    query, key, value = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
+    q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    # the kernel reads 16 bytes at a time: rows that do not allow it are copied
+    steps = (q_st[0] | q_st[1] | k_st[0] | k_st[1] | v_st[0] | v_st[1]) * query.element_size()
+    if (q | k | v | steps) & 15 or k_st[0] > CROSS_MAX_STRIDE or v_st[0] > CROSS_MAX_STRIDE:
+        query, key, value = (x.clone(memory_format=torch.contiguous_format)
+                             for x in (query, key, value))
+        q_st, k_st, v_st = query.stride(), key.stride(), value.stride()
+        q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
     query_start_loc, key_start_loc = query_start_loc.contiguous(), key_start_loc.contiguous()
-    sequences = query_start_loc.numel() - 1
-    longest = (min(max_query_len, num_queries), min(max_key_len, key.shape[0]))
-    need = _cross_workspace(num_queries, sequences, num_heads, head_dim, *longest, dtype)
+    longest = (min(max_query_len, num_queries), min(max_key_len, keys[0]))
+    need = _cross_workspace(num_queries, starts[0] - 1, num_heads, head_dim, *longest, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    on_device(index, lib.vfl_packed_cross_attention, query.data_ptr(), query.stride(0),
-              query.stride(1), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
-              value.stride(0), value.stride(1), out.data_ptr(), query_start_loc.data_ptr(),
-              key_start_loc.data_ptr(), num_queries, key.shape[0], sequences, num_heads, head_dim,
+    on_device(index, lib.vfl_packed_cross_attention, q, q_st[0], q_st[1], k, k_st[0], k_st[1], v,
+              v_st[0], v_st[1], out.data_ptr(), query_start_loc.data_ptr(),
+              key_start_loc.data_ptr(), num_queries, keys[0], starts[0] - 1, num_heads, head_dim,
               *longest, float(scale), dtype, workspace.data_ptr() if need else None)
     torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
 
