@@ -264,3 +264,26 @@ def test_c_entries_refuse():
     assert cross(queries=0) == 0 and cross(sequences=0) == 0
     assert lib.vfl_packed_cross_attention_workspace(5, 2, 2, 64, 3, 100000, VFL_FLOAT32) > 0
     assert lib.vfl_packed_cross_attention_workspace(5, 2, 2, 64, 3, 4, VFL_FLOAT32) == 0
+
+
+def test_entry_callables():
+    """The extension module's callables convert as the entries' types ask, and reach the same
+    library: its message is the one that the other binding reads."""
+    from vflorence_amd._lib import VFL_BFLOAT16, calls, lib
+
+    args = [A, A, 128, 64, 128, 64, A, A, 0, 2, 64, 16, 8, VFL_BFLOAT16, None]
+    call = calls.vfl_reshape_and_cache_4bit
+    assert call(*args) == 0
+    assert call(*args[:10], 40, *args[11:]) == lib.vfl_reshape_and_cache_4bit(
+        *args[:10], 40, *args[11:]) != 0
+    lib.vfl_reshape_and_cache_4bit(*args)  # clears the message
+    assert call(*args[:13], 9, None) != 0 and "dtype code 9" in _message()
+    for bad, error in ((args[:-1], TypeError), (args + [0], TypeError),
+                       (["x", *args[1:]], TypeError), ([-1, *args[1:]], OverflowError),
+                       ([*args[:9], 1 << 31, *args[10:]], OverflowError),
+                       ([*args[:2], 1 << 63, *args[3:]], OverflowError),
+                       ([*args[:2], 1.5, *args[3:]], TypeError)):
+        with pytest.raises(error):
+            call(*bad)
+    with pytest.raises(TypeError):
+        calls.vfl_packed_cross_attention(*[A] * 19, "scale", 1, None, None)

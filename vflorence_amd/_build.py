@@ -1,5 +1,6 @@
-"""In-tree builds (no cmake): libvflorence_amd.so for gfx950 (hipcc) and the engine's
-native host core libvfl_host.so (g++, CPU only).
+"""In-tree builds (no cmake): libvflorence_amd.so for gfx950 (hipcc), the Python callables over
+some of its entries (_calls.so, g++) and the engine's native host core libvfl_host.so (g++, CPU
+only).
 
     python -m vflorence_amd._build          # or __graft_entry__.build()
 
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -54,20 +56,37 @@ HOST_OUTPUT = os.path.join(HERE, "libvfl_host.so")
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra", "-Werror"]
 
 
-def build_host_library(verbose: bool = False) -> str:
-    """Compile the engine's host core into HOST_OUTPUT; always recompiles."""
+def _build_host(output: str, sources, flags, verbose: bool) -> str:
     cxx = shutil.which("g++") or shutil.which("c++")
     if not cxx:
-        raise RuntimeError("g++ not found; the engine's host core cannot be built")
-    tmp = HOST_OUTPUT + ".tmp"
-    cmd = [cxx, *HOST_FLAGS, *[os.path.join(CSRC, s) for s in HOST_SOURCES], "-o", tmp]
+        raise RuntimeError(f"g++ not found; {os.path.basename(output)} cannot be built")
+    tmp = output + ".tmp"
+    cmd = [cxx, *HOST_FLAGS, *[os.path.join(CSRC, s) for s in sources], "-o", tmp, *flags]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("g++ failed:\n" + proc.stdout + proc.stderr)
-    os.replace(tmp, HOST_OUTPUT)
-    return HOST_OUTPUT
+    os.replace(tmp, output)
+    return output
+
+
+def build_host_library(verbose: bool = False) -> str:
+    """Compile the engine's host core into HOST_OUTPUT; always recompiles."""
+    return _build_host(HOST_OUTPUT, HOST_SOURCES, (), verbose)
+
+
+CALLS_SOURCES = ("host/entry_calls.cpp",)
+CALLS_OUTPUT = os.path.join(HERE, "_calls.so")
+
+
+def build_calls(verbose: bool = False) -> str:
+    """Compile the Python callables over OUTPUT's entries into CALLS_OUTPUT; always recompiles.
+    OUTPUT has to be built: they are linked with it, and find it beside them."""
+    return _build_host(CALLS_OUTPUT, CALLS_SOURCES,
+                       (f"-I{sysconfig.get_paths()['include']}", f"-L{HERE}",
+                        f"-l:{os.path.basename(OUTPUT)}", "-Wl,-rpath,$ORIGIN",
+                        "-Wl,--allow-shlib-undefined"), verbose)
 
 
 def build_library(verbose: bool = False) -> str:
@@ -111,4 +130,5 @@ def build_library(verbose: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build_library(verbose="-v" in sys.argv))
+    print(build_calls(verbose="-v" in sys.argv))
     print(build_host_library(verbose="-v" in sys.argv))

@@ -225,6 +225,26 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
+def _load_calls():
+    """The entries whose wrappers are called per step, as callables of an extension module
+    (linked with the library above): the same arguments and status as through ``lib``."""
+    import importlib.machinery
+    import importlib.util
+
+    path = os.path.join(os.path.dirname(LIB_PATH), "_calls.so")
+    if not os.path.exists(path):
+        raise LibraryMissing(f"{path} is not built; run "
+                             "`python -c 'import __graft_entry__ as g; g.build()'`")
+    name = __package__ + "._calls"
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(module)
+    return module
+
+
+calls = _load_calls()
+
+
 class HipAttnError(RuntimeError):
     """A C-ABI call returned an error status (the library's TORCH_CHECK equivalent)."""
 

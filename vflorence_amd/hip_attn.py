@@ -22,7 +22,7 @@ from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
 
 from . import _lib
-from ._lib import SchedMeta, check, lib
+from ._lib import SchedMeta, calls, check, lib
 
 _DTYPE_CODES = {
     torch.float32: _lib.VFL_FLOAT32,
@@ -1113,7 +1113,7 @@ def reshape_and_cache_4bit(key: torch.Tensor, value: torch.Tensor, cache: torch.
     if key.requires_grad or value.requires_grad:
         refuse_gradients("reshape_and_cache_4bit")
     slot_mapping = slot_mapping.contiguous()
-    on_device(index, lib.vfl_reshape_and_cache_4bit, key.data_ptr(), value.data_ptr(), st[0],
+    on_device(index, calls.vfl_reshape_and_cache_4bit, key.data_ptr(), value.data_ptr(), st[0],
               st[1], st[3], st[4], cache.data_ptr(), slot_mapping.data_ptr(), tokens, heads, dim,
               block_size, num_blocks, dtype)
     torch.autograd.graph.increment_version((cache,))  # autograd's check of saved tensors
@@ -1132,7 +1132,7 @@ def gather_cache_4bit(cache: torch.Tensor, slot_mapping: torch.Tensor, key: torc
     if key.requires_grad or value.requires_grad:
         refuse_gradients("gather_cache_4bit")
     slot_mapping = slot_mapping.contiguous()
-    on_device(index, lib.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(),
+    on_device(index, calls.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(),
               key.data_ptr(), value.data_ptr(), st[0], st[1], st[3], st[4], tokens, heads, dim,
               block_size, num_blocks, dtype)
     torch.autograd.graph.increment_version((key, value))  # autograd's check of saved tensors
@@ -1174,7 +1174,7 @@ def attention_with_kv_cache_4bit(query: torch.Tensor, cache: torch.Tensor, out: 
     start, order, num_groups, most = _shared_groups(scheduler_metadata, shape, index, block_size)
     need = _attention_4bit_workspace(num_rows, num_groups, num_heads, head_dim, block_size, width)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    on_device(index, lib.vfl_attention_with_kv_cache_4bit, query.data_ptr(), st[0], st[1],
+    on_device(index, calls.vfl_attention_with_kv_cache_4bit, query.data_ptr(), st[0], st[1],
               cache.data_ptr(), out.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(),
               table_step if num_rows > 1 else width, width,
               None if start is None else start.data_ptr(),
@@ -1251,7 +1251,7 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     longest = (min(max_query_len, num_queries), min(max_key_len, keys[0]))
     need = _cross_workspace(num_queries, starts[0] - 1, num_heads, head_dim, *longest, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    on_device(index, lib.vfl_packed_cross_attention, q, q_st[0], q_st[1], k, k_st[0], k_st[1], v,
+    on_device(index, calls.vfl_packed_cross_attention, q, q_st[0], q_st[1], k, k_st[0], k_st[1], v,
               v_st[0], v_st[1], out.data_ptr(), query_start_loc.data_ptr(),
               key_start_loc.data_ptr(), num_queries, keys[0], starts[0] - 1, num_heads, head_dim,
               *longest, float(scale), dtype, workspace.data_ptr() if need else None)
