@@ -118,9 +118,11 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
   int64_t pos;
   int h;
   xcd_position(blockIdx.x, (unsigned)H, pos, h);
-  const int split = (int)(pos % a.splits);
+  // (a launch has fewer than 2^32 threads: positions divide in 32 bits)
+  const unsigned parts = (unsigned)a.splits, place = (unsigned)pos / parts;
+  const int split = (int)((unsigned)pos - place * parts);
   int64_t row0;
-  const int nrows = group_rows(a, pos / a.splits, row0);
+  const int nrows = group_rows(a, place, row0);
   if (nrows <= 0) return;
 
   const int first = split * NW + wave, step = a.splits * NW;

@@ -8,7 +8,8 @@
 // them (half-wave hf of step s holds keys 16 s + 4 hf + 0..3 and 16 s + 8 + 4 hf + 0..3).  V lies
 // in LDS as it came, key by key, and is turned by the transposing reads.
 //
-// 16-bit inputs go in as they are, the weights rounded to that type (fp16's times 2^7, which keeps
+// 16-bit inputs go in as they are, the weights rounded to that type, in launches of few queries in
+// two terms of it (fp16's times 2^7, which keeps
 // those down to 2^-21 of the reference clear of its subnormals; the others' times 2^-20).  fp32 goes in as three bf16 terms
 // each, rounded, of whose nine products the six largest are taken: the others are 2^-26 of the whole
 // or less.
@@ -109,6 +110,14 @@ template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float c)
                                            __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
 }
 
+// A term of four weights, rounded, with the remainder left in f.
+template <int DT> __device__ __forceinline__ uint2 take_weights(float (&f)[4]) {
+  const uint2 w = make_uint2(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]));
+  f[0] -= Mfma<DT>::widen_lo(w.x), f[1] -= Mfma<DT>::widen_hi(w.x);
+  f[2] -= Mfma<DT>::widen_lo(w.y), f[3] -= Mfma<DT>::widen_hi(w.y);
+  return w;
+}
+
 // Of 16 lanes, lane 4 i + c points to 4 elements of row i; lane n gets the four rows' element n
 // of the 16 that the lanes point to.
 __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
@@ -121,7 +130,9 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
 constexpr int WAVES = 4;
 template <int DT, int DG, int KS> struct CrossShape {
   static constexpr bool F32 = DT == VFL_FLOAT32;
-  static constexpr int PLANES = F32 ? 3 : 1;   // bf16 terms
+  static constexpr int PLANES = F32 ? 3 : 1;   // bf16 terms of queries, keys and values
+  // terms of a weight: two where products cost little, in launches of few queries
+  static constexpr int TERMS = F32 ? 3 : KS > 1 ? 2 : 1;
   static constexpr int KT = DG > 1 && (F32 || DG > 4 || (DG > 2 && KS > 1)) ? 32 : 64;  // keys of a tile
   static constexpr int STRIDE = DG * 64 + 16;  // bytes of a tile's row: rows on different banks
   static constexpr int PLANE = KT * STRIDE;
@@ -354,7 +365,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
         return s;
       };
       // a lane's weights as the second product takes them, and their sum as it sees them
-      uint4 pop[2][PLANES];
+      uint4 pop[2][S::TERMS];
       float sum;
       auto take = [&](floatx16_t &s) {
         sum = 0.f;
@@ -369,6 +380,14 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
 #pragma unroll
             for (int t = 0; t < PLANES; ++t) {
               const uint2 lo = take_bf16<true>(p0), hi = take_bf16<true>(p1);
+              pop[st][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+          } else if constexpr (S::TERMS == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += p0[i] + p1[i];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint2 lo = take_weights<DT>(p0), hi = take_weights<DT>(p1);
               pop[st][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
           } else {
@@ -387,7 +406,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
       // rounded by is the same for every weight of the row), two where it does not: by row, so that
       // none hangs on its neighbours.
       auto weights = [&](floatx16_t &s) {
-        if (!wide) {
+        if (__builtin_expect(!wide, 1)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale_log2, -ms));
         } else {
@@ -401,11 +420,11 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
         }
         take(s);
       };
-      if (!fresh) {
+      if (__builtin_expect(!fresh, 1)) {
         floatx16_t s = scores();
         weights(s);
       }
-      if (fresh || __builtin_amdgcn_ballot_w64(!(sum <= MOST_SUM)) != 0) {
+      if (__builtin_expect(fresh || __builtin_amdgcn_ballot_w64(!(sum <= MOST_SUM)) != 0, 0)) {
         // rows whose own sums pass the slack move, whatever stands beside them
         bool need = true;
         if (!fresh) {
@@ -451,7 +470,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
             const uint2 v1 = read_turned(vp + p * S::PLANE + 64 * d + 8 * STRIDE);
             const uint4 vop = make_uint4(v0.x, v0.y, v1.x, v1.y);
 #pragma unroll
-            for (int t = PLANES - 1 - p; t >= 0; --t) o[d] = mfma32<MDT>(vop, pop[st][t], o[d]);
+            for (int t = S::TERMS - 1 - p; t >= 0; --t) o[d] = mfma32<MDT>(vop, pop[st][t], o[d]);
           }
         }
       }

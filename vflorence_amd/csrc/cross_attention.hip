@@ -21,8 +21,8 @@ struct CrossPlan {
 //   / 48.1, but 64 of 20 to 32 110 / 128 / 120, 16 of 31 to 257 67.8 / 86.4 / 116.
 // - runs of keys are split where that leaves no more workgroups than two a CU (fp32: one): 8 runs
 //   of 20 to 32 queries over 1000 to 2000 keys whole 22.9, in four parts 17.9, in eight 20.7; fp32 4
-//   of 60 to 64 whole 63.6, in four 26.6, in eight 30.4; more than 16 parts cost the join more
-//   (2 runs of 17 and 33 over 17001 and 39999 keys, fp16, 8 heads of 128: 16 parts 45.4, 32 49.6).
+//   of 60 to 64 whole 63.6, in four 26.6, in eight 30.4; 60 queries x 8 heads of 128 over 30000 keys
+//   in 16 parts 48.0, in 32 35.5 (21 and 29 over 17001 and 39999 57.6 / 58.0).
 // - launches of up to two workgroups a CU go to any XCD: 12 heads, fp32, 590 queries in two parts
 //   21.2, a head to an XCD 33.6.
 CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool f32,
@@ -43,7 +43,7 @@ CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool 
   const int64_t wgs = workgroups(p.ks);
   const int64_t fill = (f32 ? 256 : 512) / wgs, parts = max_keys / (f32 ? 64 : 256 * p.ks);
   const int64_t most_parts = fill < parts ? fill : parts;
-  if (most_parts >= 2) p.splits = most_parts < 16 ? (int)most_parts : 16;
+  if (most_parts >= 2) p.splits = most_parts < 32 ? (int)most_parts : 32;
   p.spread = wgs * p.splits <= 512;
   return p;
 }
