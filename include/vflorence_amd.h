@@ -635,8 +635,9 @@ int vfl_attention_with_kv_cache_4bit(const void *query, int64_t query_stride_tok
  * [num_sequences + 1], rising; they are limited to the rows there are).  Rows of no sequence are
  * neither read nor written; queries without keys get 0.  query [num_queries], key and value
  * [num_keys] rows of num_heads x head_dim, 16-byte aligned with strides that are multiples of 16
- * bytes; out contiguous, query itself or apart from it, apart from key and value.  head_dim up to 256; scale finite.  Sums and softmax in fp32,
- * the weights rounded to the type for the second product (fp32: kept to 2^-24).
+ * bytes; out contiguous, query itself or apart from it, apart from key and value.  head_dim up to
+ * 256; scale finite.  Sums and softmax in fp32, the weights rounded to the type for the second
+ * product (fp32: kept to 2^-24).
  * max_query_len and max_key_len, the longest runs expected, shape the launch (longer ones are
  * served too).  workspace as above, of vfl_packed_cross_attention_workspace bytes.
  */

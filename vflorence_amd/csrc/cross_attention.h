@@ -8,11 +8,29 @@
 // them (half-wave hf of step s holds keys 16 s + 4 hf + 0..3 and 16 s + 8 + 4 hf + 0..3).  V lies
 // in LDS as it came, key by key, and is turned by the transposing reads.
 //
-// 16-bit inputs go in as they are, the weights rounded to that type, in launches of few queries in
-// two terms of it (fp16's times 2^7, which keeps
-// those down to 2^-21 of the reference clear of its subnormals; the others' times 2^-20).  fp32 goes in as three bf16 terms
-// each, rounded, of whose nine products the six largest are taken: the others are 2^-26 of the whole
-// or less.
+// 16-bit inputs go in as they are, the weights rounded to that type (fp16's times 2^7, which
+// keeps those down to 2^-21 of the reference clear of its subnormals; the others' times 2^-20).
+// Their sum is that of the rounded weights, so an output's error is up to about 1.4 of its own
+// rounding's, two errors of a size.  A second term of a weight would take that away, at 2 to 16%
+// (8 runs of 60 to 128 queries 13.5 / 15.7 us, 21 and 29 over 17001 and 39999 keys 48.9 / 50.3).
+// fp32 goes in as three bf16 terms each, rounded, of whose nine products the six largest are taken:
+// the others are 2^-26 of the whole or less.
+//
+// What bounds it: long texts the vector and matrix units together (64 texts of 128 to 1024 tokens
+// over 256 to 1024, 16 heads of 64, bf16: 161 us, 94 GFLOP, 585 TFLOP/s of a large matrix product's
+// 1205; vector units busy for 65 us, matrix units for 40, at 2.4 GHz, in three waves a SIMD.  Copies
+// that left work out: without loading tiles 134, nor storing them 118, nor exponentials 108).  fp32
+// its six products (4 texts of 1024 over 1024 105 us, 980 TFLOP/s of bf16 products; 16 of 31 to 257
+// over 256 to 1024, whose workgroups are one round of unequal length, 65).  Few queries HBM: 64
+// single tokens over 256 to 1024 keys 35 us, 4.8 TB/s; 21 and 29 over 17001 and 39999, heads of 128,
+// fp16, 56 us, 4.1 TB/s (46 to 49 where the last call left some of the keys in the cache).
+// What the steps gave, us, these long texts / fp32 / long keys in the cache / 9 over 590:
+//   loads under conditions, maxima for every tile               242 / 88 / 61 / 12.4
+//   no conditions, 32 keys at a time                            197 / 77 / 54
+//   the last tile apart                                         175 / 71 / 50
+//   workgroups found by the rows' offsets, no empty ones        168 / 72 / 49 / 9.1
+//   weights about the references as they stand                  163 / 67
+//   parts, groups and XCDs by the launch's size                 160 / 65 / 46 / 8.7
 #pragma once
 
 #include <math.h>
@@ -110,14 +128,6 @@ template <int DT> __device__ __forceinline__ float add_pair(uint32_t w, float c)
                                            __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
 }
 
-// A term of four weights, rounded, with the remainder left in f.
-template <int DT> __device__ __forceinline__ uint2 take_weights(float (&f)[4]) {
-  const uint2 w = make_uint2(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]));
-  f[0] -= Mfma<DT>::widen_lo(w.x), f[1] -= Mfma<DT>::widen_hi(w.x);
-  f[2] -= Mfma<DT>::widen_lo(w.y), f[3] -= Mfma<DT>::widen_hi(w.y);
-  return w;
-}
-
 // Of 16 lanes, lane 4 i + c points to 4 elements of row i; lane n gets the four rows' element n
 // of the 16 that the lanes point to.
 __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
@@ -130,9 +140,7 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
 constexpr int WAVES = 4;
 template <int DT, int DG, int KS> struct CrossShape {
   static constexpr bool F32 = DT == VFL_FLOAT32;
-  static constexpr int PLANES = F32 ? 3 : 1;   // bf16 terms of queries, keys and values
-  // terms of a weight: two where products cost little, in launches of few queries
-  static constexpr int TERMS = F32 ? 3 : KS > 1 ? 2 : 1;
+  static constexpr int PLANES = F32 ? 3 : 1;   // bf16 terms
   static constexpr int KT = DG > 1 && (F32 || DG > 4 || (DG > 2 && KS > 1)) ? 32 : 64;  // keys of a tile
   static constexpr int STRIDE = DG * 64 + 16;  // bytes of a tile's row: rows on different banks
   static constexpr int PLANE = KT * STRIDE;
@@ -144,7 +152,8 @@ template <int DT, int DG, int KS> struct CrossShape {
   static constexpr int GT = 64 * GW;           // threads of a key group
   static constexpr int PIECES = KT * DG * 4;   // of 8 elements, of K or V
   static constexpr int CH = (PIECES + GT - 1) / GT;  // a thread's
-  static constexpr int OCC = !F32 && DG <= 2 && KS == 1 ? 3 : 1;  // waves of a SIMD at least
+  // waves of a SIMD at least: three of heads of up to 64 (long texts 162 us; four, which spill, 173)
+  static constexpr int OCC = !F32 && DG <= 2 && KS == 1 ? 3 : 1;
   static_assert(BUFS * KS * TILE <= 160 * 1024, "the tiles fit the LDS");
 };
 
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
         return s;
       };
       // a lane's weights as the second product takes them, and their sum as it sees them
-      uint4 pop[2][S::TERMS];
+      uint4 pop[2][PLANES];
       float sum;
       auto take = [&](floatx16_t &s) {
         sum = 0.f;
@@ -380,14 +389,6 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
 #pragma unroll
             for (int t = 0; t < PLANES; ++t) {
               const uint2 lo = take_bf16<true>(p0), hi = take_bf16<true>(p1);
-              pop[st][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
-          } else if constexpr (S::TERMS == 2) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += p0[i] + p1[i];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              const uint2 lo = take_weights<DT>(p0), hi = take_weights<DT>(p1);
               pop[st][t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
           } else {
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
             const uint2 v1 = read_turned(vp + p * S::PLANE + 64 * d + 8 * STRIDE);
             const uint4 vop = make_uint4(v0.x, v0.y, v1.x, v1.y);
 #pragma unroll
-            for (int t = S::TERMS - 1 - p; t >= 0; --t) o[d] = mfma32<MDT>(vop, pop[st][t], o[d]);
+            for (int t = PLANES - 1 - p; t >= 0; --t) o[d] = mfma32<MDT>(vop, pop[st][t], o[d]);
           }
         }
       }
@@ -622,8 +623,8 @@ __device__ __forceinline__ bool in_sequence(const CrossArgs &a, int row) {
 }
 
 // The splits of each (query, head) joined: of many a workgroup takes one (query, head), of few a
-// thread four dims.  (50 queries x 8 heads of 128 in 32 parts, with the attention: 43 / 55 us;
-// 590 x 12 of 64 in two 26 / 21.)
+// thread four dims.  (With the attention, us: 60 queries x 8 heads of 128 in 32 parts 31.3 / 45.0, 8
+// runs of 20 to 32 x 16 of 64 in four 21.9 / 20.0, 590 x 12 in two, fp32, 25.6 / 20.7.)
 constexpr int CROSS_JOIN_NT = 256;
 constexpr int CROSS_JOIN_FEW = 8;
 template <int DT> __global__ __launch_bounds__(JOIN_NT) void cross_join_many_kernel(CrossArgs a) {
