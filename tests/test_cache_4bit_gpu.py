@@ -199,6 +199,16 @@ def test_gather_refuses_expanded_rows():
         hip_attn.gather_cache_4bit(cache, slots, out, out[:1].expand(3, 2, 64))
 
 
+def test_gather_refuses_one_tensor_for_both():
+    from vflorence_amd import hip_attn
+
+    cache = hip_attn.kv_cache_4bit(2, 2, 16, 64, DEV)
+    out = torch.zeros(3, 2, 64, device=DEV)
+    slots = torch.zeros(3, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="memory of their own"):
+        hip_attn.gather_cache_4bit(cache, slots, out, out)
+
+
 def test_gather_any_slots():
     """Repeated, skipped and unordered slots; nothing at all; an empty pool."""
     gen = torch.Generator().manual_seed(8)

@@ -264,6 +264,12 @@ def test_c_entries_refuse():
     assert cross(queries=0) == 0 and cross(sequences=0) == 0
     assert lib.vfl_packed_cross_attention_workspace(5, 2, 2, 64, 3, 100000, VFL_FLOAT32) > 0
     assert lib.vfl_packed_cross_attention_workspace(5, 2, 2, 64, 3, 4, VFL_FLOAT32) == 0
+    assert cross(queries=(1 << 31) - 1) != 0 and cross(keys=(1 << 31) - 1) != 0
+    # rows of no sequence take no more than a bounded workspace: two parts of 2^15 rows x 8 heads
+    # would be 2 * 2^18 * (64 * 4 + 8) = 138.4 MB, more than 2^27
+    for rows in (9, 1000, 1 << 15, 1 << 20, 1 << 31, 1 << 62):
+        need = lib.vfl_packed_cross_attention_workspace(rows, 1, 8, 64, 9, 40000, VFL_BFLOAT16)
+        assert (need > 0) == (rows < 1 << 15) and need <= 1 << 27
 
 
 def test_entry_callables():

@@ -105,6 +105,20 @@ def test_rows_of_no_sequence_are_left_alone():
             assert bool((out[:4] == 5).all()) and bool((out[77:] == 5).all())
 
 
+@pytest.mark.parametrize("rows", [40000, 300000, 700000])
+def test_few_queries_among_many_rows(rows):
+    """A padded call: the keys are split over as many parts as its rows leave memory for."""
+    gen = torch.Generator().manual_seed(rows)
+    q, k, v = inputs(gen, [rows], [5000, 1200], 1, 32, torch.bfloat16)
+    first = rows - 40
+    out = run(q, k, v, [first, first + 9, first + 30], [0, 5000, 6200], 0.2)
+    found = cross(q[first:], k, v, [0, 9, 30], [0, 5000, 6200], 0.2)
+    limit = cross_tolerance(q.dtype, 32, 5000, *found)
+    error = (out[first:].double().cpu() - found[0]).abs()[:30]
+    assert bool((error <= limit[:30]).all())
+    assert bool((out[:first] == 5.0).all()) and bool((out[first + 30:] == 5.0).all())
+
+
 def test_offsets_past_the_rows_are_limited():
     """Starts outside the tensors, falling ones, no sequences, no rows, no keys at all."""
     gen = torch.Generator().manual_seed(10)

@@ -2,6 +2,8 @@
 // are cross_attention.h's).
 #include "cross_attention.h"
 
+#include <algorithm>
+
 namespace vfl {
 
 namespace {
@@ -22,12 +24,18 @@ struct CrossPlan {
 // - runs of keys are split where that leaves no more workgroups than two a CU (fp32: one): 8 runs
 //   of 20 to 32 queries over 1000 to 2000 keys whole 22.9, in four parts 17.9, in eight 20.7; fp32 4
 //   of 60 to 64 whole 63.6, in four 26.6, in eight 30.4; 60 queries x 8 heads of 128 over 30000 keys
-//   in 16 parts 48.0, in 32 35.5 (21 and 29 over 17001 and 39999 57.6 / 58.0).
+//   in 16 parts 48.0, in 32 35.5 (21 and 29 over 17001 and 39999 57.6 / 58.0).  A call's rows all take
+//   a place for each part, also those of no sequence: parts that would need more than 128 MB, twice
+//   what a launch's own queries ever take, are not made.
 // - launches of up to two workgroups a CU go to any XCD: 12 heads, fp32, 590 queries in two parts
 //   21.2, a head to an XCD 33.6.
+constexpr int64_t MOST_ROWS = 2147483647LL - 1024;  // (a tile past the last is counted in 32 bits)
+constexpr int64_t CROSS_MOST_WORKSPACE = 1LL << 27;
+
 CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool f32,
                      int64_t max_queries, int64_t max_keys) {
   const int DG = (D + 31) / 32;
+  max_queries = std::min(max_queries, num_queries);
   CrossPlan p{1, 1, false};
   auto workgroups = [&](int ks) {  // that hold queries, at most
     const int64_t qt = 128 / ks, tiles = (max_queries + qt - 1) / qt;
@@ -42,8 +50,9 @@ CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool 
   while (p.ks > 1 && 64 * (p.ks / 2) >= max_keys) p.ks /= 2;
   const int64_t wgs = workgroups(p.ks);
   const int64_t fill = (f32 ? 256 : 512) / wgs, parts = max_keys / (f32 ? 64 : 256 * p.ks);
-  const int64_t most_parts = fill < parts ? fill : parts;
-  if (most_parts >= 2) p.splits = most_parts < 32 ? (int)most_parts : 32;
+  const int64_t room = CROSS_MOST_WORKSPACE / (num_queries * H * split_part_bytes(D));
+  const int64_t most_parts = std::min({fill, parts, room, (int64_t)32});
+  if (most_parts >= 2) p.splits = (int)most_parts;
   p.spread = wgs * p.splits <= 512;
   return p;
 }
@@ -58,7 +67,10 @@ extern "C" int64_t vfl_packed_cross_attention_workspace(int64_t num_queries, int
                                                         int num_heads, int head_dim,
                                                         int64_t max_query_len,
                                                         int64_t max_key_len, int dtype) {
-  if (num_queries <= 0 || num_sequences <= 0 || num_heads <= 0 || head_dim <= 0) return 0;
+  if (num_queries <= 0 || num_sequences <= 0 || num_heads <= 0 || head_dim <= 0 ||
+      num_queries > MOST_ROWS || num_heads > 65535 || num_sequences > MOST_ROWS / num_heads ||
+      head_dim > 256)
+    return 0;  // nothing to do, or refused
   const CrossPlan p = cross_plan(num_queries, num_sequences, num_heads, head_dim,
                                  dtype == VFL_FLOAT32, max_query_len, max_key_len);
   return p.splits > 1 ? num_queries * num_heads * p.splits * split_part_bytes(head_dim) : 0;
@@ -81,7 +93,7 @@ extern "C" int vfl_packed_cross_attention(
     set_error("%s: no kernel for head_dim %d", who, head_dim);
     return VFL_E_UNSUPPORTED;
   }
-  if (num_queries < 0 || num_keys < 0 || num_queries > 2147483647LL || num_keys > 2147483647LL ||
+  if (num_queries < 0 || num_keys < 0 || num_queries > MOST_ROWS || num_keys > MOST_ROWS ||
       num_sequences < 0 || num_heads <= 0 || num_heads > 65535 || max_query_len < 0 ||
       max_key_len < 0 || max_query_len > 2147483647LL || num_sequences > 2147483647LL / num_heads) {
     set_error("%s: bad sizes (queries %lld keys %lld sequences %lld heads %d longest %lld %lld)", who,

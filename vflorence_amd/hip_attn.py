@@ -1122,8 +1122,8 @@ def reshape_and_cache_4bit(key: torch.Tensor, value: torch.Tensor, cache: torch.
 def gather_cache_4bit(cache: torch.Tensor, slot_mapping: torch.Tensor, key: torch.Tensor,
                       value: torch.Tensor) -> None:
     """The way back from ``reshape_and_cache_4bit``: ``key[t]`` and ``value[t]`` ([T, H, D] in
-    float32, bfloat16 or float16, any strides that give every element a place of its own, a
-    contiguous last dimension) become what ``cache`` holds at ``slot_mapping[t]`` (int64 [T], in
+    float32, bfloat16 or float16, any strides that give every element of the two a place of
+    its own, a contiguous last dimension) become what ``cache`` holds at ``slot_mapping[t]`` (int64 [T], in
     any order), and 0 for a slot that is negative or past the pool."""
     (tokens, heads, dim), num_blocks, block_size, st, dtype, index = _check_4bit_rows(
         key, value, cache, slot_mapping)
@@ -1131,10 +1131,12 @@ def gather_cache_4bit(cache: torch.Tensor, slot_mapping: torch.Tensor, key: torc
         raise ValueError("key and value are written: expanded tensors do not do")
     if key.requires_grad or value.requires_grad:
         refuse_gradients("gather_cache_4bit")
+    k, v = key.data_ptr(), value.data_ptr()
+    if k == v and tokens:
+        raise ValueError("key and value are written: they need memory of their own")
     slot_mapping = slot_mapping.contiguous()
-    on_device(index, calls.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(),
-              key.data_ptr(), value.data_ptr(), st[0], st[1], st[3], st[4], tokens, heads, dim,
-              block_size, num_blocks, dtype)
+    on_device(index, calls.vfl_gather_cache_4bit, cache.data_ptr(), slot_mapping.data_ptr(), k, v,
+              st[0], st[1], st[3], st[4], tokens, heads, dim, block_size, num_blocks, dtype)
     torch.autograd.graph.increment_version((key, value))  # autograd's check of saved tensors
 
 
@@ -1207,10 +1209,10 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     head strides, a contiguous last dimension, head sizes up to 256.  Sequence n has queries
     ``query_start_loc[n]`` to ``query_start_loc[n + 1] - 1`` and keys ``key_start_loc[n]`` to
     ``key_start_loc[n + 1] - 1`` (int32 [sequences + 1], rising, on the GPU).  Of ``out``, a
-    contiguous tensor of query's shape and dtype, ``query`` itself or apart from it, the rows of
-    the sequences are written, 0 where one has no keys; rows of none are left as they were.
-    ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch and
-    change no result."""
+    contiguous tensor of query's shape and dtype, ``query`` itself or apart from it, and apart from
+    ``key`` and ``value``, the rows of the sequences are written, 0 where one has no keys; rows of none are left as they were.
+    ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch; longer
+    ones are served too."""
     rows, keys = query.shape, key.shape
     if len(rows) != 3 or len(keys) != 3 or value.shape != keys or rows[1:] != keys[1:]:
         raise ValueError("query must be [T, H, D], key and value [S, H, D], got "
