@@ -319,7 +319,7 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
     };
 
     // the next 64 tokens' loads go out before the current ones are used, but for wide heads, whose
-    // second buffer would not fit the registers
+    // second buffer does not fit the registers (64 rows x 8 heads of 256 29.9 us, with it 39.9)
     constexpr bool AHEAD = G <= 4;
     if (count > 0) {
       Chunk<G> x;
@@ -386,8 +386,9 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
 // workgroup, were the slower ones (2 rows of 17001 and 39999 tokens x 8 heads of 128, us: workgroups
 // of four waves, 4 / 8 / 12 / 16 a CU 18.9 / 17.8 / 19.4 / 20.5, of eight 25.2 / 19.4 / 22.5 / 21.6;
 // one row of 40000 x 16 of 64 16.8 / 14.9 / 15.6 / 15.4).  What is not split takes eight waves where
-// workgroups are few (16 rows of 2000 to 4000 tokens x 16 heads 14.7, four waves 17.6; 1536 workgroups
-// of up to 1000 tokens 18.6, four waves 14.9).
+// there is a workgroup a CU or fewer (eight / four: 16 rows of 2000 to 4000 tokens x 16 heads 14.7 /
+// 17.6, of 400 to 1000 6.3 / 6.1, 32 x 8 heads of 256 15.5 / 16.4; 384 workgroups of 64 dims 8.3 / 8.0,
+// 512 of 128 dims 15.9 / 12.9, of 256 dims 29.9 / 26.9, 1536 of 64 dims 18.6 / 14.9).
 struct Attn4Plan {
   int waves, splits;
 };
@@ -397,7 +398,7 @@ inline Attn4Plan attn4_plan(int64_t num_groups, int H, int D, int64_t max_tokens
   const int64_t fill = 256 * (D <= 256 ? 8 : 4) / (wgs * 4), most = max_tokens / (4 * 128);
   const int64_t parts = fill < most ? fill : most;
   if (parts >= 4) return Attn4Plan{4, (int)parts};
-  return Attn4Plan{D <= 256 && wgs <= (D <= 64 ? 256 : 512) ? 8 : 4, 1};
+  return Attn4Plan{D <= 256 && wgs <= 256 ? 8 : 4, 1};
 }
 
 template <int DT, int G, int ROWS>

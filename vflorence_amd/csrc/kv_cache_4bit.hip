@@ -14,8 +14,9 @@
 // every run.
 //
 // What bounds it: prompts HBM (64 of 256 to 1024 tokens x 16 heads of 64, bf16, written 36.1 us, read
-// back 35.9, on tensors that the last call left in the 256 MB of last-level cache, 46 and 41 on others:
-// 213 MB either way, which a large copy moves in 41.7; 166 MB fetched and 44 written by the counters).  Steps their chain of slots, rows and stores: 256 rows x 16 heads 3.6
+// back 35.9 on tensors that the last call left in the 256 MB of last-level cache, 46 and 41 on
+// others: 213 MB either way, which a large copy moves in 41.7; the counters show 166 MB fetched and
+// 44 written by the append).  Steps their chain of slots, rows and stores: 256 rows x 16 heads 3.6
 // and 3.2 us, 4 x 12 2.8 both.
 #include <stdio.h>
 
@@ -322,11 +323,10 @@ __global__ __launch_bounds__(CACHE4_NT) void gather_4bit_kernel(Cache4Args a, in
 
 // A decode step's tokens lie in parts of their own: a wave a token and 32 groups.  A prompt's fill
 // parts.  The host does not see which they are: calls of up to 512 tokens (the most rows of a
-// step that the projections take) are taken for steps.  16 heads of 64,
-// us, written / read, as a step against as a prompt: 256 rows 3.66 / 3.12 against 4.05 / 3.24, 512
-// 4.52 / 3.31 against 4.86 / 3.51; a prompt of 512 4.21 / 3.30 against 2.99 / 3.21, of 590 4.84 / 3.77
-// against 3.11 / 3.40, eight of 590 18.3 / 11.6 against 7.0 / 8.2: larger calls are prompts, and
-// would cost a prompt most.
+// step that the projections take) are taken for steps.  16 heads of 64, us, written / read, as a step
+// against as a prompt: 256 rows 3.66 / 3.12 against 4.05 / 3.24, 512 4.52 / 3.31 against 4.86 / 3.51;
+// a prompt of 512 4.21 / 3.30 against 2.99 / 3.21, of 590 4.84 / 3.77 against 3.11 / 3.40, eight of
+// 590 18.3 / 11.6 against 7.0 / 8.2: a larger call would cost a prompt more than it gives a step.
 inline bool is_step(int64_t T) { return T <= 512; }
 
 template <bool APPEND>

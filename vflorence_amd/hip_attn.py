@@ -1210,7 +1210,8 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     ``query_start_loc[n]`` to ``query_start_loc[n + 1] - 1`` and keys ``key_start_loc[n]`` to
     ``key_start_loc[n + 1] - 1`` (int32 [sequences + 1], rising, on the GPU).  Of ``out``, a
     contiguous tensor of query's shape and dtype, ``query`` itself or apart from it, and apart from
-    ``key`` and ``value``, the rows of the sequences are written, 0 where one has no keys; rows of none are left as they were.
+    ``key`` and ``value``, the rows of the sequences are written, 0 where one has no keys; rows of
+    none are left as they were.
     ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch; longer
     ones are served too."""
     rows, keys = query.shape, key.shape
