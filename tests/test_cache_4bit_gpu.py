@@ -327,6 +327,20 @@ def test_attention_long_contexts(dtype, bs, dim, heads, lens, groups):
                     [tables[g] for g in rows], dim**-0.5, groups=groups)
 
 
+@pytest.mark.parametrize("rows", [3000, 20000])
+def test_attention_few_rows_among_many(rows):
+    """A padded call: the context is split while its rows leave memory for four parts."""
+    gen = torch.Generator().manual_seed(rows)
+    cache = random_cache(gen, 200, 2, 16, 256)
+    table = torch.randperm(200, generator=gen)[:188].tolist()
+    query = queries(gen, rows, 2, 256, torch.bfloat16)
+    out = run_attention(query, cache, [3000] * rows, [table] * rows, 0.07, groups=[3])
+    found = attend(query[:3], values_of(cache, 256), [3000] * 3, [table] * 3, 0.07)
+    limit = attend_tolerance(query.dtype, 256, 3000, *found)
+    assert bool(((out[:3].double().cpu() - found[0]).abs() <= limit).all())
+    assert bool((out[3:] == 5.0).all())
+
+
 @pytest.mark.parametrize("bs", [16, 32])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_ignores_what_lies_behind(dtype, bs):

@@ -247,6 +247,11 @@ def test_c_entries_refuse():
     assert attend(rows=0, groups=0) == 0
     assert lib.vfl_attention_4bit_workspace(1, 1, 1, 64, 16, 4096) > 0
     assert lib.vfl_attention_4bit_workspace(256, 64, 16, 64, 16, 64) == 0
+    # rows of no group take no more than a bounded workspace: four parts of 4096 rows x 16 heads of
+    # 128 would be 4 * 2^16 * (128 * 4 + 8) = 136.3 MB, more than 2^27
+    for rows in (1, 500, 2000, 4096, 1 << 20, 1 << 62):
+        need = lib.vfl_attention_4bit_workspace(rows, 1, 16, 128, 16, 2500)
+        assert (need > 0) == (rows <= 2000) and need <= 1 << 27
 
     def cross(q=A, k=A, v=A, out=A, starts=A, queries=5, keys=7, sequences=2, heads=2, dim=64,
               longest=(3, 4), scale=0.125, dtype=VFL_FLOAT32, work=None):

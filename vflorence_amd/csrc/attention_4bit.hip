@@ -28,6 +28,7 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <utility>
 
 #include "e2m1.h"
@@ -389,14 +390,18 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
 // there is a workgroup a CU or fewer (eight / four: 16 rows of 2000 to 4000 tokens x 16 heads 14.7 /
 // 17.6, of 400 to 1000 6.3 / 6.1, 32 x 8 heads of 256 15.5 / 16.4; 384 workgroups of 64 dims 8.3 / 8.0,
 // 512 of 128 dims 15.9 / 12.9, of 256 dims 29.9 / 26.9, 1536 of 64 dims 18.6 / 14.9).
+// A call's rows all take a place for each part, also those of no group: parts that would need more
+// than 128 MB (the rows of a launch's own groups take 4.3 at most) are not made.
 struct Attn4Plan {
   int waves, splits;
 };
 
-inline Attn4Plan attn4_plan(int64_t num_groups, int H, int D, int64_t max_tokens) {
+inline Attn4Plan attn4_plan(int64_t num_rows, int64_t num_groups, int H, int D,
+                            int64_t max_tokens) {
   const int64_t wgs = num_groups * H;
   const int64_t fill = 256 * (D <= 256 ? 8 : 4) / (wgs * 4), most = max_tokens / (4 * 128);
-  const int64_t parts = fill < most ? fill : most;
+  const int64_t room = MOST_WORKSPACE / H / split_part_bytes(D) / num_rows;
+  const int64_t parts = std::min({fill, most, room});
   if (parts >= 4) return Attn4Plan{4, (int)parts};
   return Attn4Plan{D <= 256 && wgs <= 256 ? 8 : 4, 1};
 }
@@ -450,7 +455,7 @@ extern "C" int64_t vfl_attention_4bit_workspace(int64_t num_rows, int64_t num_gr
       max_blocks_per_seq <= 0)
     return 0;
   const Attn4Plan p =
-      attn4_plan(num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
+      attn4_plan(num_rows, num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
   return p.splits > 1 ? num_rows * num_heads * p.splits * split_part_bytes(head_dim) : 0;
 }
 
@@ -510,7 +515,7 @@ extern "C" int vfl_attention_with_kv_cache_4bit(
   a.num_blocks = num_blocks;
   a.sign = scale < 0.f ? -1.f : 1.f;
   if (table == 0) a.bt = seq_lens, a.bt_stride = 0, a.width = 1;  // read, and not used
-  const Attn4Plan plan = attn4_plan(num_groups, num_heads, head_dim, table * block_size);
+  const Attn4Plan plan = attn4_plan(num_rows, num_groups, num_heads, head_dim, table * block_size);
   if (plan.splits > 1) {
     if (!workspace) {
       set_error("%s: null workspace", who);

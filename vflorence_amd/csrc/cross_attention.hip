@@ -30,7 +30,6 @@ struct CrossPlan {
 // - launches of up to two workgroups a CU go to any XCD: 12 heads, fp32, 590 queries in two parts
 //   21.2, a head to an XCD 33.6.
 constexpr int64_t MOST_ROWS = 2147483647LL - 1024;  // (a tile past the last is counted in 32 bits)
-constexpr int64_t CROSS_MOST_WORKSPACE = 1LL << 27;
 
 CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool f32,
                      int64_t max_queries, int64_t max_keys) {
@@ -50,7 +49,7 @@ CrossPlan cross_plan(int64_t num_queries, int64_t sequences, int H, int D, bool 
   while (p.ks > 1 && 64 * (p.ks / 2) >= max_keys) p.ks /= 2;
   const int64_t wgs = workgroups(p.ks);
   const int64_t fill = (f32 ? 256 : 512) / wgs, parts = max_keys / (f32 ? 64 : 256 * p.ks);
-  const int64_t room = CROSS_MOST_WORKSPACE / (num_queries * H * split_part_bytes(D));
+  const int64_t room = MOST_WORKSPACE / (num_queries * H * split_part_bytes(D));
   const int64_t most_parts = std::min({fill, parts, room, (int64_t)32});
   if (most_parts >= 2) p.splits = (int)most_parts;
   p.spread = wgs * p.splits <= 512;

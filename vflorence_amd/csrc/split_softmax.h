@@ -53,6 +53,9 @@ struct SplitOut {
 // Bytes a (row, head) of one split takes in the workspace.
 inline int64_t split_part_bytes(int head_dim) { return head_dim * 4 + 8; }
 
+// Bytes of workspace that a launch takes at most.
+constexpr int64_t MOST_WORKSPACE = 1LL << 27;
+
 // A launch's rows and where their results go.
 struct DecodeRows {
   void *out;
