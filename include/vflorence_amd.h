@@ -637,7 +637,8 @@ int vfl_attention_with_kv_cache_4bit(const void *query, int64_t query_stride_tok
  * [num_keys] rows of num_heads x head_dim, 16-byte aligned with strides that are multiples of 16
  * bytes; out contiguous, query itself or apart from it, apart from key and value.  head_dim up to
  * 256; scale finite.  Sums and softmax in fp32, the weights rounded to the type for the second
- * product (fp32: kept to 2^-24).
+ * product (fp32: kept to 2^-24).  Infinities and NaN stay in the rows, heads and dims that the
+ * formula gives them to; a row whose scores are all -inf gets 0.
  * max_query_len and max_key_len, the longest runs expected, shape the launch (longer ones are
  * served too).  workspace as above, of vfl_packed_cross_attention_workspace bytes.
  */

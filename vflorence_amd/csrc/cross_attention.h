@@ -14,7 +14,9 @@
 // rounding's, two errors of a size.  A second term of a weight would take that away, at 2 to 16%
 // (8 runs of 60 to 128 queries 13.5 / 15.7 us, 21 and 29 over 17001 and 39999 keys 48.9 / 50.3).
 // fp32 goes in as three bf16 terms each, rounded, of whose nine products the six largest are taken:
-// the others are 2^-26 of the whole or less.
+// the others are 2^-26 of the whole or less.  An infinity has no such terms and makes NaN of its
+// scores or sums: those scores are taken again from the fp32 elements, and of those sums the
+// infinite values alone count.
 //
 // What bounds it: long texts the vector and matrix units together (64 texts of 128 to 1024 tokens
 // over 256 to 1024, 16 heads of 64, bf16: 161 us, 94 GFLOP, 585 TFLOP/s of a large matrix product's
@@ -91,8 +93,9 @@ template <int DT> __device__ __forceinline__ floatx16_t mfma32(uint4 a, uint4 b,
 }
 
 // A bf16 term of four floats, rounded, with the remainder left in f.  (In the first one, magnitudes
-// that would round to infinity give the largest finite one, and their remainder the rest: so do
-// an infinity and a NaN, which the second term then is.)
+// that would round to infinity give the largest finite one, and their remainder the rest.  An
+// infinity has no three terms: its third is NaN, which the sums that meet it then are, and by which
+// score_of and infinite_values' callers find them.)
 __device__ __forceinline__ uint2 take_rounded(float (&f)[4], bool first) {
   constexpr float MOST = 3.38953138925153547590e38f;
   float c[4];
@@ -136,6 +139,55 @@ __device__ __forceinline__ uint2 read_turned(const uint8_t *p) {
       uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(uint32_t)(uintptr_t)p));
 }
 
+// NaN where one of 16 registers is no finite number.
+__device__ __forceinline__ float not_finite(const floatx16_t &x) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t = fmaf(x[i], 0.f, t);
+  return t;
+}
+// Which of 16 registers are NaN.
+__device__ __forceinline__ uint32_t nan_places(const floatx16_t &x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m |= (x[i] != x[i] ? 1u : 0u) << i;
+  return m;
+}
+
+// The score of a query and a key from their fp32 elements, as the definition has it for infinities.
+// (One at a time: it is rare, and registers that it takes are all waves'.)
+__device__ __forceinline__ float score_of(const CrossArgs &a, const float *q, const float *k) {
+  float s = 0.f;
+#pragma unroll 1
+  for (int d = 0; d < a.D; ++d) s = fmaf(q[d], k[d], s);
+  return a.negative ? -s : s;
+}
+
+// The sum of one dim of `keys` values, among them infinities or NaN, beside which the finite ones
+// do not count: weighted by a score of -inf they are 0 * inf.  (0: there are none.)
+__device__ __forceinline__ float infinite_values(const CrossArgs &a, const float *q, const float *k,
+                                                 const float *v, int keys) {
+  constexpr int AT_ONCE = 8;
+  float r = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < keys; j += AT_ONCE) {
+    float x[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) x[i] = v[min(j + i, keys - 1) * a.v_st];
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) finite = finite && fabsf(x[i]) < INFINITY;
+    if (finite) continue;
+#pragma unroll 1
+    for (int i = j; i < min(j + AT_ONCE, keys); ++i) {
+      const float y = v[i * a.v_st];
+      if (fabsf(y) < INFINITY) continue;
+      r += score_of(a, q, k + i * a.k_st) == NEG_INF_F ? NAN : y;
+    }
+  }
+  return r;
+}
+
 // Shape of a launch: heads of up to 32 DG dims, KS key groups of 4 / KS waves.
 constexpr int WAVES = 4;
 template <int DT, int DG, int KS> struct CrossShape {
@@ -152,8 +204,9 @@ template <int DT, int DG, int KS> struct CrossShape {
   static constexpr int GT = 64 * GW;           // threads of a key group
   static constexpr int PIECES = KT * DG * 4;   // of 8 elements, of K or V
   static constexpr int CH = (PIECES + GT - 1) / GT;  // a thread's
-  // waves of a SIMD at least: three of heads of up to 64 (long texts 162 us; four, which spill, 173)
-  static constexpr int OCC = !F32 && DG <= 2 && KS == 1 ? 3 : 1;
+  // waves of a SIMD at least: three of heads of up to 64 (long texts 162 us; four, which spill, 173);
+  // fp32's heads of 96 two, which the LDS leaves them (those of up to 64 have them anyway)
+  static constexpr int OCC = KS > 1 ? 1 : F32 ? (DG == 3 ? 2 : 1) : DG <= 2 ? 3 : 1;
   static_assert(BUFS * KS * TILE <= 160 * 1024, "the tiles fit the LDS");
 };
 
@@ -345,8 +398,8 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
     bool fresh = true;  // (of the wave) no row has one yet
     bool wide = false;  // (of the wave) some row's ms loses its units
 
-    // 32 keys from row 32 b of the buffer on; ragged: `left` of them
-    auto attend_block = [&](int left, int b, int buf, auto ragged) {
+    // 32 keys, the run's from `key0` on, from row 32 b of the buffer on; ragged: `left` of them
+    auto attend_block = [&](int key0, int left, int b, int buf, auto ragged) {
       const uint8_t *kt = tile0 + buf * BUF + 32 * b * STRIDE, *vt = kt + PLANES * S::PLANE;
       auto scores = [&]() {
         floatx16_t s;
@@ -434,6 +487,20 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
           need = !(sa <= MOST_SUM && sb <= MOST_SUM);
         }
         floatx16_t s = scores();
+        if constexpr (S::F32) {  // (a NaN weight always comes here)
+          const float t = not_finite(s);
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(t != t) != 0, 0)) {
+            const uint32_t lost = nan_places(s);
+#pragma unroll 1
+            for (int n = 0; n < 16; ++n) {
+              if (!(lost >> n & 1)) continue;
+              const int key = key0 + 8 * (n / 4) + n % 4 + 4 * hf;
+              const float x = score_of(a, qp, k + key * a.k_st);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[i] = i == n ? x : s[i];
+            }
+          }
+        }
         float mx = m;
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -478,15 +545,17 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
       if constexpr (S::F32) __builtin_amdgcn_s_setprio(0);
     };
 
-    auto attend = [&](int buf) {
+    auto attend = [&](int t, int buf) {
+      const int key0 = (tile_first + t) * KT;
 #pragma unroll
-      for (int b = 0; b < KB; ++b) attend_block(32, b, buf, std::false_type{});
+      for (int b = 0; b < KB; ++b) attend_block(key0 + 32 * b, 32, b, buf, std::false_type{});
     };
     auto attend_last = [&](int t, int buf) {  // of the run's last tile some rows may be no keys
-      const int left = nk - (tile_first + t) * KT;
+      const int key0 = (tile_first + t) * KT, left = nk - key0;
 #pragma unroll
       for (int b = 0; b < KB; ++b)
-        if (left > 32 * b) attend_block(left - 32 * b, b, buf, std::true_type{});
+        if (left > 32 * b)
+          attend_block(key0 + 32 * b, left - 32 * b, b, buf, std::true_type{});
     };
 
     // Step t: the group's tile of step t is in buffer t % BUFS, the next one's rows in flight.
@@ -500,7 +569,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
       for (int t = 0; t < steps - 1; ++t) {
         store((t + 1) * KS + grp, (t + 1) & 1);
         if (t + 2 < steps) load((t + 2) * KS + grp);
-        if (active) attend(t & 1);
+        if (active) attend(t * KS + grp, t & 1);
         __syncthreads();
       }
     } else {
@@ -510,7 +579,7 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
         __syncthreads();
         if (t + 1 >= steps) break;
         load((t + 1) * KS + grp);
-        if (active) attend(0);
+        if (active) attend(t * KS + grp, 0);
         __syncthreads();
       }
     }
@@ -558,6 +627,25 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
             for (int i = 0; i < 16; ++i) o[b][i] = fmaf(src[(16 * b + i) * 64], f, o[b][i]);
         }
         m = M;
+      }
+    }
+    if constexpr (S::F32) {
+      // Sums that met an infinite value are NaN, whatever its weights: such dims are looked at again.
+      // (Before any of the row's results is written, which may be where its query is.)
+      const int key0 = tile_first * KT, keys = min(ntiles * KT, nk - key0);
+#pragma unroll
+      for (int b = 0; b < DG; ++b) {
+        const float t = not_finite(o[b]);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(t != t) == 0, 1)) continue;
+        const uint32_t lost = grp == 0 && query < nq && l == l ? nan_places(o[b]) : 0;
+#pragma unroll 1
+        for (int n = 0; n < 16; ++n) {
+          if (!(lost >> n & 1)) continue;  // (a NaN sum has keys; dims past the head are 0)
+          const int d = 32 * b + 8 * (n / 4) + n % 4 + 4 * hf;
+          const float r = infinite_values(a, qp, k + key0 * a.k_st, v + key0 * a.v_st + d, keys);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[b][i] = i == n && r != 0.f ? r : o[b][i];
+        }
       }
     }
     if (grp == 0 && query < nq) {

@@ -1213,7 +1213,8 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     ``key`` and ``value``, the rows of the sequences are written, 0 where one has no keys; rows of
     none are left as they were.
     ``max_query_len`` and ``max_key_len``, the lengths of the longest, shape the launch; longer
-    ones are served too."""
+    ones are served too.  Infinities and NaN stay in the rows, heads and dims that the formula
+    gives them to; a row whose scores are all -inf is 0."""
     rows, keys = query.shape, key.shape
     if len(rows) != 3 or len(keys) != 3 or value.shape != keys or rows[1:] != keys[1:]:
         raise ValueError("query must be [T, H, D], key and value [S, H, D], got "
