@@ -11,7 +11,7 @@
 //   online softmax per row over 64 tokens, fp32, a register a row
 //   O[row][d]   += (P[row][tok] vs[tok]) . V[tok][d]   a lane is two dims of its row of lanes'
 //                  16 tokens.  A group's V scales go to the weights: 64 tokens' V codes are
-//                  converted unscaled, four tokens to a block's operand
+//                  converted by a constant, four tokens to a block's operand
 // Queries go in as bf16 terms, which hold all of their bits: one of bf16, two of fp16, three of
 // fp32.  Weights as two terms, 2^-17 relative, or three for fp32 outputs, 2^-25: below the
 // output's rounding.  Their sum is taken in fp32.
@@ -90,6 +90,14 @@ template <int CTRL> __device__ __forceinline__ float quad(float x) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xF, 0xF,
                                                                true));
 }
+
+// What is summed is taken down by 2^-20, so that sums of 2^12 tokens of the largest values (6 *
+// 2^125), whose weights pass their reference by the slack, are finite: a weight by 2^-6, which with
+// its V scale is 2^127 at most then, V's codes by 2^-14, the weights' own sum by both.  A weight of
+// the least scale, 2^-100, keeps its terms above 2^-134: 2^-28 of that scale.  (A smaller slack in
+// place of the first costs up to 5% of the time, this up to 1.)
+constexpr float WEIGHT_FACTOR = 0x1p-6f, CODE_FACTOR = 0x1p-14f;
+static_assert(RESCALE_SLACK_LOG2 <= 8.f, "2^(125 + slack - 6) is finite");
 
 // Four registers to the one of each row of 16 lanes (row q: register q), each summed over the rows.
 __device__ __forceinline__ float rows_scatter4(const floatx4_t &x) {
@@ -272,7 +280,8 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
         }
       static_for<G>([&](auto g) {
         // (a masked token's scale may be anything)
-        const float vs = x.ok ? e2m1_scale((x.s[G + g] >> byte) & 255u) : 0.f;
+        const float vs =
+            x.ok ? e2m1_scale((x.s[G + g] >> byte) & 255u) * WEIGHT_FACTOR : 0.f;
         uint2 pop[QUADS][PT];
 #pragma unroll
         for (int u = 0; u < QUADS; ++u) {
@@ -306,8 +315,10 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
           // byte 1 of lo: tokens 1 and 0, byte 3: 3 and 2; of hi bytes 0 and 2
           const uint32_t lo = (w[i] << 12 & 0xf000f000u) | (w[i] & 0x0fff0fffu);
           const uint32_t hi = (w[i] >> 12 & 0x000f000fu) | (w[i] & 0xfff0fff0u);
-          const uint2 b0 = make_uint2(e2m1_bf16x2<1>(lo, 1.f), e2m1_bf16x2<3>(lo, 1.f));
-          const uint2 b1 = make_uint2(e2m1_bf16x2<0>(hi, 1.f), e2m1_bf16x2<2>(hi, 1.f));
+          const uint2 b0 = make_uint2(e2m1_bf16x2<1>(lo, CODE_FACTOR),
+                                      e2m1_bf16x2<3>(lo, CODE_FACTOR));
+          const uint2 b1 = make_uint2(e2m1_bf16x2<0>(hi, CODE_FACTOR),
+                                      e2m1_bf16x2<2>(hi, CODE_FACTOR));
 #pragma unroll
           for (int u = 0; u < QUADS; ++u)
 #pragma unroll
@@ -352,7 +363,7 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
           to[rg * DP + 32 * g + 16 * e + p16] = rows_scatter4(acc[u][g][e]);
 #pragma unroll
       for (int r = 0; r < QR; ++r) {
-        const float sum = group_sum<64>(l[u][r]);
+        const float sum = group_sum<64>(l[u][r]) * (WEIGHT_FACTOR * CODE_FACTOR);
         if (lane == 0) {
           s_m[(wave * QUADS + u) * 4 + r] = m[u][r];
           s_l[(wave * QUADS + u) * 4 + r] = sum;
