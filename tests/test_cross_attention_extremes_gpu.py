@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.cache_4bit_oracle import cross, cross_tolerance
+from tests.cache_4bit_oracle import cross, cross_tolerance, tolerance
 from tests.test_cross_attention_gpu import DEV, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -140,3 +140,27 @@ def test_rows_of_no_finite_score(dtype, scale, keys):
     error = (out[:, 1].double() - v[keys - 3, 1].double()).abs()
     steps = 5 if dtype == torch.float32 else 1
     assert bool((error <= v[keys - 3, 1].double().abs() * steps * torch.finfo(dtype).eps).all())
+
+
+@pytest.mark.parametrize("base", [3000.0, 30000.0, -40000.0, 45410.0, 60000.0])
+@pytest.mark.parametrize("dim,queries,keys", [(64, 130, 700), (64, 9, 700), (64, 9, 6000),
+                                              (128, 40, 2500), (256, 5, 900)])
+def test_fp32_scores_far_from_zero(dim, queries, keys, base):
+    """Scores that lie ``base`` from zero and rise by 6, so that references move, are apart in
+    the key groups and in the parts: weights follow their differences (on either side of 2^16 in
+    log2 units, from where a reference is no whole number, and across it).  Query and key have one
+    dim that is not 0, of 22 bits: scores are exact.  A weight's exponent is rounded at 16 to 32
+    in size, 2^-20, its exponential is good to 2^-22, a correction between two references adds
+    three roundings below 2^-21 (of a difference of at most 9 in log2 units)."""
+    gen = torch.Generator().manual_seed(dim + keys)
+    q, k, v = inputs(gen, [queries], [keys], 1, dim, torch.float32)
+    q.zero_()
+    q[:, 0, 7] = 1.0
+    steps = torch.randint(-64, 64, (keys,), generator=gen) + torch.linspace(0, 384, keys).long()
+    k[:, 0, 7] = (base + steps / 64).to(DEV)
+    out = run(q, k, v, [0, queries], [0, keys], 1.0)
+    o, weight, size = cross(q, k, v, [0, queries], [0, keys], 1.0)
+    limit = tolerance(torch.float32, 0, keys, 3 * 2.0**-26, o, weight, size * 0)
+    limit += weight * 2 * (2.0**-20 + 3 * 2.0**-21)
+    error = (out.double().cpu() - o).abs()
+    assert bool((error <= limit).all()), float((error / limit).max())

@@ -392,11 +392,19 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
     for (int b = 0; b < DG; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
-    // A row's reference m is a score; weights are 2^((score - m) scale + WEIGHT_LOG2).
+    // A row's reference m is a score; weights are 2^(score scale - ms), ms the whole number next to
+    // m scale, less WEIGHT_LOG2: exact up to WHOLE, so that weights about different references,
+    // key groups' and parts' too, are apart by a power of two.  Where it is larger, they are
+    // 2^((score - m) scale + WEIGHT_LOG2).
+    constexpr float WHOLE = 65536.f;
     float m = NO_SCORE, l = 0.f;
-    float ms = 0.f;     // m * scale - WEIGHT_LOG2
+    float ms = INFINITY;
     bool fresh = true;  // (of the wave) no row has one yet
-    bool wide = false;  // (of the wave) some row's ms loses its units
+    bool wide = false;  // (of the wave) some row's ms is past WHOLE
+    // log2 of what weights are above those about m itself
+    auto above = [&](float m, float ms) {
+      return fabsf(ms) <= WHOLE ? fmaf(m, a.scale_log2, -(ms + WEIGHT_LOG2)) : 0.f;
+    };
 
     // 32 keys, the run's from `key0` on, from row 32 b of the buffer on; ragged: `left` of them
     auto attend_block = [&](int key0, int left, int b, int buf, auto ragged) {
@@ -456,15 +464,14 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
       };
       // Weights about the references as they stand, without a look at the scores' maxima: a weight
       // that passes its reference by more than the slack shows in its lane's sum.
-      // One operation a weight where the product m * scale keeps its units to 2^-8 (what it is
-      // rounded by is the same for every weight of the row), two where it does not: by row, so that
-      // none hangs on its neighbours.
+      // One operation a weight where the reference is a whole number, two where it is not: by row,
+      // so that none hangs on its neighbours.
       auto weights = [&](floatx16_t &s) {
         if (__builtin_expect(!wide, 1)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], a.scale_log2, -ms));
         } else {
-          const bool one = fabsf(ms) <= 65536.f;
+          const bool one = fabsf(ms) <= WHOLE;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float x = fmaf(s[i], a.scale_log2, -ms);
@@ -507,8 +514,10 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
         float ma, mb;
         half_pair(mx, ma, mb);
         mx = fmaxf(ma, mb);
+        const float to = rintf(mx * a.scale_log2) - WEIGHT_LOG2;
         if (!fresh) {
-          const float corr = need ? fast_exp2((m - mx) * a.scale_log2) : 1.f;
+          const float corr =
+              need ? fast_exp2((m - mx) * a.scale_log2 + (above(mx, to) - above(m, ms))) : 1.f;
           l *= corr;
 #pragma unroll
           for (int d = 0; d < DG; ++d)
@@ -516,9 +525,9 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
             for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
         m = need ? mx : m;
-        ms = fmaf(m, a.scale_log2, -WEIGHT_LOG2);
+        ms = need ? to : ms;
         fresh = false;
-        wide = __builtin_amdgcn_ballot_w64(!(fabsf(ms) <= 65536.f)) != 0;
+        wide = __builtin_amdgcn_ballot_w64(!(fabsf(ms) <= WHOLE)) != 0;
         weights(s);
       }
       l += sum;
@@ -591,6 +600,14 @@ __global__ __launch_bounds__(64 * WAVES, (CrossShape<DT, DG, KS>::OCC)) void cro
       float la, lb;
       half_pair(l, la, lb);
       l = la + lb;
+    }
+    if (KS > 1 || a.splits > 1) {  // parts meet about m itself
+      const float f = fast_exp2(-above(m, ms));
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DG; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= f;
     }
 
     if constexpr (KS > 1) {
