@@ -797,3 +797,22 @@ def test_refuses_gradients_of_the_cache_and_counts_writes():
         hip_attn.reshape_and_cache_8bit(key, key, *held, slots)
         other = torch.empty_like(query)
         attend_into(other)
+
+
+@pytest.mark.parametrize("rows", [3000, 20000])
+def test_attention_few_rows_among_many(rows):
+    """A padded call: the context is split while its rows leave memory for four parts."""
+    from vflorence_amd import hip_attn
+
+    query, cache, lens, tables, _, starts = paged_case(17, torch.bfloat16, 256, 16, [3000], 3)
+    many = torch.randn(rows, 2, 256, generator=torch.Generator().manual_seed(rows))
+    many = many.to(torch.bfloat16).to(DEV)
+    many[:3] = query
+    out = torch.full_like(many, 7.0)
+    hip_attn.attention_with_kv_cache_8bit(
+        many, *cache, out, torch.tensor(lens[:1], dtype=torch.int32, device=DEV).expand(rows),
+        scale=256**-0.5,
+        block_table=torch.tensor(tables[:1], dtype=torch.int32, device=DEV).expand(rows, -1),
+        scheduler_metadata=metadata(many, 16, 3, starts))
+    close(query, out[:3], Cache.of(*cache), lens, tables, 256**-0.5)
+    assert bool((out[3:] == 7.0).all())

@@ -219,3 +219,13 @@ def test_oracle_append_rescales_a_growing_block():
     cache.append(one * 1000, one, torch.tensor([17]))
     assert cache.scales[1, 0, 0] == 4.0 and float(cache.values()[0][1, 0, 0, 0]) == 1.0
     assert float(cache.values()[0][1, 0, 1, 0]) == 1024.0  # 250 lies between 240 and 256
+
+
+def test_attention_workspace_is_bounded():
+    """Rows of no group take a place for each part: four parts of 4096 rows x 16 heads of 128
+    would be 4 * 2^16 * (128 * 4 + 8) = 136.3 MB, more than 2^27."""
+    from vflorence_amd._lib import lib
+
+    for rows in (1, 500, 2000, 4000, 4096, 20000, 1 << 30, 1 << 62):
+        need = lib.vfl_attention_8bit_workspace(rows, 1, 16, 128, 16, 2500)
+        assert (need > 0) == (rows <= 4000) and need <= 1 << 27, rows

@@ -33,6 +33,8 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "e4m3.h"
 #include "split_softmax.h"
 
@@ -414,11 +416,14 @@ __global__ __launch_bounds__(64 * NW) void attention_8bit_kernel(Attn8Args a) {
 // join costs 4.6 us (512 workgroups of 128 dims to 1024 tokens 24.9 in two parts, 20.5 whole; 16
 // heads of 64, one group: 1024 tokens 8.8 split, 7.0 whole; 2048 8.8 / 10.3; 4096 9.1 / 16.4; 2
 // rows of 17001 and 39999 tokens x 8 heads of 128 27.0 in 16 parts, 27.6 in 8, 28.6 in 32).
+// A call's rows all take a place for each part, also those of no group: parts that would need more
+// than 128 MB are not made.
 struct Attn8Plan {
   int waves, splits;
 };
 
-inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens) {
+inline Attn8Plan attn8_plan(int64_t num_rows, int64_t num_groups, int H, int D,
+                            int64_t max_tokens) {
   // waves of a launch that the card holds at once, by the registers that a head of D takes
   const int64_t resident = 256 * (D <= 128 ? 16 : D <= 192 ? 12 : D <= 256 ? 8 : 4);
   const int64_t wgs = num_groups * H;
@@ -427,7 +432,8 @@ inline Attn8Plan attn8_plan(int64_t num_groups, int H, int D, int64_t max_tokens
   if (bytes > (192 << 10) && wgs * p.waves < resident) {
     const int64_t fill = resident / (wgs * p.waves);
     const int64_t most = max_tokens / 32 / (p.waves * 2);
-    const int64_t parts = fill < most ? fill : most;
+    const int64_t room = MOST_WORKSPACE / H / split_part_bytes(D) / num_rows;
+    const int64_t parts = std::min({fill, most, room});
     if (parts >= 4) p.splits = (int)parts;
   }
   return p;
@@ -470,7 +476,7 @@ extern "C" int64_t vfl_attention_8bit_workspace(int64_t num_rows, int64_t num_gr
       max_blocks_per_seq <= 0)
     return 0;
   const Attn8Plan p =
-      attn8_plan(num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
+      attn8_plan(num_rows, num_groups, num_heads, head_dim, max_blocks_per_seq * block_size);
   return p.splits > 1 ? num_rows * num_heads * p.splits * split_part_bytes(head_dim) : 0;
 }
 
@@ -530,7 +536,7 @@ extern "C" int vfl_attention_with_kv_cache_8bit(
   a.q_vec = (uintptr_t)query % 16 == 0 && query_stride_token % (16 / eb) == 0 &&
             query_stride_head % (16 / eb) == 0;
   if (table == 0) a.bt = seq_lens, a.bt_stride = 0, a.width = 1;  // read, and not used
-  const Attn8Plan plan = attn8_plan(num_groups, num_heads, head_dim, table * block_size);
+  const Attn8Plan plan = attn8_plan(num_rows, num_groups, num_heads, head_dim, table * block_size);
   if (plan.splits > 1) {
     if (!workspace) {
       set_error("%s: null workspace", who);
