@@ -605,3 +605,27 @@ def test_serving_together():
     both = limit[first] + attend_tolerance(torch.bfloat16, dim, max(lens),
                                            *(x[first] for x in found))
     assert bool(((step.double().cpu() - out[first].double().cpu()).abs() <= both).all())
+
+
+def test_either_binding(monkeypatch):
+    """Through ctypes the calls give what they give through the extension module."""
+    from vflorence_amd import hip_attn
+    from vflorence_amd._lib import lib
+
+    gen = torch.Generator().manual_seed(31)
+    key, value = tokens_of(gen, 40, 2, 64, torch.bfloat16)
+    slots, query = torch.arange(40, device=DEV), queries(gen, 3, 2, 64, torch.bfloat16)
+
+    def step():
+        cache = hip_attn.kv_cache_4bit(3, 2, 16, 64, DEV)
+        hip_attn.reshape_and_cache_4bit(key, value, cache, slots)
+        out = run_attention(query, cache, [40] * 3, [[0, 1, 2]] * 3, 0.125)
+        starts = [torch.tensor(s, dtype=torch.int32, device=DEV) for s in ([0, 3], [0, 40])]
+        across = torch.empty_like(query)
+        hip_attn.packed_cross_attention(query, key, value, across, *starts, scale=0.125,
+                                        max_query_len=3, max_key_len=40)
+        return cache, out, across, *read(cache, slots, 40, 2, 64, torch.bfloat16)
+
+    want = step()
+    monkeypatch.setattr(hip_attn, "calls", lib)
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))

@@ -298,3 +298,32 @@ def test_entry_callables():
             call(*bad)
     with pytest.raises(TypeError):
         calls.vfl_packed_cross_attention(*[A] * 19, "scale", 1, None, None)
+
+
+def test_entries_without_the_extension_module(tmp_path):
+    """A package that holds the library alone loads, and calls the same entries through it."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+
+    import vflorence_amd
+    from vflorence_amd import _lib
+
+    assert _lib._load_calls(str(tmp_path / "_calls.so")) is _lib.lib
+    (tmp_path / "_calls.so").write_text("no shared object")
+    assert _lib._load_calls(str(tmp_path / "_calls.so")) is _lib.lib
+    here = os.path.dirname(vflorence_amd.__file__)
+    shutil.copytree(here, tmp_path / "vflorence_amd",
+                    ignore=lambda _, names: [n for n in names
+                                             if n.startswith("_calls") or n in ("_build", "csrc")])
+    code = ("from vflorence_amd import _lib, hip_attn\n"
+            f"assert _lib.__file__.startswith({str(tmp_path)!r}), _lib.__file__\n"
+            "assert hip_attn.calls is _lib.lib\n"
+            f"args = [{A}, {A}, 128, 64, 128, 64, {A}, {A}, 0, 2, 64, 16, 8, 1, None]\n"
+            "assert hip_attn.calls.vfl_reshape_and_cache_4bit(*args) == 0\n"
+            "args[13] = 9\n"
+            "assert hip_attn.calls.vfl_reshape_and_cache_4bit(*args) != 0\n")
+    run = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True,
+                         env=dict(os.environ, PYTHONPATH=str(tmp_path)))
+    assert run.returncode == 0, run.stderr

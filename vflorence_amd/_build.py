@@ -1,5 +1,5 @@
 """In-tree builds (no cmake): libvflorence_amd.so for gfx950 (hipcc), the Python callables over
-some of its entries (_calls.so, g++) and the engine's native host core libvfl_host.so (g++, CPU
+some of its entries (_calls, g++) and the engine's native host core libvfl_host.so (g++, CPU
 only).
 
     python -m vflorence_amd._build          # or __graft_entry__.build()
@@ -14,6 +14,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from importlib.machinery import EXTENSION_SUFFIXES
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -77,14 +78,20 @@ def build_host_library(verbose: bool = False) -> str:
 
 
 CALLS_SOURCES = ("host/entry_calls.cpp",)
-CALLS_OUTPUT = os.path.join(HERE, "_calls.so")
+# (the name carries this interpreter's tag: another one does not load it)
+CALLS_OUTPUT = os.path.join(HERE, "_calls" + EXTENSION_SUFFIXES[0])
 
 
-def build_calls(verbose: bool = False) -> str:
+def build_calls(verbose: bool = False) -> str | None:
     """Compile the Python callables over OUTPUT's entries into CALLS_OUTPUT; always recompiles.
-    OUTPUT has to be built: they are linked with it, and find it beside them."""
+    OUTPUT has to be built: they are linked with it, and find it beside them.  None where the
+    interpreter's headers are not installed: the package then calls OUTPUT through ctypes."""
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        print(f"no Python.h in {include}: {os.path.basename(CALLS_OUTPUT)} is not built", flush=True)
+        return None
     return _build_host(CALLS_OUTPUT, CALLS_SOURCES,
-                       (f"-I{sysconfig.get_paths()['include']}", f"-L{HERE}",
+                       (f"-I{include}", f"-L{HERE}",
                         f"-l:{os.path.basename(OUTPUT)}", "-Wl,-rpath,$ORIGIN",
                         "-Wl,--allow-shlib-undefined"), verbose)
 

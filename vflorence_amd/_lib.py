@@ -9,10 +9,14 @@ run a fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 LIB_NAME = "libvflorence_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
+CALLS_PATH = os.path.join(os.path.dirname(LIB_PATH),
+                          "_calls" + importlib.machinery.EXTENSION_SUFFIXES[0])
 
 VFL_FLOAT32, VFL_BFLOAT16, VFL_FLOAT16 = 0, 1, 2
 VFL_GROUP_SHARED_TABLE, VFL_GROUP_OWN_TABLES = 0, 1
@@ -225,20 +229,17 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
-def _load_calls():
+def _load_calls(path: str = CALLS_PATH):
     """The entries whose wrappers are called per step, as callables of an extension module
-    (linked with the library above): the same arguments and status as through ``lib``."""
-    import importlib.machinery
-    import importlib.util
-
-    path = os.path.join(os.path.dirname(LIB_PATH), "_calls.so")
-    if not os.path.exists(path):
-        raise LibraryMissing(f"{path} is not built; run "
-                             "`python -c 'import __graft_entry__ as g; g.build()'`")
+    (linked with the library above): the same arguments and status as through ``lib``, which
+    serves them itself where the module is not built or not for this interpreter."""
     name = __package__ + "._calls"
     loader = importlib.machinery.ExtensionFileLoader(name, path)
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
-    loader.exec_module(module)
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+        loader.exec_module(module)
+    except ImportError:
+        return lib
     return module
 
 

@@ -2,6 +2,7 @@
 // argument handling: a ctypes call converts 15 to 24 arguments in 1.7 to 2.4 us, these in 0.2 to
 // 0.3.  Arguments go by position, an address as an int or None; the result is the entry's status.
 // An argument of another type or out of its C type's range raises before the entry is called.
+// (The package does without this module where it is not built, through ctypes.)
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
