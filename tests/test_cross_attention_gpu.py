@@ -273,3 +273,31 @@ def test_other_stream_gradients_and_versions():
     version = out._version
     run(q, k, v, [0, 40], [0, 90], 0.125, out=out)
     assert out._version > version
+
+
+@pytest.mark.parametrize("which", ["query", "key", "value", "far"])
+def test_a_misaligned_tensor_is_copied_alone(which):
+    """One operand at an odd element or, ``far``, of a token stride past the kernel's: of the
+    others nothing is copied."""
+    gen = torch.Generator().manual_seed(19)
+    sizes = dict(query=9, key=5000, value=5000)
+    at = {}
+    for name, rows in sizes.items():
+        odd = int(name == which)
+        base = torch.randn(rows * 128 + odd, generator=gen).to(torch.bfloat16).to(DEV)
+        at[name] = base[odd:].view(rows, 2, 64)
+    if which == "far":
+        base = torch.zeros(40, (1 << 22) + 8, dtype=torch.bfloat16, device=DEV)
+        base[:, :128].copy_(at["key"][:40].flatten(1))
+        at["key"], at["value"] = base[:, :128].view(40, 2, 64), at["value"][:40]
+    keys = at["key"].shape[0]
+    aligned = [x.clone(memory_format=torch.contiguous_format) for x in at.values()]
+    want = check(*aligned, [0, 9], [0, keys], 0.125, longest=(9, 64))  # (one part: no workspace)
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    assert torch.equal(run(*at.values(), [0, 9], [0, keys], 0.125, longest=(9, 64), out=out), want)
+    used = torch.cuda.max_memory_allocated() - before
+    copied = at.get(which, at["key"]).numel() * 2
+    assert copied <= used <= copied + (1 << 14), (used, copied)

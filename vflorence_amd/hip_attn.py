@@ -1244,11 +1244,16 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     if (query.requires_grad or key.requires_grad or value.requires_grad or out.requires_grad):
         refuse_gradients("packed_cross_attention")
     q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
-    # the kernel reads 16 bytes at a time: rows that do not allow it are copied
-    steps = (q_st[0] | q_st[1] | k_st[0] | k_st[1] | v_st[0] | v_st[1]) * query.element_size()
+    # the kernel reads 16 bytes at a time: tensors whose rows do not allow it are copied
+    size = query.element_size()
+    steps = (q_st[0] | q_st[1] | k_st[0] | k_st[1] | v_st[0] | v_st[1]) * size
     if (q | k | v | steps) & 15 or k_st[0] > CROSS_MAX_STRIDE or v_st[0] > CROSS_MAX_STRIDE:
-        query, key, value = (x.clone(memory_format=torch.contiguous_format)
-                             for x in (query, key, value))
+        if (q | (q_st[0] | q_st[1]) * size) & 15:
+            query = query.clone(memory_format=torch.contiguous_format)
+        if (k | (k_st[0] | k_st[1]) * size) & 15 or k_st[0] > CROSS_MAX_STRIDE:
+            key = key.clone(memory_format=torch.contiguous_format)
+        if (v | (v_st[0] | v_st[1]) * size) & 15 or v_st[0] > CROSS_MAX_STRIDE:
+            value = value.clone(memory_format=torch.contiguous_format)
         q_st, k_st, v_st = query.stride(), key.stride(), value.stride()
         q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
     query_start_loc, key_start_loc = query_start_loc.contiguous(), key_start_loc.contiguous()
