@@ -301,3 +301,17 @@ def test_a_misaligned_tensor_is_copied_alone(which):
     used = torch.cuda.max_memory_allocated() - before
     copied = at.get(which, at["key"]).numel() * 2
     assert copied <= used <= copied + (1 << 14), (used, copied)
+
+
+def test_refuses_its_keys_or_values_as_the_output():
+    gen = torch.Generator().manual_seed(20)
+    q, _, _ = inputs(gen, [40], [1], 2, 64, torch.float32)
+    k, v = torch.ones_like(q), torch.zeros_like(q)
+    for args, out in (((q, k, v), k), ((q, k, v), v), ((q, q, q), q)):
+        with pytest.raises(ValueError, match="memory of its own"):
+            run(*args, [0, 40], [0, 40], 0.125, out=out)
+    assert bool((k == 1).all()) and not v.any() and q.any()
+    assert not run(q, k, v, [0, 40], [0, 40], 0.125, out=q).any()
+    # (no queries, or no keys, no address to share)
+    run(q[:0], k, v, [0, 0], [0, 40], 0.125)
+    run(q, k[:0], v[:0], [0, 40], [0, 0], 0.125)

@@ -1243,7 +1243,9 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     index = one_gpu(query, key, value, out, query_start_loc, key_start_loc)
     if (query.requires_grad or key.requires_grad or value.requires_grad or out.requires_grad):
         refuse_gradients("packed_cross_attention")
-    q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    q, k, v, to = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    if (to == k or to == v) and num_queries and keys[0]:
+        raise ValueError("out is written while key and value are read: it needs memory of its own")
     # the kernel reads 16 bytes at a time: tensors whose rows do not allow it are copied
     size = query.element_size()
     steps = (q_st[0] | q_st[1] | k_st[0] | k_st[1] | v_st[0] | v_st[1]) * size
@@ -1261,7 +1263,7 @@ def packed_cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.
     need = _cross_workspace(num_queries, starts[0] - 1, num_heads, head_dim, *longest, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     on_device(index, calls.vfl_packed_cross_attention, q, q_st[0], q_st[1], k, k_st[0], k_st[1], v,
-              v_st[0], v_st[1], out.data_ptr(), query_start_loc.data_ptr(),
+              v_st[0], v_st[1], to, query_start_loc.data_ptr(),
               key_start_loc.data_ptr(), num_queries, keys[0], starts[0] - 1, num_heads, head_dim,
               *longest, float(scale), dtype, workspace.data_ptr() if need else None)
     torch.autograd.graph.increment_version((out,))  # autograd's check of saved tensors
