@@ -15,8 +15,8 @@
 //
 // What bounds it: prompts HBM (64 of 256 to 1024 tokens x 16 heads of 64, bf16, written 36.1 us, read
 // back 35.9 on tensors that the last call left in the 256 MB of last-level cache, 46 and 41 on
-// others: 213 MB either way, which a large copy moves in 41.7; the counters show 166 MB fetched and
-// 44 written by the append).  Steps their chain of slots, rows and stores: 256 rows x 16 heads 3.6
+// other caches, read back into rows that were not written lately 65: 213 MB either way, which a large
+// copy moves in 41.7; the counters show 166 MB fetched and 44 written by the append).  Steps their chain of slots, rows and stores: 256 rows x 16 heads 3.6
 // and 3.2 us, 4 x 12 2.8 both.
 #include <stdio.h>
 
@@ -111,14 +111,6 @@ __device__ __forceinline__ uint32_t of_neighbour(uint32_t x) {
   return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, DPP_QUAD_XOR1, 0xF, 0xF, false);
 }
 
-// Which of a wave's groups a lane has.  STEP: groups 32 w .. of one token; else groups 2 w and
-// 2 w + 1 of 16 tokens.
-struct Unit {
-  int token, hg;  // hg: head * G + group, or past the last
-  int64_t slot;   // -1: none
-  bool full;      // the wave's tokens fill a part in order (wave-uniform)
-};
-
 constexpr int CACHE4_NT = 256;
 
 // Waves of a launch: token windows by groups, K and V each.
@@ -150,8 +142,10 @@ struct Window {
   }
 };
 
-// Calls `body(token, hg, slot, whole)` for a lane's groups; whole: the wave's 16 tokens are a
-// part (a wave-uniform compile-time flag).
+// Calls `body(token, hg, slot, in, whole)` for a lane's groups: head and group hg = h * G + g of
+// `token` (its own only where `in`), whose slot is `slot` (-1: none).  STEP: 32 groups of one token a
+// wave; else two groups of 16 tokens.  whole: the wave's 16 tokens are a part (a wave-uniform
+// compile-time flag).
 template <bool STEP, typename F>
 __device__ __forceinline__ void for_units(const Cache4Args &a, int64_t w, F body) {
   const int lane = __lane_id(), HG = a.H * a.G;
@@ -323,10 +317,11 @@ __global__ __launch_bounds__(CACHE4_NT) void gather_4bit_kernel(Cache4Args a, in
 
 // A decode step's tokens lie in parts of their own: a wave a token and 32 groups.  A prompt's fill
 // parts.  The host does not see which they are: calls of up to 512 tokens (the most rows of a
-// step that the projections take) are taken for steps.  16 heads of 64, us, written / read, as a step
-// against as a prompt: 256 rows 3.66 / 3.12 against 4.05 / 3.24, 512 4.52 / 3.31 against 4.86 / 3.51;
-// a prompt of 512 4.21 / 3.30 against 2.99 / 3.21, of 590 4.84 / 3.77 against 3.11 / 3.40, eight of
-// 590 18.3 / 11.6 against 7.0 / 8.2: a larger call would cost a prompt more than it gives a step.
+// step that the projections take) are taken for steps, since a step's call comes for every token
+// generated and a prompt's once a request.  16 heads of 64, us, written / read, as a step against as
+// a prompt: 256 rows 3.66 / 3.12 against 4.05 / 3.24, 512 4.52 / 3.31 against 4.86 / 3.51; a prompt
+// of 512 loses what three or four steps gain, 4.21 / 3.30 against 2.99 / 3.21; of 590 it would be
+// 4.84 / 3.77 against 3.11 / 3.40, and eight of 590 18.3 / 11.6 against 7.0 / 8.2.
 inline bool is_step(int64_t T) { return T <= 512; }
 
 template <bool APPEND>
