@@ -18,12 +18,14 @@
 //
 // What bounds it: HBM, after the launch and five dependent loads (arguments, order, group, length
 // and block ids, pages) that every workgroup waits for.  64 groups of 4 rows x 16 heads of 64, 256 to
-// 1024 tokens: 13.6 us for 45.5 MB, which a large copy moves in 8.9; 93 single rows to 1000 tokens,
-// fp16, 14.9 us for 51 MB; 2 rows of 17001 and 39999 tokens x 8 heads of 128 17.8 us for 62 MB, 3.8 of
-// them the join.  Nearly all of a launch's pages are on their way at once.  The vector units are busy
-// for 8.2 us of the first (5.06 M quad cycles over 1024 SIMDs at 2.4 GHz: about 64 conversions, 32
-// operations that pair V's tokens, 8 exponentials a 64 tokens of 64 dims, a third of what 16-column
-// tiles would take with 12 columns empty), the matrix units for 1.7.
+// 1024 tokens: 13.8 us for 45.5 MB, which a large copy moves in 8.9; 93 single rows to 1000 tokens,
+// fp16, 15.0 us for 51 MB; 2 rows of 17001 and 39999 tokens x 8 heads of 128 18.2 us for 62 MB, 3.8 of
+// them the join.  Nearly all of a launch's pages are on their way at once (16 waves a CU of two
+// buffers of 4.3 KB: 36 MB), so what is left is the chain and the contexts' unequal lengths: four
+// steps of 64 tokens a wave for the longest, 2.5 on average.  The vector units are busy for 8.3 us of
+// the first (5.09 M quad cycles over 1024 SIMDs at 2.4 GHz: about 64 conversions, 32 operations that
+// pair V's tokens, 8 exponentials a 64 tokens of 64 dims, a third of what 16-column tiles would take
+// with 12 columns empty), the matrix units for 1.7.
 // Pages are read once a launch: non-temporal loads (13.6 against 14.8 us).
 #include <math.h>
 #include <stdio.h>
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(attn4_threads<G>()) void attention_4bit_kernel(Attn
     };
 
     // the next 64 tokens' loads go out before the current ones are used, but for wide heads, whose
-    // second buffer does not fit the registers (64 rows x 8 heads of 256 29.9 us, with it 39.9)
+    // second buffer does not fit the registers (64 rows x 8 heads of 256 23.7 us, with it 32.6)
     constexpr bool AHEAD = G <= 4;
     if (count > 0) {
       Chunk<G> x;

@@ -9,21 +9,24 @@
 // in LDS as it came, key by key, and is turned by the transposing reads.
 //
 // 16-bit inputs go in as they are, the weights rounded to that type (fp16's times 2^7, which
-// keeps those down to 2^-21 of the reference clear of its subnormals; the others' times 2^-20).
-// Their sum is that of the rounded weights, so an output's error is up to about 1.4 of its own
-// rounding's, two errors of a size.  A second term of a weight would take that away, at 2 to 16%
-// (8 runs of 60 to 128 queries 13.5 / 15.7 us, 21 and 29 over 17001 and 39999 keys 48.9 / 50.3).
+// keeps those down to 2^-20 of the reference clear of its subnormals; the others' times 2^-20).
+// Their sum is that of the rounded weights.  An output is off by up to half an eps of its type times
+// sum p |v| beside its own rounding: of random values 1.35 of that alone in the 2-norm (0.0023 for
+// 0.0017 in bf16), where positive and negative ones cancel more.  A second term of a weight would
+// take that away, at 2 to 16% (8 runs of 60 to 128 queries 13.5 / 15.7 us, 21 and 29 over 17001
+// and 39999 keys 48.9 / 50.3).
 // fp32 goes in as three bf16 terms each, rounded, of whose nine products the six largest are taken:
 // the others are 2^-26 of the whole or less.  An infinity has no such terms and makes NaN of its
 // scores or sums: those scores are taken again from the fp32 elements, and of those sums the
 // infinite values alone count.
 //
-// What bounds it: long texts the vector and matrix units together (64 texts of 128 to 1024 tokens
-// over 256 to 1024, 16 heads of 64, bf16: 161 us, 94 GFLOP, 585 TFLOP/s of a large matrix product's
-// 1205; vector units busy for 65 us, matrix units for 40, at 2.4 GHz, in three waves a SIMD.  Copies
-// that left work out: without loading tiles 134, nor storing them 118, nor exponentials 108).  fp32
-// its six products (4 texts of 1024 over 1024 105 us, 980 TFLOP/s of bf16 products; 16 of 31 to 257
-// over 256 to 1024, whose workgroups are one round of unequal length, 65).  Few queries HBM: 64
+// What bounds it: long texts no unit alone (64 texts of 128 to 1024 tokens over 256 to 1024, 16
+// heads of 64, bf16: 157 us, 94 GFLOP, 600 TFLOP/s of a large matrix product's 1205; vector units busy
+// for 65 us, matrix units for 40, at 2.4 GHz, in three waves a SIMD; each operand read from LDS feeds
+// one product, 3 GB in 12 reads for 8 products, 39 us at 128 bytes a clock, and 10 of bank conflicts.
+// Copies that left work out: without loading tiles 134, nor storing them 118, nor exponentials 108).
+// fp32 its six products (4 texts of 1024 over 1024 105 us, 980 TFLOP/s of bf16 products; 16 of 31 to
+// 257 over 256 to 1024, whose workgroups are one round of unequal length, 67).  Few queries HBM: 64
 // single tokens over 256 to 1024 keys 35 us, 4.8 TB/s; 21 and 29 over 17001 and 39999, heads of 128,
 // fp16, 56 us, 4.1 TB/s (46 to 49 where the last call left some of the keys in the cache).
 // What the steps gave, us, these long texts / fp32 / long keys in the cache / 9 over 590:
