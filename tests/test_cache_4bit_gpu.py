@@ -629,3 +629,47 @@ def test_either_binding(monkeypatch):
     want = step()
     monkeypatch.setattr(hip_attn, "calls", lib)
     assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,groups", [([70, 300], [4, 3]), ([300, 70], [8, 1]), ([6000], None)])
+def test_attention_nan_query_stays_in_its_row(dtype, lens, groups):
+    gen = torch.Generator().manual_seed(33)
+    cache = random_cache(gen, 400, 2, 16, 64)
+    tables = [torch.randperm(400, generator=gen)[: -(-n // 16)].tolist() for n in lens]
+    rows = [g for g, n in enumerate(groups or [1] * len(lens)) for _ in range(n)]
+    args = ([lens[g] for g in rows], [tables[g] for g in rows], 0.125)
+    query = queries(gen, len(rows), 2, 64, dtype)
+    want = run_attention(query, cache, *args, groups=groups)
+    for bad in (math.nan, math.inf):
+        query[0, 1, 5] = bad
+        out = run_attention(query, cache, *args, groups=groups)
+        assert out[0, 1].isnan().all()
+        out[0, 1] = want[0, 1]
+        assert torch.equal(out, want)
+
+
+def test_values_of_a_device_cache():
+    from vflorence_amd import hip_attn
+
+    cache = random_cache(torch.Generator().manual_seed(34), 5, 3, 32, 96)
+    for a, b in zip(hip_attn.kv_cache_4bit_values(cache, 96), values_of(cache, 96)):
+        assert a.is_cuda and same(a, b)
+
+
+def test_two_streams_at_once():
+    """Calls that split their contexts, on two streams at once, have parts of their own."""
+    gen = torch.Generator().manual_seed(35)
+    cache = random_cache(gen, 400, 2, 16, 64)
+    tables = [torch.randperm(400, generator=gen)[:375].tolist()]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    query = [queries(gen, 1, 2, 64, torch.bfloat16) for _ in streams]
+    want = [run_attention(q, cache, [6000], tables, 0.125) for q in query]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for q, s in zip(query, streams):
+            with torch.cuda.stream(s):
+                got.append(run_attention(q, cache, [6000], tables, 0.125))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -12,8 +12,8 @@ from tests.test_cross_attention_gpu import DEV, inputs, run
 pytestmark = pytest.mark.gpu
 
 # heads of one to eight 32 dims, runs in one part and in several, in one key group and in more
-SHAPES = [(32, 100), (64, 100), (64, 2500), (96, 300), (128, 2500), (160, 70), (256, 100),
-          (256, 1300)]
+SHAPES = [(32, 100), (48, 300), (64, 100), (64, 2500), (80, 2500), (96, 300), (128, 2500),
+          (160, 70), (224, 100), (256, 100), (256, 1300)]
 
 
 def as_defined(out, infinite, starts, keys, finite, finite_keys, scale=0.125):

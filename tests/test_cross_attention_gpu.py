@@ -315,3 +315,39 @@ def test_refuses_its_keys_or_values_as_the_output():
     # (no queries, or no keys, no address to share)
     run(q[:0], k, v, [0, 0], [0, 40], 0.125)
     run(q, k[:0], v[:0], [0, 40], [0, 0], 0.125)
+
+
+@pytest.mark.parametrize("sequences", [63, 64, 127, 300, 3969, 3970, 5000])
+@pytest.mark.parametrize("longest", [(3, 5), (200, 90)])
+def test_many_sequences(sequences, longest):
+    """More than a wave looks up at a time, once and twice over, empty ones among them."""
+    gen = torch.Generator().manual_seed(sequences)
+    queries = torch.randint(0, 4, (sequences,), generator=gen)
+    keys = torch.randint(0, 6, (sequences,), generator=gen)
+    queries[torch.rand(sequences, generator=gen) < 0.3] = 0
+    queries[sequences // 2], keys[sequences // 2] = longest[0], longest[1]
+    queries[-1], keys[0] = longest[0], longest[1]
+    queries, keys = queries.tolist(), keys.tolist()
+    q, k, v = inputs(gen, queries, keys, 1, 32, torch.bfloat16)
+    check(q, k, v, starts_of(queries), starts_of(keys), 0.2)
+
+
+def test_rows_far_apart():
+    """Queries, keys and values whose last rows lie past 2^31 elements."""
+    gen = torch.Generator().manual_seed(23)
+    rows, step = 70000, 32768  # 2.3e9 elements
+    base = torch.zeros(rows, step, dtype=torch.bfloat16, device=DEV)
+    q, k, v = (base[:, a: a + 64].view(rows, 1, 64) for a in (0, 64, 128))
+    at = [0, 5, rows - 300, rows - 40, rows]
+    for x in (q, k, v):
+        for a, b in ((0, 5), (rows - 300, rows)):
+            x[a:b] = torch.randn(b - a, 1, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    out = run(q, k, v, at, at, 0.125)
+    tail = [x[rows - 300:].contiguous() for x in (q, k, v)]
+    found = cross(*tail, [0, 260, 300], [0, 260, 300], 0.125)
+    limit = cross_tolerance(torch.bfloat16, 64, 260, *found)
+    assert bool(((out[rows - 300:].double().cpu() - found[0]).abs() <= limit).all())
+    found = cross(*(x[:5].contiguous() for x in (q, k, v)), [0, 5], [0, 5], 0.125)
+    limit = cross_tolerance(torch.bfloat16, 64, 5, *found)
+    assert bool(((out[:5].double().cpu() - found[0]).abs() <= limit).all())
+    assert not out[5: rows - 300].any()
